@@ -1,0 +1,379 @@
+"""Timed cases of the 4-bit key/value cache: writing rows into it, reading rows
+back, and attention over it.
+
+The cache is paged. A page holds `page` tokens of every kv head; sequence s
+finds its pages in row s of a table. A batch's rows are ragged: rows
+starts[s] .. starts[s+1] - 1 belong to sequence s and are its last positions,
+so row i of its n is at position lens[s] - n + i. A row attends to the
+positions up to its own, the last `window` of them where a window is set.
+
+Values are held in blocks of 32 dimensions of one token and head, as a scale d
+and 32 codes c in 0..15 that stand for (c - 8) d. With m the block's value of
+largest magnitude (the positive one of a tie), NaN taken as 0 and values
+limited to 65280 either way, d = -m / 8 is rounded to 8 significant bits and
+to fp16's exponents, and c - 8 = x / d rounded to the nearest (ties to even)
+within -8 .. 7.
+
+Bytes of 32 tokens (a group) of one head, from which a page is made head by
+head: K codes, V codes (16 hd bytes each), K scales, V scales (fp16, 2 hd
+bytes each); the order inside is written down at `_order`.
+"""
+import functools
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+DEV = "cuda"
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def listed():
+    return [
+        # a decode step of eight sequences at a context of 32768 stores its
+        # token (8 kv heads of 64): latency alone
+        dict(name="write_step_8", kind="write", type="f32", seqs=8, kv=8, hd=64, page=64, rows=1, lo=32768, hi=32768),
+        # the second 2048-row pass of a 4096-token prompt
+        dict(name="write_tile_2048", kind="write", type="f32", seqs=1, kv=8, hd=64, page=64, rows=2048, lo=4096, hi=4096),
+        # prompts of a serving batch, of odd lengths, K and V parts of one
+        # fused projection
+        dict(name="write_ragged_bf16", kind="write", type="bf16", seqs=24, kv=8, hd=128, page=128, rows=701, lo=701, hi=2309),
+        # a prompt's rows taken out for a prefix store
+        dict(name="read_prefix_4096", kind="read", type="f32", seqs=1, kv=8, hd=64, page=64, rows=4096, lo=4096, hi=4096),
+        # eight whole caches widened to fp16 (a session moved to another cache)
+        dict(name="read_8x32768_f16", kind="read", type="f16", seqs=8, kv=8, hd=64, page=256, rows=32768, lo=32768, hi=32768),
+        # single tokens: the 1.2B model's attention layer at batch 1
+        dict(name="step_1x4096", kind="attend", type="f32", seqs=1, heads=32, kv=8, hd=64, page=64, rows=1, lo=4096, hi=4096, window=0),
+        # and at batch 8 with long contexts
+        dict(name="step_8x32768", kind="attend", type="f32", seqs=8, heads=32, kv=8, hd=64, page=64, rows=1, lo=32768, hi=32768, window=0),
+        # a serving batch of single tokens, contexts from one token on
+        dict(name="step_64_ragged_bf16", kind="attend", type="bf16", seqs=64, heads=32, kv=8, hd=128, page=64, rows=1, lo=1, hi=8192, window=0),
+        # seven query heads a kv head, 96 dimensions, a sliding window
+        dict(name="step_window_f16", kind="attend", type="f16", seqs=5, heads=28, kv=4, hd=96, page=32, rows=1, lo=3000, hi=20011, window=4097),
+        # drafted tokens verified, up to five a sequence
+        dict(name="verify_16x5_bf16", kind="attend", type="bf16", seqs=16, heads=32, kv=4, hd=128, page=64, rows=5, lo=4001, hi=12000, window=0),
+        # the second 2048-row pass of a 4096-token prompt
+        dict(name="tile_2048_f32", kind="attend", type="f32", seqs=1, heads=32, kv=8, hd=64, page=64, rows=2048, lo=4096, hi=4096, window=0),
+        # long prompts in passes of up to 2048 rows, two sequences
+        dict(name="prompt_2x32768_bf16", kind="attend", type="bf16", seqs=2, heads=32, kv=8, hd=128, page=128, rows=2048, lo=30001, hi=32768, window=0),
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(("write", "read", "attend", "attend", "attend"))
+    c = dict(kind=kind, type=rng.choice(("f32", "f16", "bf16")), kv=rng.choice((1, 2, 3, 4, 8)),
+             hd=rng.choice((32, 64, 64, 96, 128, 128, 192, 256)), page=rng.choice((32, 64, 96, 128, 256)))
+    if kind != "attend":
+        c["seqs"] = _log(rng, 1, 64)
+        c["rows"] = _log(rng, 1, max(1, 32768 // c["seqs"]))
+        c["lo"] = c["rows"]
+        c["hi"] = c["rows"] + _log(rng, 1, max(1, 65536 // c["seqs"]))
+        return c
+    c["heads"] = c["kv"] * rng.choice((1, 2, 3, 4, 6, 7, 8))
+    form = rng.choice(("step", "step", "few", "many"))
+    c["seqs"] = _log(rng, 1, 64 if form != "many" else 6)
+    c["rows"] = 1 if form == "step" else _log(rng, 2, 16) if form == "few" else _log(rng, 17, 2048 // c["seqs"])
+    c["hi"] = c["rows"] + _log(rng, 1, (262144 if form == "step" else 131072 if form == "few" else 32768) // c["seqs"])
+    c["lo"] = rng.choice((0, c["rows"], c["hi"]))
+    c["window"] = _log(rng, 1, c["hi"]) if rng.random() < 0.25 else 0
+    return c
+
+
+def _shape(case):
+    """(rows, lengths) of the sequences: the same for every seed of a case. A
+    batch whose rows are more than one and whose lengths differ is ragged in
+    its rows too; a length under the row count leaves the rows before the
+    sequence's start without a position."""
+    r = np.random.RandomState(case["seqs"] * 7919 + case["rows"] * 31 + case["hi"])
+    s = case["seqs"]
+    lens = r.randint(case["lo"], case["hi"] + 1, s)
+    lens[0] = case["hi"]
+    rows = r.randint(max(1, case["rows"] // 2), case["rows"] + 1, s) if case["lo"] != case["hi"] else np.full(s, case["rows"])
+    rows[0] = case["rows"]
+    if case["lo"] >= case["rows"]:
+        lens = np.maximum(lens, rows)
+    return rows.astype(np.int64), lens.astype(np.int64)
+
+
+def work(case):
+    rows, lens = _shape(case)
+    kv, hd, e = case["kv"], case["hd"], TYPES[case["type"]].itemsize
+    if case["kind"] != "attend":
+        n = int(rows.sum()) * kv
+        held = n * hd * 36 // 32
+        # a write goes through the cache: values in, codes out, codes in, values out
+        return dict(bytes=n * 2 * hd * e * (2 if case["kind"] == "write" else 1) + held * (2 if case["kind"] == "write" else 1),
+                    flops=n * 2 * hd)
+    w = case["window"]
+    seen = pairs = 0
+    for n, t in zip(rows.tolist(), lens.tolist()):
+        first = max(0, t - n)
+        seen += t - (max(0, first + 1 - w) if w else 0)
+        p = np.arange(first, t, dtype=np.int64) + 1
+        pairs += int((np.minimum(p, w) if w else p).sum())
+    return dict(bytes=seen * kv * hd * 36 // 32 + int(rows.sum()) * case["heads"] * hd * e * 2, flops=4 * hd * case["heads"] * pairs)
+
+
+@functools.lru_cache(maxsize=None)
+def _order(hd):
+    """Where a group keeps its codes and scales: for token t and dimension d,
+    the byte and shift of the K code and of the V code, and for token t and
+    block b the fp16 index of the K scale and of the V scale."""
+    t, d = np.arange(32)[:, None], np.arange(hd)[None, :]
+    blocks = hd // 32
+    b, i = d // 32, d % 32
+
+    def at(b, lane):  # 8 bytes a block and lane, two blocks side by side where there are two
+        pair = b // 2 < blocks // 2
+        return np.where(pair, b // 2 * 1024 + lane * 16 + b % 2 * 8, b // 2 * 1024 + lane * 8)
+
+    # K: lane = token mod 16 and the block's quarter; a dword a half of the
+    # group, its 8 dimensions even ones in the low half, odd ones in the high
+    e = i % 8
+    nib = e // 2 + 4 * (e % 2)
+    k_byte = at(b, t % 16 + 16 * (i // 8)) + t // 16 * 4 + nib // 2
+    k_shift = nib % 2 * 4 + 0 * t
+    # V: lane = dimension mod 16 and the token's quarter; a byte a token, the
+    # low nibble the block's first 16 dimensions, the high one its last
+    byte = np.array([0, 2, 1, 3])[t % 4]
+    v_byte = 16 * hd + at(b, i % 16 + 16 * (t % 16 // 4)) + t // 16 * 4 + byte
+    v_shift = i // 16 * 4 + 0 * t
+    bb = np.arange(blocks)[None, :]
+    k_scale = 16 * hd + t % 16 * 2 * blocks + t // 16 * blocks + bb
+    v_scale = 17 * hd + bb * 32 + t % 16 // 4 * 8 + t // 16 * 4 + t % 4
+    cuda = lambda a: torch.from_numpy(np.ascontiguousarray(a).astype(np.int64)).to(DEV)  # noqa: E731
+    return tuple(cuda(np.broadcast_to(a, (32, hd))) for a in (k_byte, k_shift, v_byte, v_shift)) + (cuda(k_scale), cuda(v_scale))
+
+
+def _quantise(x):
+    """Codes and scales of x[..., hd]."""
+    x = torch.nan_to_num(x.float(), nan=0.0, posinf=65280.0, neginf=-65280.0).clamp(-65280.0, 65280.0)
+    x = x.reshape(*x.shape[:-1], -1, 32).double()
+    hi, lo = x.amax(-1), x.amin(-1)
+    d = (torch.where(hi >= -lo, hi, lo) / -8).clamp(-8160.0, 8160.0).float().to(torch.bfloat16).to(torch.float16)
+    # 64 bits: a quotient next to a half goes the right way
+    w = d.double().unsqueeze(-1)
+    c = torch.where(w == 0, 0.0, (x / torch.where(w == 0, 1.0, w)).round().clamp(-8, 7)) + 8
+    return c.to(torch.uint8).flatten(-2), d
+
+
+def _write(s, k, v):
+    c = s["case"]
+    order = _order(c["hd"])
+    page, group, token = s["row_page"], s["row_group"], s["row_token"]
+    heads = torch.arange(c["kv"], device=DEV)
+    cells = s["cache"].view(-1, c["kv"], c["page"] // 32, 36 * c["hd"])
+    at = (page[:, None, None], heads[None, :, None], group[:, None, None])
+    for x, byte, shift, scale in ((k, order[0], order[1], order[4]), (v, order[2], order[3], order[5])):
+        codes, d = _quantise(x)
+        low = torch.argsort(byte[0] * 2 + shift[0] // 4)  # the byte's low nibble and its high one, in turn
+        pairs = codes[..., low].view(*codes.shape[:2], -1, 2)
+        cells[(*at, byte[:, low[::2]][token][:, None, :])] = pairs[..., 0] | pairs[..., 1] << 4
+        cells.view(torch.float16)[(*at, scale[token][:, None, :])] = d
+
+
+def _values(groups, hd):
+    """K and V of groups [..., 36 hd] as [..., 32, hd] in 32 bits."""
+    order = _order(hd)
+    halves = groups.view(torch.float16)
+
+    def side(byte, shift, scale):
+        codes = groups[..., byte] >> shift.to(torch.uint8) & 15
+        return (codes.float() - 8) * halves[..., scale].float().repeat_interleave(32, -1)
+    return side(*order[:2], order[4]), side(*order[2:4], order[5])
+
+
+def _read(s):
+    c = s["case"]
+    page, group, token = s["row_page"], s["row_group"], s["row_token"]
+    cells = s["cache"].view(-1, c["kv"], c["page"] // 32, 36 * c["hd"])
+    order = _order(c["hd"])
+    heads = torch.arange(c["kv"], device=DEV)[None, :, None]
+    at = (page[:, None, None], heads, group[:, None, None])
+
+    def side(byte, shift, scale):
+        codes = cells[(*at, byte[token][:, None, :])] >> shift[token][:, None, :].to(torch.uint8) & 15
+        d = cells.view(torch.float16)[(*at, scale[token][:, None, :])].float()
+        return ((codes.float() - 8).unflatten(-1, (-1, 32)) * d.unsqueeze(-1)).flatten(-2).to(TYPES[c["type"]])
+    return side(*order[:2], order[4]), side(*order[2:4], order[5])
+
+
+def _attend(s):
+    c = s["case"]
+    n, kv, hd, g = c["seqs"], c["kv"], c["hd"], c["heads"] // c["kv"]
+    cells = s["cache"].view(-1, kv, c["page"] // 32, 36 * hd)
+    k, v = _values(cells[s["pages"].long()].transpose(1, 2).flatten(2, 3), hd)  # [n, kv, groups, 32, hd]
+    k, v = k.flatten(2, 3), v.flatten(2, 3)
+    starts, lens = s["starts"].long(), s["lens"].long()
+    r = torch.arange(c["rows"], device=DEV)
+    count = starts[1:] - starts[:-1]
+    real = r[None, :] < count[:, None]
+    q = s["q"].float()[(starts[:-1, None] + r).clamp(max=s["q"].shape[0] - 1)]  # [n, rows, heads, hd]
+    q = q.view(n, -1, kv, g, hd).permute(0, 2, 3, 1, 4).reshape(n, kv, -1, hd)
+    scores = torch.matmul(q, k.transpose(-1, -2)).mul_(1 / math.sqrt(hd)).view(n, kv, g, c["rows"], -1)
+    pos = (lens - count)[:, None] + r
+    t = torch.arange(k.shape[2], device=DEV)
+    seen = t <= pos[..., None]
+    if c["window"]:
+        seen &= t > pos[..., None] - c["window"]
+    scores.masked_fill_(~seen[:, None, None], -math.inf)
+    top = scores.amax(-1, keepdim=True)
+    scores.sub_(torch.where(top == -math.inf, 0.0, top)).exp_()
+    total = scores.sum(-1, keepdim=True)
+    out = torch.matmul(scores.view(n, kv, g * c["rows"], -1), v).view(n, kv, g, c["rows"], hd)
+    out = out / torch.where(total == 0, 1.0, total)  # a row that sees nothing is zero
+    return out.permute(0, 3, 1, 2, 4).flatten(2, 3)[real].to(TYPES[c["type"]])
+
+
+def prepare(case, seed):
+    rng = np.random.RandomState(seed)
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    kv, hd, page, dt = case["kv"], case["hd"], case["page"], TYPES[case["type"]]
+    rows, lens = _shape(case)
+    starts = np.concatenate([[0], np.cumsum(rows)])
+    per = max(1, -(-int(lens.max()) // page))
+    table = rng.permutation(case["seqs"] * per + 3)[:case["seqs"] * per].reshape(case["seqs"], per)
+    n = int(starts[-1])
+    s = dict(case=dict(case), pages=torch.from_numpy(table.astype(np.int32)).to(DEV),
+             starts=torch.from_numpy(starts.astype(np.int32)).to(DEV), lens=torch.from_numpy(lens.astype(np.int32)).to(DEV))
+    total = case["seqs"] * per + 3
+    bytes_ = total * page // 32 * kv * 36 * hd
+    s["cache"] = torch.randint(0, 256, (bytes_,), dtype=torch.uint8, device=DEV, generator=gen)
+    # a used cache: codes of bell-shaped values, scales as blocks of 32 such values have
+    cells = s["cache"].view(-1, 36 * hd)
+    a, b = (torch.randint(0, 256, (cells.shape[0], 32 * hd), dtype=torch.uint8, device=DEV, generator=gen) & 0x77 for _ in range(2))
+    cells[:, :32 * hd] = (cells[:, :32 * hd] & 0x11) + a + b
+    del a, b
+    d = (0.26 + 0.05 * torch.randn((cells.shape[0], 2 * hd), device=DEV, generator=gen)).abs()
+    d *= torch.randint(0, 2, d.shape, device=DEV, generator=gen) * 2 - 1
+    cells.view(torch.float16)[:, 16 * hd:] = d.to(torch.bfloat16).to(torch.float16)
+    del d
+    if case["kind"] == "attend":
+        # the query part of a fused projection: rows further apart than they are long
+        heads = case["heads"]
+        s["q"] = (3 * torch.randn((n, heads + 2 * kv, hd), device=DEV, generator=gen)).to(dt)[:, :heads]
+        return s
+    owner = np.repeat(np.arange(case["seqs"]), rows)
+    pos = lens[owner] - rows[owner] + np.arange(n) - starts[owner]
+    cuda = lambda a: torch.from_numpy(np.ascontiguousarray(a).astype(np.int64)).to(DEV)  # noqa: E731
+    s["row_page"], s["row_group"], s["row_token"] = cuda(table[owner, pos // page]), cuda(pos % page // 32), cuda(pos % 32)
+    if case["kind"] == "write":
+        x = torch.randn((n, 2 * kv, hd), device=DEV, generator=gen)
+        x *= 0.5 + torch.rand((2 * kv, hd), device=DEV, generator=gen) * 2  # channels of different spread
+        x = x.to(dt)
+        s["k"], s["v"] = x[:, :kv], x[:, kv:]
+    return s
+
+
+def run(s):
+    c = s["case"]
+    if not own:
+        if c["kind"] == "write":
+            _write(s, s["k"], s["v"])
+        return dict(zip("kv", _read(s))) if c["kind"] != "attend" else dict(out=_attend(s))
+    import_path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mivi-v4_amd")
+    if import_path not in sys.path:
+        sys.path.insert(0, import_path)
+    import mivi_hip
+    if "handle" not in s:  # names the user's own tensors, once
+        s["handle"] = mivi_hip.KvCacheQ4(s["cache"], s["pages"], c["kv"], c["hd"], c["page"])
+    cache = s["handle"]
+    if c["kind"] == "attend":
+        q = s["q"]
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        mivi_hip.kv_q4_attention(out, q, cache, s["starts"], s["lens"], c["rows"], 1 / math.sqrt(c["hd"]), c["window"])
+        return dict(out=out)
+    n = s["row_page"].numel()
+    k, v = (torch.empty((n, c["kv"], c["hd"]), dtype=TYPES[c["type"]], device=DEV) for _ in range(2))
+    if c["kind"] == "write":
+        mivi_hip.kv_q4_append(cache, s["k"], s["v"], s["starts"], s["lens"])
+    mivi_hip.kv_q4_read(cache, k, v, s["starts"], s["lens"])
+    return dict(k=k, v=v)
+
+
+def _held(s, seq, count):
+    """K and V [kv, count, hd] of a sequence's first positions in 64 bits,
+    taken apart from the bytes by views."""
+    c = s["case"]
+    hd, blocks, gpp = c["hd"], c["hd"] // 32, c["page"] // 32
+    raw = s["cache"].view(-1, c["kv"], gpp, 36 * hd)[s["pages"][seq].long()]
+    raw = raw.transpose(0, 1).reshape(c["kv"], -1, 36 * hd)[:, :-(-count // 32)]
+
+    def cut(x):  # [kv, groups, block, lane 16 x quarter 4, 8 bytes]
+        two = blocks // 2 * 1024
+        a = x[..., :two].unflatten(-1, (blocks // 2, 4, 16, 2, 8)).permute(0, 1, 2, 5, 3, 4, 6).flatten(2, 3) if two else None
+        b = x[..., two:].unflatten(-1, (1, 4, 16, 8)) if blocks % 2 else None
+        return a if b is None else b if a is None else torch.cat([a, b], 2)
+
+    k = cut(raw[..., :16 * hd])  # quarter of the dimensions, token of 16, (half, 4 bytes)
+    k = k.unflatten(-1, (2, 4))
+    lo, hi = k & 15, k >> 4
+    e = torch.stack([lo[..., 0], lo[..., 2], hi[..., 0], hi[..., 2], lo[..., 1], lo[..., 3], hi[..., 1], hi[..., 3]], -1)
+    k = e.permute(0, 1, 5, 4, 2, 3, 6).reshape(c["kv"], -1, 32, hd)  # half, token, block, quarter, 8
+    v = cut(raw[..., 16 * hd:32 * hd])  # quarter of the tokens, dimension of 16, (half, 4 tokens)
+    v = v.unflatten(-1, (2, 4))[..., [0, 2, 1, 3]]
+    v = torch.stack([v & 15, v >> 4], 3)  # [kv, g, block, 2, quarter, dim, half, 4]... the dimension's half at 3
+    v = v.permute(0, 1, 6, 4, 7, 2, 3, 5).reshape(c["kv"], -1, 32, hd)
+    sc = raw[..., 32 * hd:].contiguous().view(torch.float16).double()
+    ks = sc[..., :hd].unflatten(-1, (16, 2, blocks)).transpose(2, 3).reshape(c["kv"], -1, 32, blocks)
+    vs = sc[..., hd:].unflatten(-1, (blocks, 4, 2, 4)).permute(0, 1, 4, 3, 5, 2).reshape(c["kv"], -1, 32, blocks)
+
+    def mul(codes, d):
+        return ((codes.double() - 8).unflatten(-1, (blocks, 32)) * d[..., None]).flatten(-2).flatten(1, 2)[:, :count]
+    return mul(k, ks), mul(v, vs)
+
+
+def _nearest(x):
+    """The values that x[n, kv, hd] is held as, in 64 bits, from the definition."""
+    x = x.double()
+    x = torch.where(torch.isnan(x), 0.0, x).clamp(-65280, 65280).unflatten(-1, (-1, 32))
+    big = x.abs().amax(-1)
+    m = torch.where((x == big[..., None]).any(-1), big, -big)
+    y = (-m / 8).clamp(-8160, 8160)
+    y = torch.where(y.abs() < 2.0 ** -40, 0.0, y)  # far below fp16
+    part = torch.frexp(y).mantissa  # y by its part in [0.5, 1) is a power of two, exactly
+    d = torch.where(y == 0, 0.0, (part * 256).round() / 256 * (y / torch.where(y == 0, 1.0, part)))
+    d = torch.where(d.abs() < 2.0 ** -14, (d * 2.0 ** 24).round() / 2.0 ** 24, d)[..., None]
+    n = torch.where(d == 0, 0.0, (x / torch.where(d == 0, 1.0, d)).round().clamp(-8, 7))
+    return (n * d).flatten(-2)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    rows, lens = (x.tolist() for x in _shape(case))
+    if case["kind"] == "write":
+        return dict(k=_nearest(s["k"]), v=_nearest(s["v"]))
+    outs = []
+    first = 0
+    for i, (n, t) in enumerate(zip(rows, lens)):
+        if t == 0:
+            outs.append(torch.zeros((n, case["heads"], case["hd"]), dtype=torch.float64, device=DEV))
+            first += n
+            continue
+        k, v = _held(s, i, t)
+        if case["kind"] == "read":
+            outs.append((k[:, t - n:].transpose(0, 1), v[:, t - n:].transpose(0, 1)))
+            continue
+        g = case["heads"] // case["kv"]
+        q = s["q"][first:first + n].double().unflatten(1, (case["kv"], g))
+        p, at = torch.arange(t - n, t, device=DEV)[:, None], torch.arange(t, device=DEV)
+        hide = (at > p) | (at <= p - case["window"]) if case["window"] else at > p
+        out = torch.zeros((n, case["kv"], g, case["hd"]), dtype=torch.float64, device=DEV)
+        for h in range(case["kv"]):
+            for j in range(g):
+                w = (q[:, h, j] @ k[h].T / math.sqrt(case["hd"])).masked_fill(hide, -math.inf)
+                w = torch.softmax(w, -1)
+                out[:, h, j] = torch.nan_to_num(w, nan=0.0) @ v[h]  # no position: nothing
+        outs.append(out.flatten(1, 2))
+        first += n
+    if case["kind"] == "read":
+        return dict(k=torch.cat([o[0] for o in outs]), v=torch.cat([o[1] for o in outs]))
+    return dict(out=torch.cat(outs))

@@ -10,7 +10,7 @@ positions up to its own, the last `window` of them where a window is set.
 Values are held in blocks of 32 dimensions of one token and head, as a scale d
 and 32 codes c in 0..15 that stand for (c - 8) d. With m the block's value of
 largest magnitude (the positive one of a tie), NaN taken as 0 and values
-limited to 65280 either way, d = -m / 8 is rounded to 8 significant bits and
+limited to 21760 either way, d = -m / 8 is rounded to 8 significant bits and
 to fp16's exponents, and c - 8 = x / d rounded to the nearest (ties to even)
 within -8 .. 7.
 
@@ -155,10 +155,10 @@ def _order(hd):
 
 def _quantise(x):
     """Codes and scales of x[..., hd]."""
-    x = torch.nan_to_num(x.float(), nan=0.0, posinf=65280.0, neginf=-65280.0).clamp(-65280.0, 65280.0)
+    x = torch.nan_to_num(x.float(), nan=0.0, posinf=21760.0, neginf=-21760.0).clamp(-21760.0, 21760.0)
     x = x.reshape(*x.shape[:-1], -1, 32).double()
     hi, lo = x.amax(-1), x.amin(-1)
-    d = (torch.where(hi >= -lo, hi, lo) / -8).clamp(-8160.0, 8160.0).float().to(torch.bfloat16).to(torch.float16)
+    d = (torch.where(hi >= -lo, hi, lo) / -8).clamp(-2720.0, 2720.0).float().to(torch.bfloat16).to(torch.float16)
     # 64 bits: a quotient next to a half goes the right way
     w = d.double().unsqueeze(-1)
     c = torch.where(w == 0, 0.0, (x / torch.where(w == 0, 1.0, w)).round().clamp(-8, 7)) + 8
@@ -334,10 +334,10 @@ def _held(s, seq, count):
 def _nearest(x):
     """The values that x[n, kv, hd] is held as, in 64 bits, from the definition."""
     x = x.double()
-    x = torch.where(torch.isnan(x), 0.0, x).clamp(-65280, 65280).unflatten(-1, (-1, 32))
+    x = torch.where(torch.isnan(x), 0.0, x).clamp(-21760, 21760).unflatten(-1, (-1, 32))
     big = x.abs().amax(-1)
     m = torch.where((x == big[..., None]).any(-1), big, -big)
-    y = (-m / 8).clamp(-8160, 8160)
+    y = (-m / 8).clamp(-2720, 2720)
     y = torch.where(y.abs() < 2.0 ** -40, 0.0, y)  # far below fp16
     part = torch.frexp(y).mantissa  # y by its part in [0.5, 1) is a power of two, exactly
     d = torch.where(y == 0, 0.0, (part * 256).round() / 256 * (y / torch.where(y == 0, 1.0, part)))

@@ -196,6 +196,87 @@ int32_t mivi_hip_dot_q8_0_f32(const float* q, size_t q_len, const uint8_t* k_blo
                               size_t k_len, float* out, size_t out_len, size_t n, void* stream);
 
 /* ---------------------------------------------------------------------
+ * A paged key/value cache held in 4 bits (mivi-kv's place beside the model's
+ * own caches; the reference's 4-bit precisions, crates/mivi-kv/src/cache.rs:5-15,
+ * rotate rows and use code books: no counterpart of these calls there)
+ *
+ * Values: blocks of 32 dimensions of one token and head, a scale d and codes
+ * c in 0..15 standing for (c - 8) d. With m the block's value of largest
+ * magnitude (the positive one of a tie), d = -m / 8 rounded to nearest to 8
+ * significant bits and then to fp16, c - 8 = x / d rounded to nearest (ties to
+ * even) within -8 .. 7. NaN is held as 0 and values past +-21760 as +-21760.
+ * 1.125 bytes a dimension pair (K and V of one dimension).
+ *
+ * `cache`: cache_len / page_bytes pages, 16-byte aligned; a page holds
+ * page_tokens tokens (a multiple of 32, at most 1024) of all n_kv_heads heads
+ * of head_dim (32, 64, 96, 128, 192 or 256). Its inner order is the library's.
+ * `pages`: page ids on the device, n_seq rows of pages_per_seq, pages_stride
+ * apart: token t of sequence s is in page pages[s * pages_stride + t /
+ * page_tokens]. Sequences may share pages that none of them writes.
+ * `starts` [n_seq + 1], `lens` [n_seq] on the device: rows starts[s] ..
+ * starts[s + 1] - 1 of a call's tensors belong to sequence s and are its last
+ * positions: row i of its n is at position lens[s] - n + i (lens counts them).
+ * starts does not decrease. All three are read when the work runs, so a
+ * captured call follows their contents at each replay.
+ *
+ * Positions below 0 or past the table, and ids that are no page of the cache,
+ * are no positions: such rows are not written, read as zeros, and are not
+ * attended to. Rows outside starts[0] .. starts[n_seq] - 1 are left alone.
+ *
+ * Tensors: `type` MIVI_GGML_F32, F16 or BF16, [rows][heads][head_dim] with the
+ * last dimension contiguous and strides in elements; lengths in elements.
+ * Written tensors must not overlap themselves or other arguments. Work is
+ * enqueued on `stream`, of the current device; calls that write and that use
+ * the same page must be ordered. Nothing is allocated: calls may be captured.
+ * ------------------------------------------------------------------- */
+
+/* Bytes of a page; 0 where the geometry is not one of the above. */
+size_t mivi_hip_kv_q4_page_bytes(size_t n_kv_heads, size_t head_dim, size_t page_tokens);
+
+/* Quantises rows of k and v into the cache. */
+int32_t mivi_hip_kv_q4_append(uint8_t* cache, size_t cache_len, size_t n_kv_heads, size_t head_dim,
+                              size_t page_tokens, const int32_t* pages, size_t pages_stride,
+                              size_t pages_per_seq, size_t n_seq, const int32_t* starts,
+                              const int32_t* lens, int32_t type, const void* k, size_t k_len,
+                              size_t k_row_stride, size_t k_head_stride, const void* v, size_t v_len,
+                              size_t v_row_stride, size_t v_head_stride, size_t rows, void* stream);
+
+/* Reads the rows back: the held values, rounded to `type` (exact in F32 and
+ * F16). */
+int32_t mivi_hip_kv_q4_read(const uint8_t* cache, size_t cache_len, size_t n_kv_heads, size_t head_dim,
+                            size_t page_tokens, const int32_t* pages, size_t pages_stride,
+                            size_t pages_per_seq, size_t n_seq, const int32_t* starts,
+                            const int32_t* lens, int32_t type, void* k, size_t k_len,
+                            size_t k_row_stride, size_t k_head_stride, void* v, size_t v_len,
+                            size_t v_row_stride, size_t v_head_stride, size_t rows, void* stream);
+
+/* Bytes of mivi_hip_kv_q4_attention's workspace for batches of up to these
+ * sizes, max_tokens = pages_per_seq * page_tokens (0: none is needed). */
+size_t mivi_hip_kv_q4_attention_workspace(size_t n_seq, size_t rows, size_t max_rows, size_t n_heads,
+                                          size_t n_kv_heads, size_t head_dim, size_t max_tokens);
+
+/* out = softmax(scale q K^T) V for every row and head over the cache, which
+ * holds the rows' own tokens already: a row at position p sees the positions
+ * 0 .. p, or with window > 0 the last `window` of them; query head j reads kv
+ * head j / (n_heads / n_kv_heads). A row that sees nothing is zero. max_rows:
+ * at least the rows of any one sequence; a sequence's rows past it are not
+ * computed. F32 queries and softmax weights enter the products as two fp16
+ * planes (22 bits), F16 and BF16 ones as one (queries exactly, weights to 11
+ * bits); a weight below 2^-29 of its row's largest to 2^-40 of that; sums are
+ * f32. An infinity or NaN in q stays in its row and head.
+ * `workspace`: 16-byte aligned, mivi_hip_kv_q4_attention_workspace bytes for
+ * the call's arguments, in use until the call's work is done; calls that may
+ * overlap need workspaces of their own. */
+int32_t mivi_hip_kv_q4_attention(int32_t type, void* out, size_t out_len, size_t out_row_stride,
+                                 size_t out_head_stride, const void* q, size_t q_len,
+                                 size_t q_row_stride, size_t q_head_stride, size_t rows, size_t max_rows,
+                                 size_t n_heads, float scale, size_t window, const uint8_t* cache,
+                                 size_t cache_len, size_t n_kv_heads, size_t head_dim, size_t page_tokens,
+                                 const int32_t* pages, size_t pages_stride, size_t pages_per_seq,
+                                 size_t n_seq, const int32_t* starts, const int32_t* lens,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------
  * mivi-model: one hybrid (ShortConv + GQA) model resident on the GPU
  * ------------------------------------------------------------------- */
 

@@ -145,6 +145,27 @@ pub mod ffi {
         pub fn mivi_hip_dot_q8_0_f32(q: *const f32, q_len: usize, k_blocks: *const u8, k_len: usize,
             out: *mut f32, out_len: usize, n: usize, stream: *mut c_void) -> i32;
 
+        // paged 4-bit key/value cache (mivi-kv)
+        pub fn mivi_hip_kv_q4_page_bytes(n_kv_heads: usize, head_dim: usize, page_tokens: usize) -> usize;
+        pub fn mivi_hip_kv_q4_append(cache: *mut u8, cache_len: usize, n_kv_heads: usize,
+            head_dim: usize, page_tokens: usize, pages: *const i32, pages_stride: usize, pages_per_seq: usize,
+            n_seq: usize, starts: *const i32, lens: *const i32, type_: i32, k: *const c_void, k_len: usize,
+            k_row_stride: usize, k_head_stride: usize, v: *const c_void, v_len: usize, v_row_stride: usize,
+            v_head_stride: usize, rows: usize, stream: *mut c_void) -> i32;
+        pub fn mivi_hip_kv_q4_read(cache: *const u8, cache_len: usize, n_kv_heads: usize,
+            head_dim: usize, page_tokens: usize, pages: *const i32, pages_stride: usize, pages_per_seq: usize,
+            n_seq: usize, starts: *const i32, lens: *const i32, type_: i32, k: *mut c_void, k_len: usize,
+            k_row_stride: usize, k_head_stride: usize, v: *mut c_void, v_len: usize, v_row_stride: usize,
+            v_head_stride: usize, rows: usize, stream: *mut c_void) -> i32;
+        pub fn mivi_hip_kv_q4_attention_workspace(n_seq: usize, rows: usize, max_rows: usize, n_heads: usize,
+            n_kv_heads: usize, head_dim: usize, max_tokens: usize) -> usize;
+        pub fn mivi_hip_kv_q4_attention(type_: i32, out: *mut c_void, out_len: usize, out_row_stride: usize,
+            out_head_stride: usize, q: *const c_void, q_len: usize, q_row_stride: usize, q_head_stride: usize,
+            rows: usize, max_rows: usize, n_heads: usize, scale: f32, window: usize, cache: *const u8, cache_len: usize, n_kv_heads: usize,
+            head_dim: usize, page_tokens: usize, pages: *const i32, pages_stride: usize, pages_per_seq: usize,
+            n_seq: usize, starts: *const i32, lens: *const i32,
+            workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> i32;
+
         // crates/mivi-model/src/model.rs:105-606
         pub fn mivi_hip_model_create(gguf: *const u8, gguf_len: usize, max_ctx: usize, kv_precision: i32,
             max_batch: usize, out: *mut *mut MiviModel) -> i32;

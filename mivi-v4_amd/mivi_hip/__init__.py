@@ -104,6 +104,7 @@ class SamplerConfig(C.Structure):
 
 _lib = C.CDLL(LIB_PATH)
 _P, _S, _I = C.c_void_p, C.c_size_t, C.c_int32
+_kv_q4 = [_P, _S, _S, _S, _S, _P, _S, _S, _S, _P, _P]  # a 4-bit cache and the batch over it
 _sig = {
     "mivi_hip_last_error": ([C.POINTER(MiviError)], _I),
     "mivi_hip_version": ([], C.c_char_p),
@@ -123,6 +124,12 @@ _sig = {
     "mivi_hip_dequantize_slice": ([_I, _P, _S, _P, _S, _P], _I),
     "mivi_hip_quantize_q8_0": ([_P, _S, _P, _S, _S, _P], _I),
     "mivi_hip_dot_q8_0_f32": ([_P, _S, _P, _S, _P, _S, _S, _P], _I),
+    "mivi_hip_kv_q4_page_bytes": ([_S, _S, _S], _S),
+    "mivi_hip_kv_q4_append": (_kv_q4 + [_I, _P, _S, _S, _S, _P, _S, _S, _S, _S, _P], _I),
+    "mivi_hip_kv_q4_read": (_kv_q4 + [_I, _P, _S, _S, _S, _P, _S, _S, _S, _S, _P], _I),
+    "mivi_hip_kv_q4_attention_workspace": ([_S] * 7, _S),
+    "mivi_hip_kv_q4_attention": ([_I, _P, _S, _S, _S, _P, _S, _S, _S, _S, _S, _S, C.c_float, _S] + _kv_q4
+                                 + [_P, _S, _P], _I),
     "mivi_hip_model_create": ([_P, _S, _S, _I, _S, C.POINTER(_P)], _I),
     "mivi_hip_model_destroy": ([_P], None),
     "mivi_hip_model_info": ([_P, C.POINTER(MiviModelInfo)], _I),
@@ -384,4 +391,5 @@ def synth_random_weights(ggml_type, seed: int, rows: int, cols: int, std: float 
     return dst
 
 
+from .kv_q4 import KvCacheQ4, kv_q4_append, kv_q4_attention, kv_q4_page_bytes, kv_q4_read  # noqa: E402,F401
 from .model import Model, PrefixCache, chunk_hash  # noqa: E402,F401

@@ -253,7 +253,8 @@ int32_t mivi_hip_kv_q4_read(const uint8_t* cache, size_t cache_len, size_t n_kv_
 /* Bytes of mivi_hip_kv_q4_attention's workspace for batches of up to these
  * sizes, max_tokens = pages_per_seq * page_tokens (0: none is needed). */
 size_t mivi_hip_kv_q4_attention_workspace(size_t n_seq, size_t rows, size_t max_rows, size_t n_heads,
-                                          size_t n_kv_heads, size_t head_dim, size_t max_tokens);
+                                          size_t n_kv_heads, size_t head_dim, size_t max_tokens,
+                                          size_t window);
 
 /* out = softmax(scale q K^T) V for every row and head over the cache, which
  * holds the rows' own tokens already: a row at position p sees the positions

@@ -35,6 +35,7 @@
 // Batches. Rows are ragged: rows starts[s] .. starts[s + 1] - 1 belong to
 // sequence s and are its last positions, lens[s] - n .. lens[s] - 1.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -45,6 +46,7 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2_a4 __attribute__((ext_vector_type(2), aligned(4)));
 typedef uint32_t u32x4_a8 __attribute__((ext_vector_type(4), aligned(8)));
 
@@ -60,6 +62,7 @@ struct Q4Batch {
     const int32_t* lens;    // [n_seq]
     int64_t page_stride, n_pages, page_bytes;
     int n_seq, n_kv, hd, gpp;  // gpp: groups of a page
+    uint32_t gpp_inv;          // floor(2^32 / gpp) + 1, 0 for gpp 1
     int cap;                   // positions that the table covers
 };
 
@@ -67,6 +70,11 @@ struct Q4Batch {
 // two, so that a lane's 16 bytes are one load.
 __host__ __device__ constexpr int q4_at(int nb, int b, int lane) {
     return b / 2 < nb / 2 ? b / 2 * 1024 + lane * 16 + b % 2 * 8 : b / 2 * 1024 + lane * 8;
+}
+
+// Page of group g of a sequence, g / gpp: exact for gpp <= 32 and g < 2^27.
+__device__ __forceinline__ int page_index(const Q4Batch& a, int g) {
+    return a.gpp_inv ? (int)__umulhi((uint32_t)g, a.gpp_inv) : g;
 }
 
 // Sequence of row r, or -1: the last s with starts[s] <= r, if r is before
@@ -84,7 +92,7 @@ __device__ __forceinline__ int seq_of(const Q4Batch& a, int r) {
 // Address of the group of sequence s and kv head h at group index g, or null
 // where the table has no page of the cache there.
 __device__ __forceinline__ uint8_t* group_ptr(const Q4Batch& a, int s, int h, int g) {
-    const int pi = g / a.gpp;
+    const int pi = page_index(a, g);
     const int page = a.pages[(int64_t)s * a.page_stride + pi];
     if (page < 0 || page >= a.n_pages) return nullptr;
     return a.cache + (int64_t)page * a.page_bytes + ((int64_t)h * a.gpp + (g - pi * a.gpp)) * (36 * a.hd);
@@ -159,14 +167,35 @@ __device__ __forceinline__ void store_n(void* p, int64_t i, bool wide, const flo
 }
 
 // --------------------------------------------------------------- append
+// Largest over the four lanes l mod 16 + 16 j.
+__device__ __forceinline__ float quarters_max(float v) {
+    float x, y;
+    swap16(v, x, y);
+    v = fmaxf(x, y);
+    swap32(v, x, y);
+    return fmaxf(x, y);
+}
+
 // Value i of a quad of lanes' neighbour (quad_perm).
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
 }
 
-// The codes of 8 values of a block whose other 24 the quad's lanes hold, each
+// Largest over the four lanes of a block: a quad, or the quarters l mod 16 + 16 j.
+template <bool QUAD>
+__device__ __forceinline__ float block_max(float v) {
+    if constexpr (QUAD) {
+        v = fmaxf(v, dpp_mov<0xB1>(v));
+        return fmaxf(v, dpp_mov<0x4E>(v));
+    } else {
+        return quarters_max(v);
+    }
+}
+
+// The codes of 8 values of a block whose other 24 three more lanes hold, each
 // 0..15, and the block's scale as fp16 bits.
+template <bool QUAD>
 __device__ __forceinline__ uint32_t quantise8(const float (&in)[8], int (&code)[8]) {
     float x[8];
 #pragma unroll
@@ -176,10 +205,8 @@ __device__ __forceinline__ uint32_t quantise8(const float (&in)[8], int (&code)[
     float hi = x[0], lo = x[0];
 #pragma unroll
     for (int e = 1; e < 8; e++) hi = fmaxf(hi, x[e]), lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, dpp_mov<0xB1>(hi));
-    hi = fmaxf(hi, dpp_mov<0x4E>(hi));
-    lo = fminf(lo, dpp_mov<0xB1>(lo));
-    lo = fminf(lo, dpp_mov<0x4E>(lo));
+    hi = block_max<QUAD>(hi);
+    lo = -block_max<QUAD>(-lo);
     const float m = hi >= -lo ? hi : lo;
     const float y = fminf(fmaxf(m * -0.125f, -kMaxScale), kMaxScale);
     const uint32_t dh = f32_to_half_bits((float)(__bf16)y);
@@ -224,7 +251,7 @@ __global__ void __launch_bounds__(256) kv_q4_append_kernel(Q4Batch a, const void
     int code[8];
     load8<T>(is_v ? v : k, (int64_t)row * (is_v ? v_row : k_row) + h * (is_v ? v_head : k_head) + b * 32 + c * 8,
              is_v ? wide_v : wide_k, x);
-    const uint32_t d = quantise8(x, code);
+    const uint32_t d = quantise8<true>(x, code);
     if (!is_v) {
         uint32_t w = 0;
 #pragma unroll
@@ -289,6 +316,195 @@ __global__ void __launch_bounds__(256) kv_q4_read_kernel(Q4Batch a, void* k, voi
                   is_v ? wide_v : wide_k, x);
 }
 
+// ------------------------------------------------- whole groups at a time
+// Rows that are many: a wave takes one group of one sequence and head, K or V.
+// Sequence s has the units from U(s) = starts[s] / 32 + 2 s on: its n rows touch
+// at most (n - 2) / 32 + 2 groups, and U(s + 1) - U(s) is no less, so no sum
+// over the sequences is needed to place them.
+struct Q4Unit {
+    uint8_t* g;    // the group, null where the table has no page of the cache
+    int64_t row0;  // row of the group's token 0
+    int t0, t1;    // tokens of the group that are rows of the call
+};
+
+// Last s with key(s) <= u (key does not decrease): 64 sequences a look.
+template <class Key>
+__device__ __forceinline__ int wave_search(int n, int lane, int u, Key key) {
+    int lo = 0;
+    while (n > 1) {
+        const int step = (n + 63) / 64;
+        const int64_t i = (int64_t)lane * step;
+        const int count = __popcll(__ballot(i < n && key(lo + (int)i) <= u));
+        if (count == 0) return lo;
+        lo += (count - 1) * step;
+        n = min(step, n - (count - 1) * step);
+    }
+    return lo;
+}
+
+__device__ __forceinline__ bool unit_of(const Q4Batch& a, int u, int h, int rows, int lane, Q4Unit* o) {
+    const int s = __builtin_amdgcn_readfirstlane(
+        wave_search(a.n_seq, lane, u, [&](int i) { return (a.starts[i] >> 5) + 2 * i; }));
+    const int start = a.starts[s];
+    const int local = u - ((start >> 5) + 2 * s);
+    const int64_t count = min<int64_t>((int64_t)a.starts[s + 1] - start, (int64_t)rows - start);
+    if (start < 0 || count <= 0 || local < 0) return false;
+    const int64_t p0 = (int64_t)a.lens[s] - ((int64_t)a.starts[s + 1] - start);  // position of the first row
+    const int64_t g = (p0 >> 5) + local, base = g * kGroup;
+    if (base >= p0 + count) return false;
+    o->row0 = start + (base - p0);
+    o->t0 = (int)max<int64_t>(p0 - base, 0);
+    o->t1 = (int)min<int64_t>(p0 + count - base, kGroup);
+    o->g = base >= 0 && base < a.cap ? group_ptr(a, s, h, (int)g) : nullptr;
+    return true;
+}
+
+// Byte of a group's V codes in its LDS image: 16 bytes more every 256, so that
+// the quarters of the tokens are in different banks.
+__device__ __forceinline__ int image_at(int byte) { return byte + (byte >> 8 << 4); }
+constexpr int kImage = 16 * 256 / 256 * 272;  // bytes of the largest
+
+template <int T>
+__global__ void __launch_bounds__(256) kv_q4_append_groups_kernel(Q4Batch a, const void* k, const void* v,
+                                                                  int64_t k_row, int64_t k_head, int64_t v_row,
+                                                                  int64_t v_head, int rows, int wide_k, int wide_v) {
+    __shared__ __attribute__((aligned(16))) uint8_t image[4][kImage];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int which = blockIdx.y * 4 + wave, h = which >> 1;
+    const bool is_v = which & 1;
+    if (h >= a.n_kv) return;
+    Q4Unit u;
+    if (!unit_of(a, blockIdx.x, h, rows, lane, &u) || !u.g) return;
+    const int hd = a.hd, nb = hd / 32, t16 = lane & 15, c = lane >> 4;
+    const void* x = is_v ? v : k;
+    const int64_t rs = is_v ? v_row : k_row;
+    const int wide = is_v ? wide_v : wide_k;
+    const int64_t base = (u.row0 + t16) * rs + h * (is_v ? v_head : k_head) + c * 8;
+    const bool in[2] = {t16 >= u.t0 && t16 < u.t1, t16 + 16 >= u.t0 && t16 + 16 < u.t1};
+    const bool whole = u.t1 - u.t0 == kGroup;
+    uint8_t* img = image[wave];
+    for (int b = 0; b < nb; b += 2) {
+        const bool two = b + 1 < nb;
+        float val[4][8];  // [block of the pair][half]
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) val[i][e] = 0.f;
+            if (in[i % 2] && (i < 2 || two)) load8<T>(x, base + i % 2 * 16 * rs + (b + i / 2) * 32, wide, val[i]);
+        }
+        uint32_t w[4], d[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            int code[8];
+            d[i] = quantise8<false>(val[i], code);
+            w[i] = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[i] |= (uint32_t)code[e] << (is_v ? 4 * e : 4 * (e / 2) + 16 * (e % 2));
+        }
+        const int off = q4_at(nb, b, lane);  // of the lane's dwords: [block][half]
+        if (!is_v) {
+            if (whole) {
+                if (two) *(u32x4*)(u.g + off) = u32x4{w[0], w[1], w[2], w[3]};
+                else *(u32x2*)(u.g + off) = u32x2{w[0], w[1]};
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (in[i % 2] && (i < 2 || two)) *(uint32_t*)(u.g + off + 4 * i) = w[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (c == 0 && in[i % 2] && (i < 2 || two))
+                    *(uint16_t*)(u.g + 32 * hd + 2 * (t16 * 2 * nb + i % 2 * nb + b + i / 2)) = (uint16_t)d[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (i >= 2 && !two) break;
+                // lanes of quarters 0 and 1 hold dimensions 0..15 of the block,
+                // 2 and 3 the ones 16 further: a lane stores four of the eight
+                // pairs that it can form with the lane 32 away
+                float a0, a1;
+                swap32(__uint_as_float(w[i]), a0, a1);
+                const uint32_t lo = __float_as_uint(a0), hi = __float_as_uint(a1);
+                const int byte = i % 2 * 4 + ((t16 & 1) * 2 | (t16 >> 1 & 1));
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int e = (c >> 1) * 4 + j, n = (c & 1) * 8 + e;
+                    const uint8_t pair = (uint8_t)((lo >> (4 * e) & 15) | (hi >> (4 * e) & 15) << 4);
+                    const int at = q4_at(nb, b + i / 2, n + 16 * (t16 / 4)) + byte;
+                    if (whole) img[image_at(at)] = pair;
+                    else if (in[i % 2]) u.g[16 * hd + at] = pair;
+                }
+                if (c == 0 && in[i % 2])
+                    *(uint16_t*)(u.g + 34 * hd + 2 * ((b + i / 2) * 32 + t16 / 4 * 8 + i % 2 * 4 + t16 % 4)) = (uint16_t)d[i];
+            }
+        }
+    }
+    if (is_v && whole) {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        for (int i = lane * 16; i < 16 * hd; i += 1024) *(u32x4*)(u.g + 16 * hd + i) = *(const u32x4*)(img + image_at(i));
+    }
+}
+
+template <int T>
+__global__ void __launch_bounds__(256) kv_q4_read_groups_kernel(Q4Batch a, void* k, void* v, int64_t k_row,
+                                                                int64_t k_head, int64_t v_row, int64_t v_head,
+                                                                int rows, int wide_k, int wide_v) {
+    __shared__ __attribute__((aligned(16))) uint8_t image[4][kImage];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int which = blockIdx.y * 4 + wave, h = which >> 1;
+    const bool is_v = which & 1;
+    if (h >= a.n_kv) return;
+    Q4Unit u;
+    if (!unit_of(a, blockIdx.x, h, rows, lane, &u)) return;
+    const int hd = a.hd, nb = hd / 32, t16 = lane & 15, c = lane >> 4;
+    void* x = is_v ? v : k;
+    const int64_t rs = is_v ? v_row : k_row;
+    const int wide = is_v ? wide_v : wide_k;
+    const int64_t base = (u.row0 + t16) * rs + h * (is_v ? v_head : k_head) + c * 8;
+    const bool in[2] = {t16 >= u.t0 && t16 < u.t1, t16 + 16 >= u.t0 && t16 + 16 < u.t1};
+    uint8_t* img = image[wave];
+    if (is_v && u.g) {
+        for (int i = lane * 16; i < 16 * hd; i += 1024) *(u32x4*)(img + image_at(i)) = *(const u32x4*)(u.g + 16 * hd + i);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    for (int b = 0; b < nb; b += 2) {
+        const bool two = b + 1 < nb;
+        u32x4 w = {0, 0, 0, 0};  // K codes [block of the pair][half]
+        if (!is_v && u.g) {
+            if (two) {
+                w = *(const u32x4*)(u.g + q4_at(nb, b, lane));
+            } else {
+                const u32x2 y = *(const u32x2*)(u.g + q4_at(nb, b, lane));
+                w[0] = y[0], w[1] = y[1];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (!in[i % 2] || (i >= 2 && !two)) continue;
+            float out[8] = {};
+            if (u.g) {
+                const int at = is_v ? 34 * hd + 2 * ((b + i / 2) * 32 + t16 / 4 * 8 + i % 2 * 4 + t16 % 4)
+                                    : 32 * hd + 2 * (t16 * 2 * nb + i % 2 * nb + b + i / 2);
+                const float d = half_bits_to_f32(*(const uint16_t*)(u.g + at));
+                const int byte = i % 2 * 4 + ((t16 & 1) * 2 | (t16 >> 1 & 1));
+                const int first = q4_at(nb, b + i / 2, (c & 1) * 8 + 16 * (t16 / 4)) + byte;
+                const int step = b + i / 2 < nb / 2 * 2 ? 16 : 8;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t code = is_v ? img[image_at(first + e * step)] >> (c / 2 * 4) & 15
+                                               : w[i] >> (4 * (e / 2) + 16 * (e % 2)) & 15;
+                    out[e] = (float)((int)code - 8) * d;
+                }
+            }
+            store_n<T, 8>(x, base + i % 2 * 16 * rs + (b + i / 2) * 32, wide, out);
+        }
+    }
+}
+
 // ------------------------------------------------------------ attention
 struct Q4Attn {
     Q4Batch b;
@@ -296,32 +512,71 @@ struct Q4Attn {
     void* out;
     int64_t q_row, q_head, o_row, o_head;
     int type, wide_q, wide_o;
-    int n_heads, gq;      // gq: query heads of a kv head
-    int rows, max_rows, tiles;  // row tiles of 16 (row, query head) pairs a sequence and kv head
-    int nsplit, window;
+    int n_heads, gq;            // gq: query heads of a kv head
+    int rows, max_rows, tiles;  // row tiles of tile_pairs (row, query head) pairs a sequence and kv head
+    int tile_pairs;
+    int nsplit;                 // parts of a pair that the workspace has room for
+    int chunk;                  // groups of a share of a tile; 0: even shares
+    int share_min;              // even shares: groups of the smallest
+    int window;
     float scale;
-    float* part_acc;      // [rows * n_heads][nsplit][hd]
-    float* part_ml;       // [rows * n_heads][nsplit][2]
+    float* part_acc;            // [rows * n_heads][nsplit][hd]
+    float* part_ml;             // [rows * n_heads][nsplit][2]
 };
 
+// Row of a pair.
+__device__ __forceinline__ int row_of(const Q4Attn& a, int f) { return (int)((uint32_t)f / (uint32_t)a.gq); }
+
 // Codes of one dword as four fp16 pairs 16 + c: nibbles (0, 4), (1, 5), (2, 6),
-// (3, 7) into the top mantissa bits of 16.0.
-__device__ __forceinline__ half2v pair16(uint32_t w, int i) {
-    const uint32_t x = i == 0 ? w << 6 : i == 1 ? w << 2 : i == 2 ? w >> 2 : w >> 6;
-    return __builtin_bit_cast(half2v, (x & 0x03C003C0u) | 0x4C004C00u);
-}
+// (3, 7) into the top mantissa bits of 16.0. The constants are held in
+// registers that the compiler does not see through: as literals they cost two
+// instructions (and, or) in place of one.
+struct Q4Bits {
+    uint32_t mask = 0x03C003C0u, sixteen = 0x4C004C00u;
+    __device__ __forceinline__ Q4Bits() {
+        asm("" : "+s"(mask));
+        asm("" : "+v"(sixteen));
+    }
+    __device__ __forceinline__ half2v pair(uint32_t w, int i) const {
+        const uint32_t x = i == 0 ? w << 6 : i == 1 ? w << 2 : i == 2 ? w >> 2 : w >> 6;
+        return __builtin_bit_cast(half2v, (x & mask) | sixteen);
+    }
+};
 // (16 + c) d - 24 d = (c - 8) d, exact; dm = -24 d (10 significant bits, exact)
 __device__ __forceinline__ half2v held(half2v x, half2v d, half2v dm) { return __builtin_elementwise_fma(x, d, dm); }
 
-__device__ __forceinline__ float load_q(const Q4Attn& a, int64_t i) {
-    return a.type == MIVI_GGML_F32   ? load_elem<MIVI_GGML_F32>(a.q, i)
-           : a.type == MIVI_GGML_F16 ? load_elem<MIVI_GGML_F16>(a.q, i)
-                                     : load_elem<MIVI_GGML_BF16>(a.q, i);
-}
-__device__ __forceinline__ void load_q8(const Q4Attn& a, int64_t i, float (&x)[8]) {
-    if (a.type == MIVI_GGML_F32) load8<MIVI_GGML_F32>(a.q, i, a.wide_q, x);
-    else if (a.type == MIVI_GGML_F16) load8<MIVI_GGML_F16>(a.q, i, a.wide_q, x);
-    else load8<MIVI_GGML_BF16>(a.q, i, a.wide_q, x);
+// A query row's blocks, 8 values each at i + 32 b: every load before any use.
+template <int NB>
+__device__ __forceinline__ void load_row(const Q4Attn& a, int64_t i, float (&x)[NB][8]) {
+    if (!a.wide_q) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            if (a.type == MIVI_GGML_F32) load8<MIVI_GGML_F32>(a.q, i + 32 * b, false, x[b]);
+            else if (a.type == MIVI_GGML_F16) load8<MIVI_GGML_F16>(a.q, i + 32 * b, false, x[b]);
+            else load8<MIVI_GGML_BF16>(a.q, i + 32 * b, false, x[b]);
+        }
+    } else if (a.type == MIVI_GGML_F32) {
+        f32x4 w[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+            w[b][0] = *(const f32x4*)((const float*)a.q + i + 32 * b), w[b][1] = *(const f32x4*)((const float*)a.q + i + 32 * b + 4);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[b][e] = w[b][e / 4][e % 4];
+    } else {
+        u32x4 w[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) w[b] = *(const u32x4*)((const uint16_t*)a.q + i + 32 * b);
+        const bool f16 = a.type == MIVI_GGML_F16;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint32_t u = w[b][e / 2] >> (e % 2 * 16);
+                x[b][e] = f16 ? half_bits_to_f32(u) : bf16_bits_to_f32(u);
+            }
+    }
 }
 __device__ __forceinline__ void store_o4(const Q4Attn& a, int64_t i, const float (&x)[4]) {
     if (a.type == MIVI_GGML_F32) store_n<MIVI_GGML_F32, 4>(a.out, i, a.wide_o, x);
@@ -329,37 +584,162 @@ __device__ __forceinline__ void store_o4(const Q4Attn& a, int64_t i, const float
     else store_n<MIVI_GGML_BF16, 4>(a.out, i, a.wide_o, x);
 }
 
-// value of the quarters of a lane's query row (lanes l mod 16 + 16 j), joined
-__device__ __forceinline__ float quarters_max(float v) {
-    float x, y;
-    swap16(v, x, y);
-    v = fmaxf(x, y);
-    swap32(v, x, y);
-    return fmaxf(x, y);
-}
-__device__ __forceinline__ float quarters_sum(float v) {
-    float x, y;
-    swap16(v, x, y);
-    v = x + y;
-    swap32(v, x, y);
-    return x + y;
-}
-
-// The largest finite exponent normalisation of a query row: the power of two
-// that puts its largest magnitude into [2^14, 2^15), so that fp16 holds 11 bits
-// of every value down to 2^-28 of the largest (23 bits with the second plane).
-// A row with an infinity or NaN, or of zeros, stays as it is.
+// The power of two that puts a query row's largest magnitude into
+// [2^14, 2^15), so that fp16 holds 11 bits of every value down to 2^-28 of the
+// largest (22 bits with the second plane). A row with an infinity or NaN, or
+// of zeros, stays as it is.
 __device__ __forceinline__ int row_exponent(float amax) {
     const uint32_t u = __float_as_uint(amax);
     if (u == 0 || u >= 0x7F800000u) return 0;
     return 14 - ilogbf(amax);
 }
 
-// A group's codes and scales as lane l loads them.
-template <int NB>
-struct Q4Raw {
-    uint32_t k[2 * NB], v[2 * NB], ks[NB], vs[4 * NB];
+// What a sequence's rows see: positions lo(i) .. hi(i) - 1 for row i.
+struct Q4Seen {
+    int first;  // position of row 0
+    int cap, window;
+    __device__ __forceinline__ int hi(int i) const { return min(max(first + i + 1, 0), cap); }
+    __device__ __forceinline__ int lo(int i) const { return window ? min(max(max(first + i + 1, 0) - window, 0), cap) : 0; }
 };
+
+// Groups g_lo .. g_hi - 1 hold what rows i0 .. i1 see.
+__device__ __forceinline__ void tile_groups(const Q4Seen& see, int i0, int i1, int* g_lo, int* g_hi) {
+    *g_lo = see.lo(i0) / kGroup;
+    *g_hi = (see.hi(i1) + kGroup - 1) / kGroup;
+}
+
+__device__ __forceinline__ half2v as_half2(uint32_t w) { return __builtin_bit_cast(half2v, w); }
+__device__ __forceinline__ half8 join8(half2v a, half2v b, half2v c, half2v d) {
+    return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// K codes of a token's eight dimensions: the A operand of its block.
+__device__ __forceinline__ half8 held_k(const Q4Bits& q, uint32_t w, _Float16 ds) {
+    const half2v d = {ds, ds}, dm = d * (_Float16)-24;
+    return join8(held(q.pair(w, 0), d, dm), held(q.pair(w, 1), d, dm), held(q.pair(w, 2), d, dm),
+                 held(q.pair(w, 3), d, dm));
+}
+// V codes of eight tokens: the A operands of the block's two halves of 16
+// dimensions; sc: the tokens' four scale pairs.
+__device__ __forceinline__ void held_v(const Q4Bits& q, uint32_t w0, uint32_t w1, const uint32_t* sc, half8 (&v)[2]) {
+    half2v d[4], dm[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) d[j] = as_half2(sc[j]), dm[j] = d[j] * (_Float16)-24;
+#pragma unroll
+    for (int z = 0; z < 2; z++)
+        v[z] = join8(held(q.pair(w0, z), d[0], dm[0]), held(q.pair(w0, z + 2), d[1], dm[1]),
+                     held(q.pair(w1, z), d[2], dm[2]), held(q.pair(w1, z + 2), d[3], dm[3]));
+}
+
+// A V scale pair j (of 4) of the lane's quarter in a group at t0, without the
+// tokens from `valid` on: what lies behind the sequence's end is anything, and
+// 0 * NaN is NaN.
+__device__ __forceinline__ uint32_t keep_mask(int t0, int quarter, int j, int valid) {
+    const int t = t0 + j / 2 * 16 + quarter * 4 + j % 2 * 2;
+    return (t < valid ? 0xFFFFu : 0u) | (t + 1 < valid ? 0xFFFF0000u : 0u);
+}
+
+constexpr float kPShift = 15;  // weights are held times 2^15: fp16 reaches 2^-40 of the largest
+
+// 16 (row, query head) pairs as the columns of the products; lane l works on
+// column l mod 16.
+template <int NB, int P>
+struct Q4Tile {
+    half8 q[P][NB];      // B operands: block b, dimensions 8 quarter .. + 7
+    float sc;            // a raw score times sc is the exponent to base 2
+    float m, nm;         // largest exponent so far; kPShift - m, the exponent's offset
+    f32x4 acc[2 * NB];   // sums of w V: dimensions 16 j + 4 quarter + i
+    f32x4 l;             // sums of w, the same in all four
+    int lo, hi;          // positions seen
+
+    __device__ __forceinline__ void init(const Q4Attn& a, const Q4Seen& see, int row0, int h, int f, int pairs,
+                                         int quarter) {
+        const int fc = min(f, pairs - 1);  // columns past the last pair repeat it; they are not stored
+        const int i = row_of(a, fc), head = h * a.gq + (fc - i * a.gq);
+        lo = see.lo(i), hi = see.hi(i);
+        float x[NB][8], amax = 0.f;
+        const int64_t base = (int64_t)(row0 + i) * a.q_row + head * a.q_head + quarter * 8;
+        const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
+        load_row<NB>(a, base, x);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = fabsf(x[b][e]);
+                amax = v == v ? fmaxf(amax, v) : __builtin_inff();
+            }
+        }
+        amax = quarters_max(amax);
+        const int ex = row_exponent(amax);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float y = ldexpf(x[b][e], ex) * sign;
+                const _Float16 top = (_Float16)y;
+                q[0][b][e] = top;
+                if constexpr (P == 2) q[1][b][e] = (_Float16)(y - (float)top);
+            }
+        }
+        // positive, so that the largest score has the largest exponent and a
+        // hidden one's -inf stays that
+        sc = fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -ex), 1.17549435e-38f);
+        m = -__builtin_inff(), nm = kPShift;
+        l = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 2 * NB; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // The scores of a group (tokens 4 quarter + i of each half) to weights, the
+    // B operands of the sums. The maximum over the quarters is formed only when
+    // some lane has a larger score than its row had.
+    __device__ __forceinline__ void weigh(const f32x4 (&st)[2], half8 (&w)[P]) {
+        float mx = st[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) mx = fmaxf(mx, st[i / 4][i % 4]);
+        if (__any(mx * sc > m)) {
+            const float m_new = fmaxf(m, quarters_max(mx) * sc);
+            const float f = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            nm = kPShift - (m == -__builtin_inff() ? 0.f : m);
+            l *= f;
+#pragma unroll
+            for (int j = 0; j < 2 * NB; j++) acc[j] *= f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const f32x2 x = {__builtin_amdgcn_exp2f(fmaf(st[i / 4][i % 4], sc, nm)),
+                             __builtin_amdgcn_exp2f(fmaf(st[i / 4][i % 4 + 1], sc, nm))};
+            const half2v top = __builtin_convertvector(x, half2v);
+            w[0][i] = top.x, w[0][i + 1] = top.y;
+            if constexpr (P == 2) {  // x - top, exact, in one instruction each
+                const f32x2 rest = {fmaf((float)top.x, -1.f, x.x), fmaf((float)top.y, -1.f, x.y)};
+                const half2v low = __builtin_convertvector(rest, half2v);
+                w[1][i] = low.x, w[1][i + 1] = low.y;
+            }
+        }
+    }
+
+    // Scores that the row does not see.
+    __device__ __forceinline__ void hide(f32x4 (&st)[2], int t0, int quarter) const {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int t = t0 + i / 4 * 16 + quarter * 4 + i % 4;
+            st[i / 4][i % 4] = t >= lo && t < hi ? st[i / 4][i % 4] : -__builtin_inff();
+        }
+    }
+};
+
+__device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ half8 ones8() {
+    const _Float16 o = 1;
+    return half8{o, o, o, o, o, o, o, o};
+}
+
+// A group's codes and scales as lane l loads them: K or V codes of all blocks,
+// the K scales of token l mod 16 in both halves, the V scales of the quarter.
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {  // 4-byte aligned
     if constexpr (N >= 4) {
@@ -375,268 +755,556 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {  // 
         w[0] = *(const uint32_t*)p;
     }
 }
+template <int NB, int B0 = 0, int B1 = NB>  // blocks B0 .. B1 - 1, B0 even
+__device__ __forceinline__ void load_codes(const uint8_t* p, int lane, uint32_t* w) {
+#pragma unroll
+    for (int b = B0; b < B1; b += 2) {
+        if (b + 1 < NB) {
+            const u32x4 x = __builtin_nontemporal_load((const u32x4*)(p + b / 2 * 1024 + lane * 16));
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[2 * (b - B0) + j] = x[j];
+        } else {
+            const u32x2 x = *(const u32x2*)(p + b / 2 * 1024 + lane * 8);
+            w[2 * (b - B0)] = x[0], w[2 * (b - B0) + 1] = x[1];
+        }
+    }
+}
 template <int NB>
-__device__ __forceinline__ void load_codes(const uint8_t* p, int lane, uint32_t (&w)[2 * NB]) {
+__device__ __forceinline__ void load_k(const uint8_t* g, int lane, uint32_t (&k)[2 * NB], uint32_t (&ks)[NB]) {
+    load_codes<NB>(g, lane, k);
+    load_words<NB>(g + 1024 * NB + lane % 16 * 4 * NB, ks);
+}
+template <int NB, int B0 = 0, int B1 = NB>
+__device__ __forceinline__ void load_v(const uint8_t* g, int lane, uint32_t* v, uint32_t* vs) {
+    load_codes<NB, B0, B1>(g + 512 * NB, lane, v);
 #pragma unroll
-    for (int i = 0; i < NB / 2; i++) {
-        const u32x4 x = *(const u32x4*)(p + i * 1024 + lane * 16);
+    for (int b = B0; b < B1; b++) {
+        const u32x4 x = *(const u32x4*)(g + 1088 * NB + (b * 4 + lane / 16) * 16);
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[4 * i + j] = x[j];
-    }
-    if constexpr (NB % 2) {
-        const u32x2 x = *(const u32x2*)(p + NB / 2 * 1024 + lane * 8);
-        w[2 * NB - 2] = x[0], w[2 * NB - 1] = x[1];
+        for (int j = 0; j < 4; j++) vs[4 * (b - B0) + j] = x[j];
     }
 }
 template <int NB>
-__device__ __forceinline__ void load_group(const uint8_t* g, int lane, Q4Raw<NB>& r) {
-    constexpr int hd = 32 * NB;
-    load_codes<NB>(g, lane, r.k);
-    load_words<NB>(g + 32 * hd + lane % 16 * 4 * NB, r.ks);
-    load_codes<NB>(g + 16 * hd, lane, r.v);
+__device__ __forceinline__ _Float16 k_scale(const uint32_t (&ks)[NB], int half, int b) {
+    const int i = half * NB + b;
+    return as_half2(ks[i / 2])[i % 2];
+}
+
+// What a workgroup knows of its sequence's rows.
+struct Q4Rows {
+    int start, valid, pairs;
+    Q4Seen see;
+};
+__device__ __forceinline__ bool rows_of(const Q4Attn& a, int s, Q4Rows* r) {
+    const int start = a.b.starts[s], len = a.b.lens[s];
+    const int64_t count = (int64_t)a.b.starts[s + 1] - start;
+    r->start = start;
+    // rows times heads fits 31 bits
+    r->pairs = start < 0 || start >= a.rows ? 0 : (int)min<int64_t>(count, min(a.max_rows, a.rows - start)) * a.gq;
+    r->see = Q4Seen{(int)max<int64_t>(len - count, INT32_MIN), a.b.cap, a.window};
+    r->valid = min(max(len, 0), a.b.cap);
+    return r->pairs > 0;
+}
+
+// Values d4 .. d4 + 3 of a pair's sums o over the weights' sum l: the output
+// (part < 0), or one part of it.
+__device__ __forceinline__ void store_pair(const Q4Attn& a, const Q4Rows& r, int h, int f, int part, int d4,
+                                           float m, float l, float (&o)[4]) {
+    const int i = row_of(a, f), head = h * a.gq + (f - i * a.gq);
+    if (part < 0) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that sees nothing is zero
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
-        const u32x4 x = *(const u32x4*)(g + 34 * hd + (b * 4 + lane / 16) * 16);
-#pragma unroll
-        for (int j = 0; j < 4; j++) r.vs[4 * b + j] = x[j];
+        for (int e = 0; e < 4; e++) o[e] *= inv;
+        store_o4(a, (int64_t)(r.start + i) * a.o_row + head * a.o_head + d4, o);
+    } else {
+        const int64_t p = ((int64_t)(r.start + i) * a.n_heads + head) * a.nsplit + part;
+        *(f32x4*)(a.part_acc + p * a.b.hd + d4) = f32x4{o[0], o[1], o[2], o[3]};
+        if (d4 == 0) a.part_ml[2 * p] = m, a.part_ml[2 * p + 1] = l;
     }
 }
 
-__device__ __forceinline__ half2v as_half2(uint32_t w) { return __builtin_bit_cast(half2v, w); }
-__device__ __forceinline__ half8 join8(half2v a, half2v b, half2v c, half2v d) {
-    return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+// A sequence's groups of one head: the page id of a group (loaded well before
+// its address is wanted), then the address, null where that is no page of the
+// cache. Groups from `end` on have the last one's id and no address.
+struct Q4Groups {
+    const uint8_t* base;
+    const int32_t* table;
+    int end;
+    __device__ __forceinline__ Q4Groups(const Q4Attn& a, int s, int h, int g_end)
+        : base(a.b.cache + (int64_t)h * a.b.gpp * (36 * a.b.hd)), table(a.b.pages + (int64_t)s * a.b.page_stride),
+          end(g_end) {}
+    __device__ __forceinline__ int id(const Q4Attn& a, int g) const { return table[page_index(a.b, min(g, end - 1))]; }
+    __device__ __forceinline__ const uint8_t* at(const Q4Attn& a, int g, int id) const {
+        const int64_t off = (int64_t)id * a.b.page_bytes + (g - page_index(a.b, g) * a.b.gpp) * (36 * a.b.hd);
+        return g < end && (uint32_t)id < (uint32_t)a.b.n_pages ? base + off : nullptr;
+    }
+};
+
+// A workgroup's place: a head and sequence, a tile of its pairs, a range of the
+// groups that the tile sees, and where its sums go (store_pair).
+struct Q4Place {
+    Q4Rows r;
+    int h, s, part, g_begin, g_end;
+    int f0;  // first pair of the tile
+};
+
+// Shares of `chunk` groups of a tile; false if this one has no work.
+__device__ __forceinline__ bool place_of(const Q4Attn& a, int split, int tile, int head_seq, Q4Place* p) {
+    p->part = a.nsplit == 1 ? -1 : split;
+    p->h = head_seq % a.b.n_kv, p->s = head_seq / a.b.n_kv;
+    p->f0 = tile * a.tile_pairs;
+    if (!rows_of(a, p->s, &p->r) || p->f0 >= p->r.pairs) return false;
+    int g_lo, g_hi;
+    tile_groups(p->r.see, row_of(a, p->f0), row_of(a, min(p->f0 + a.tile_pairs, p->r.pairs) - 1), &g_lo, &g_hi);
+    p->g_begin = g_lo + split * a.chunk, p->g_end = min(p->g_begin + a.chunk, g_hi);
+    return split == 0 || p->g_begin < p->g_end;  // the join does not read an empty share but the first
 }
 
-constexpr float kPShift = 15;  // weights are held times 2^15: fp16 reaches 2^-39 of the largest
+// Even shares, where a sequence's pairs are one tile: the groups of all
+// sequences and heads in one row (sequence by sequence, head by head), cut at
+// every `size` and between heads. Each piece is one workgroup's, so that no
+// workgroup has more than `size` whatever the lengths. The head and sequence i
+// at x has the workgroups from x / size + i on (the next one's first is past its
+// last). Every wave forms the cut by itself, 64 sequences a look.
+// (All positions fit 31 bits: the plan takes other shares where they might not.)
+struct Q4Cut {
+    int total;   // groups of all sequences and heads
+    int size;    // of a share
+    int lo, n;   // this lane's sequence of the first 64: its first group, its groups
+    int before;  // groups of a head of the sequences before it
+};
+__device__ __forceinline__ void seq_groups(const Q4Attn& a, int s, int* lo, int* n) {
+    Q4Rows r;
+    *lo = *n = 0;
+    if (s >= a.b.n_seq || !rows_of(a, s, &r)) return;
+    int hi;
+    tile_groups(r.see, 0, row_of(a, r.pairs - 1), lo, &hi);
+    *n = max(hi - *lo, 0);
+}
+__device__ __forceinline__ int wave_before(int v, int lane) {  // sum of the lanes before
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o, 64);
+        if (lane >= o) x += y;
+    }
+    return x - v;
+}
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ int udiv(int a, int b) { return (int)((uint32_t)a / (uint32_t)b); }
 
-// Row tiles of 16 (row, query head) pairs f = i gq + head of one sequence and
-// kv head over a share of its groups; wave w of the four takes every fourth
-// group. One pass with the running maximum and sum of the softmax; P is the
-// planes of the query rows and of the weights (2 for f32 values: each plane an
-// fp16 operand, 22 bits in all; 1 for fp16 and bf16 values, whose queries fp16
-// holds exactly and whose outputs have no more bits than the weights).
+__device__ __forceinline__ Q4Cut cut_of(const Q4Attn& a, int lane, int shares) {
+    Q4Cut c;
+    seq_groups(a, lane, &c.lo, &c.n);
+    c.before = wave_before(c.n, lane);
+    c.total = lane_value(c.before + c.n, 63);
+    int most = c.n;
+    for (int base = 64; base < a.b.n_seq; base += 64) {
+        int lo, n;
+        seq_groups(a, base + lane, &lo, &n);
+        c.total += lane_value(wave_before(n, lane) + n, 63);
+        most = max(most, n);
+    }
+    c.total *= a.b.n_kv;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+    most = __builtin_amdgcn_readfirstlane(most);
+    // no pair has more parts than the workspace has room for: n groups lie in
+    // at most (n - 1) / size + 2 shares
+    const int even = udiv(c.total + shares - 1, shares), least = udiv(most + a.nsplit - 2, max(a.nsplit - 1, 1));
+    c.size = udiv(max(max(even, least), a.share_min) + a.share_min - 1, a.share_min) * a.share_min;
+    return c;
+}
+
+// The piece of workgroup u; false if it has none.
+__device__ __forceinline__ bool piece_of(const Q4Attn& a, int lane, int shares, int u, Q4Place* p) {
+    const Q4Cut c = cut_of(a, lane, shares);
+    const int kv = a.b.n_kv;
+    int base = 0, lo = c.lo, n = c.n, before = c.before, run = 0;  // run: groups before sequence `base`
+    for (;;) {  // the 64 sequences that hold it
+        const int next = run + lane_value(before + n, 63);
+        if (base + 64 >= a.b.n_seq || udiv(next * kv, c.size) + (base + 64) * kv > u) break;
+        run = next;
+        base += 64;
+        seq_groups(a, base + lane, &lo, &n);
+        before = wave_before(n, lane);
+    }
+    const uint64_t at =
+        __ballot(base + lane < a.b.n_seq && udiv((run + before) * kv, c.size) + (base + lane) * kv <= u);
+    const int l = at ? 63 - __clzll(at) : 0;
+    lo = lane_value(lo, l), n = lane_value(n, l);
+    const int x0 = (run + lane_value(before, l)) * kv;
+    int h = 0;  // the last head whose first workgroup is u or before
+    for (int h0 = 0; h0 < kv; h0 += 64) {
+        const int hh = h0 + lane;
+        const uint64_t m = __ballot(hh < kv && udiv(x0 + hh * n, c.size) + (base + l) * kv + hh <= u);
+        if (m) h = h0 + 63 - __clzll(m);
+    }
+    const int x = x0 + h * n, first = udiv(x, c.size), last = udiv(x + max(n, 1) - 1, c.size);
+    const int part = u - (first + (base + l) * kv + h);
+    if (n == 0 || part < 0 || part > last - first || !rows_of(a, base + l, &p->r)) return false;
+    p->s = base + l, p->h = h, p->f0 = 0;
+    p->part = first == last ? -1 : part;
+    p->g_begin = lo + max((first + part) * c.size - x, 0);
+    p->g_end = lo + min((first + part + 1) * c.size - x, n);
+    return true;
+}
+
+// A workgroup's place by even shares (chunk 0), or by shares of a tile: heads and
+// sequences next to each other, so that a head's workgroups are on one XCD (and
+// its L2) where the heads are a multiple of 8; the last tiles, which see most,
+// first.
+__device__ __forceinline__ bool head_place(const Q4Attn& a, int lane, int shares, Q4Place* p) {
+    if (a.chunk == 0) return piece_of(a, lane, shares, blockIdx.x, p);
+    const int heads = a.b.n_kv * a.b.n_seq, id = blockIdx.x / heads;
+    return place_of(a, id % a.nsplit, a.tiles - 1 - id / a.nsplit, blockIdx.x % heads, p);
+}
+
+// Up to 16 pairs of a sequence and kv head: a workgroup takes a range of their
+// groups, each of its four waves every fourth one straight from memory to
+// operands, and joins the waves at the end. One pass with the running maximum
+// and sum of the softmax. P: the fp16 planes of the query rows and of the
+// weights (2 for f32 values, 22 bits in all; 1 for fp16 and bf16 values, whose
+// queries fp16 holds exactly and whose outputs have no more bits than the
+// weights). K of the next group is on its way during the sums, V during the
+// scores, and page ids two groups ahead of that.
+//
+// Waves a SIMD that the registers are held to: 17 nb words of codes, scales and
+// sums and 4 nb a plane of queries beside about 40 others.
+constexpr int step_waves(int nb, int p) {
+    const int words = nb * (17 + 4 * p);
+    return words <= 84 ? 4 : words <= 102 ? 3 : 2;
+}
 template <int NB, int P>
-__global__ void __launch_bounds__(256) kv_q4_attn_kernel(Q4Attn a) {
+__global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4Attn a, int shares) {
     constexpr int hd = 32 * NB;
     __shared__ float red_ml[4][16][2];
     __shared__ float red_acc[4][16][hd + 4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quarter = lane >> 4;
-    int64_t id = blockIdx.x;
-    const int split = (int)(id % a.nsplit);
-    id /= a.nsplit;
-    const int tile = (int)(id % a.tiles);
-    id /= a.tiles;
-    const int h = (int)(id % a.b.n_kv), s = (int)(id / a.b.n_kv);
-    const int start = a.b.starts[s], count = a.b.starts[s + 1] - start;
-    if (start < 0 || start >= a.rows) return;
-    const int64_t pairs = (int64_t)min(min(count, a.max_rows), a.rows - start) * a.gq;
-    const int64_t f0 = (int64_t)tile * 16;
-    if (f0 >= pairs) return;
-    const int len = a.b.lens[s];
-    // positions lo .. hi - 1 are seen by this lane's row; those of the tile's
-    // first and last row bound all others
-    const int64_t first_pos = (int64_t)len - count;
-    auto see_hi = [&](int64_t i) { return (int)min<int64_t>(max<int64_t>(first_pos + i + 1, 0), a.b.cap); };
-    auto see_lo = [&](int64_t i) {
-        return a.window ? (int)min<int64_t>(max<int64_t>(first_pos + i + 1 - a.window, 0), a.b.cap) : 0;
-    };
-    const int64_t f = f0 + col;
-    const bool active = f < pairs;
-    const int64_t row_i = (active ? f : pairs - 1) / a.gq;
-    const int head = h * a.gq + (int)((active ? f : pairs - 1) - row_i * a.gq);
-    const int lo = see_lo(row_i), hi = see_hi(row_i);
-    const int64_t i_first = f0 / a.gq, i_last = (min<int64_t>(f0 + 15, pairs - 1)) / a.gq;
-    const int lo_all = see_lo(i_last), hi_all = see_hi(i_first);  // seen by every row: lo_all .. hi_all - 1
-    const int valid = min(max(len, 0), a.b.cap);
-    const int g_lo = see_lo(i_first) / kGroup, g_hi = (see_hi(i_last) + kGroup - 1) / kGroup;
-    const int per = (max(g_hi - g_lo, 0) + a.nsplit - 1) / a.nsplit;
-    const int g_begin = g_lo + split * per, g_end = min(g_begin + per, g_hi);
-
-    // the query row as B operands: block b, dimensions 8 quarter .. + 7
-    half8 q[P][NB];
-    float sc;
-    {
-        float x[NB][8];
-        float amax = 0.f;
-        const int64_t base = (int64_t)(start + row_i) * a.q_row + head * a.q_head + quarter * 8;
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            load_q8(a, base + b * 32, x[b]);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float m = fabsf(x[b][e]);
-                amax = m == m ? fmaxf(amax, m) : __builtin_inff();
-            }
-        }
-        amax = quarters_max(amax);
-        const int ex = row_exponent(amax);
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float y = ldexpf(x[b][e], ex);
-                const _Float16 top = (_Float16)y;
-                q[0][b][e] = top;
-                if constexpr (P == 2) q[1][b][e] = (_Float16)(y - (float)top);
-            }
-        }
-        sc = ldexpf(a.scale * 1.44269504088896340736f, -ex);
+    Q4Place pl;
+    if (!head_place(a, lane, shares, &pl)) return;
+    const Q4Rows& r = pl.r;
+    const int lo_all = r.see.lo(row_of(a, r.pairs - 1)), hi_all = r.see.hi(0);  // seen by every row: lo_all .. hi_all - 1
+    const Q4Groups groups(a, pl.s, pl.h, pl.g_end);
+    const Q4Bits bits;
+    Q4Tile<NB, P> t;
+    uint32_t k[2 * NB], ks[NB], v[2 * NB], vs[4 * NB];
+    int g = pl.g_begin + wave;
+    const uint8_t *gp = nullptr, *next = nullptr;
+    int id = -1;  // page id of the group after next
+    if (g < pl.g_end) {
+        const int id0 = groups.id(a, g), id1 = groups.id(a, g + 4);
+        id = groups.id(a, g + 8);
+        gp = groups.at(a, g, id0), next = groups.at(a, g + 4, id1);
+        // loads go somewhere in any case: a group that is not there is read as
+        // the cache's first, and hidden
+        load_k<NB>(gp ? gp : a.b.cache, lane, k, ks);
+        load_v<NB>(gp ? gp : a.b.cache, lane, v, vs);
     }
+    t.init(a, r.see, r.start, pl.h, col, r.pairs, quarter);
 
-    float m_run = -__builtin_inff(), l_run = 0.f;
-    f32x4 acc[2 * NB];
-#pragma unroll
-    for (int j = 0; j < 2 * NB; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    for (int g = g_begin + wave; g < g_end; g += 4) {
-        const uint8_t* gp = group_ptr(a.b, s, h, g);
-        if (!gp) continue;  // no page there: not seen
-        Q4Raw<NB> r;
-        load_group<NB>(gp, lane, r);
+    for (; g < pl.g_end; g += 4) {
+        const uint8_t* from = next ? next : a.b.cache;
+        const uint8_t* after = groups.at(a, g + 8, id);
+        id = groups.id(a, g + 12);
         // scores: rows tokens, columns query rows
-        f32x4 st[2];
+        f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            st[half] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < NB; b++) {
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const int si = half * NB + b;
-                const _Float16 ds = __builtin_bit_cast(half2v, r.ks[si / 2])[si % 2];
-                const half2v d = {ds, ds}, dm = d * (_Float16)-24;
-                const uint32_t w = r.k[2 * b + half];
-                const half8 kk = join8(held(pair16(w, 0), d, dm), held(pair16(w, 1), d, dm),
-                                       held(pair16(w, 2), d, dm), held(pair16(w, 3), d, dm));
+            for (int half = 0; half < 2; half++) {
+                const half8 kk = held_k(bits, k[2 * b + half], k_scale<NB>(ks, half, b));
 #pragma unroll
-                for (int p = 0; p < P; p++)
-                    st[half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, q[p][b], st[half], 0, 0, 0);
+                for (int p = 0; p < P; p++) st[half] = mfma16(kk, t.q[p][b], st[half]);
             }
         }
+        load_k<NB>(from, lane, k, ks);
         const int t0 = g * kGroup;
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = st[i / 4][i % 4] * sc;
-        if (t0 < lo_all || t0 + kGroup > hi_all) {  // some row sees only a part
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int t = t0 + i / 4 * 16 + quarter * 4 + i % 4;
-                x[i] = t >= lo && t < hi ? x[i] : -__builtin_inff();
-            }
-            // what is behind the sequence's end is anything: no scale may be NaN
+        if (!gp || t0 < lo_all || t0 + kGroup > hi_all) {  // some row sees only a part
+            t.hide(st, gp ? t0 : -1 - kGroup, quarter);
+            const int valid = gp ? r.valid : 0;
             if (t0 + kGroup > valid) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const int t = t0 + j / 2 * 16 + quarter * 4 + j % 2 * 2;
-                    const uint32_t keep = (t < valid ? 0xFFFFu : 0u) | (t + 1 < valid ? 0xFFFF0000u : 0u);
+                    const uint32_t keep = keep_mask(t0, quarter, j, valid);
 #pragma unroll
-                    for (int b = 0; b < NB; b++) r.vs[4 * b + j] &= keep;
+                    for (int b = 0; b < NB; b++) vs[4 * b + j] &= keep;
                 }
             }
         }
-        float mx = x[0];
+        half8 w[P];
+        t.weigh(st, w);
 #pragma unroll
-        for (int i = 1; i < 8; i++) mx = fmaxf(mx, x[i]);
-        mx = quarters_max(mx);
-        if (__any(mx > m_run)) {
-            const float m_new = fmaxf(m_run, mx);
-            const float m_ref = m_new == -__builtin_inff() ? 0.f : m_new;
-            const float f_old = exp2f(m_run - m_ref);
-            m_run = m_new;
-            l_run *= f_old;
-#pragma unroll
-            for (int j = 0; j < 2 * NB; j++) acc[j] *= f_old;
-        }
-        const float m_ref = (m_run == -__builtin_inff() ? 0.f : m_run) - kPShift;
-        half8 pw[P];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float w = exp2f(x[i] - m_ref);
-            l_run += w;
-            const _Float16 top = (_Float16)w;
-            pw[0][i] = top;
-            if constexpr (P == 2) pw[1][i] = (_Float16)(w - (float)top);
-        }
+        for (int p = 0; p < P; p++) t.l = mfma16(ones8(), w[p], t.l);
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            half2v d[4], dm[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) d[j] = as_half2(r.vs[4 * b + j]), dm[j] = d[j] * (_Float16)-24;
+            half8 vv[2];
+            held_v(bits, v[2 * b], v[2 * b + 1], &vs[4 * b], vv);
 #pragma unroll
             for (int z = 0; z < 2; z++) {
-                const uint32_t w0 = r.v[2 * b], w1 = r.v[2 * b + 1];
-                const half8 vv = join8(held(pair16(w0, z), d[0], dm[0]), held(pair16(w0, z + 2), d[1], dm[1]),
-                                       held(pair16(w1, z), d[2], dm[2]), held(pair16(w1, z + 2), d[3], dm[3]));
 #pragma unroll
-                for (int p = 0; p < P; p++)
-                    acc[2 * b + z] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pw[p], acc[2 * b + z], 0, 0, 0);
+                for (int p = 0; p < P; p++) t.acc[2 * b + z] = mfma16(vv[z], w[p], t.acc[2 * b + z]);
             }
         }
+        load_v<NB>(from, lane, v, vs);
+        gp = next, next = after;
     }
-    l_run = quarters_sum(l_run);
 
     // join the four waves
-    if (quarter == 0) red_ml[wave][col][0] = m_run, red_ml[wave][col][1] = l_run;
-#pragma unroll
-    for (int j = 0; j < 2 * NB; j++) *(f32x4*)&red_acc[wave][col][j * 16 + quarter * 4] = acc[j];
-    __syncthreads();
     constexpr int kQuads = hd / 4;
-    for (int u = threadIdx.x; u < 16 * kQuads; u += 256) {
-        const int c = u / kQuads, d4 = u % kQuads * 4;
-        const int64_t fc = f0 + c;
-        if (fc >= pairs) continue;
-        float m = -__builtin_inff();
+    if (quarter == 0) red_ml[wave][col][0] = t.m, red_ml[wave][col][1] = t.l[0];
 #pragma unroll
-        for (int w = 0; w < 4; w++) m = fmaxf(m, red_ml[w][c][0]);
+    for (int j = 0; j < 2 * NB; j++) *(f32x4*)&red_acc[wave][col][j * 16 + quarter * 4] = t.acc[j];
+    __syncthreads();
+    for (int u = threadIdx.x; u < 16 * kQuads; u += 256) {
+        const int f = u / kQuads, d4 = u % kQuads * 4;
+        if (f >= r.pairs) continue;
+        float m = -__builtin_inff();  // never NaN: a NaN score is in the sums alone
+#pragma unroll
+        for (int w = 0; w < 4; w++) m = fmaxf(m, red_ml[w][f][0]);
         const float m_ref = m == -__builtin_inff() ? 0.f : m;
         float l = 0.f, o[4] = {};
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            const float e = exp2f(red_ml[w][c][0] - m_ref);
-            l += e * red_ml[w][c][1];
+            const float e = __builtin_amdgcn_exp2f(red_ml[w][f][0] - m_ref);
+            l = fmaf(e, red_ml[w][f][1], l);
+            const f32x4 x = *(const f32x4*)&red_acc[w][f][d4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = fmaf(e, red_acc[w][c][d4 + i], o[i]);
+            for (int i = 0; i < 4; i++) o[i] = fmaf(e, x[i], o[i]);
         }
-        const int64_t i = fc / a.gq;
-        const int hh = h * a.gq + (int)(fc - i * a.gq);
-        if (a.nsplit == 1) {
-            const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that sees nothing is zero
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[e] *= inv;
-            store_o4(a, (int64_t)(start + i) * a.o_row + hh * a.o_head + d4, o);
+        store_pair(a, r, pl.h, f, pl.part, d4, m, l, o);
+    }
+}
+
+// Many pairs: a workgroup's four waves take 16 NT pairs each and share the held
+// values of TG groups at a time, converted once into LDS in operand order (one
+// 16-byte piece a lane, read and written without bank conflicts); two buffers,
+// the next groups converted into one and the ones after on their way from
+// memory while the other is worked on. Each wave converts K or V, of one
+// group (TG 2) or of a part of the blocks (TG 1).
+template <int NB, int P, int NT, int TG>
+__global__ void __launch_bounds__(256) kv_q4_rows_kernel(Q4Attn a, int shares) {
+    constexpr int B0 = TG == 2 || NB < 2 ? NB : (NB / 2 + 1) / 2 * 2;  // blocks of the first wave of a kind
+    __shared__ half8 kf[2][TG][2 * NB][64], vf[2][TG][2 * NB][64];
+    __shared__ int have[2][TG];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, quarter = lane >> 4;
+    Q4Place pl;
+    if (!head_place(a, lane, shares, &pl)) return;
+    const Q4Bits bits;
+    const Q4Rows& r = pl.r;
+    const int f_wave = pl.f0 + wave * (16 * NT);
+    const bool active = f_wave < r.pairs;
+    const int i_first = row_of(a, f_wave), i_last = row_of(a, min(f_wave + 16 * NT, r.pairs) - 1);
+    int lo_any = 0, hi_any = 0, lo_all = 0, hi_all = 0;  // seen by any, by every row of the wave
+    if (active) {
+        lo_any = r.see.lo(i_first), hi_any = r.see.hi(i_last);
+        lo_all = r.see.lo(i_last), hi_all = r.see.hi(i_first);
+    }
+    const Q4Groups groups(a, pl.s, pl.h, pl.g_end);
+    const bool is_v = wave & 1;
+    const int part = wave >> 1;  // group of the step (TG 2), part of the blocks (TG 1)
+
+    uint32_t c[2 * B0], sc[4 * B0 > NB ? 4 * B0 : NB];
+    const uint8_t* gp = nullptr;
+    int page = -1;              // page id of this wave's group of the next fetch
+    auto fetch = [&](int g) {  // this wave's share of the step at g, and the id for the one after
+        const int gg = TG == 2 ? g + part : g;
+        gp = groups.at(a, gg, page);
+        page = groups.id(a, gg + TG);
+        if (!gp) return;
+        if (is_v) {
+            if (TG == 2 || part == 0) load_v<NB, 0, B0>(gp, lane, c, sc);
+            else if constexpr (B0 < NB) load_v<NB, B0, NB>(gp, lane, c, sc);
         } else {
-            const int64_t p = ((int64_t)(start + i) * a.n_heads + hh) * a.nsplit + split;
-            *(f32x4*)(a.part_acc + p * hd + d4) = f32x4{o[0], o[1], o[2], o[3]};
-            if (d4 == 0) a.part_ml[2 * p] = m, a.part_ml[2 * p + 1] = l;
+            load_words<NB>(gp + 1024 * NB + lane % 16 * 4 * NB, sc);
+            if (TG == 2 || part == 0) load_codes<NB, 0, B0>(gp, lane, c);
+            else if constexpr (B0 < NB) load_codes<NB, B0, NB>(gp, lane, c);
+        }
+    };
+    auto put_v = [&](half8 (*to)[64], int b, int n) {
+#pragma unroll
+        for (int i = 0; i < B0; i++) {
+            if (i >= n) break;
+            half8 vv[2];
+            held_v(bits, c[2 * i], c[2 * i + 1], &sc[4 * i], vv);
+            to[2 * (b + i)][lane] = vv[0];
+            to[2 * (b + i) + 1][lane] = vv[1];
+        }
+    };
+    auto put_k = [&](half8 (*to)[64], auto first, auto count) {
+        constexpr int b = decltype(first)::value, n = decltype(count)::value;
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const int si = half * NB + b + i;
+                to[half * NB + b + i][lane] = held_k(bits, c[2 * i + half], as_half2(sc[si / 2])[si % 2]);
+            }
+        }
+    };
+    auto convert = [&](int g, int buf) {
+        const int gg = TG == 2 ? part : 0;
+        if (is_v && (TG == 2 || part == 0) && lane == 0) have[buf][gg] = gp != nullptr;
+        if (!gp) return;
+        if (is_v) {
+            const int t0 = (g + gg) * kGroup;
+            if (t0 + kGroup > r.valid) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t keep = keep_mask(t0, quarter, j, r.valid);
+#pragma unroll
+                    for (int b = 0; b < B0; b++) sc[4 * b + j] &= keep;
+                }
+            }
+            if (TG == 2 || part == 0) put_v(vf[buf][gg], 0, B0);
+            else put_v(vf[buf][gg], B0, NB - B0);
+        } else {
+            if (TG == 2 || part == 0) put_k(kf[buf][gg], std::integral_constant<int, 0>{}, std::integral_constant<int, B0>{});
+            else put_k(kf[buf][gg], std::integral_constant<int, B0>{}, std::integral_constant<int, NB - B0>{});
+        }
+    };
+
+    if (pl.g_begin < pl.g_end) {
+        page = groups.id(a, TG == 2 ? pl.g_begin + part : pl.g_begin);
+        fetch(pl.g_begin);
+    }
+    Q4Tile<NB, P> t[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) t[n].init(a, r.see, r.start, pl.h, f_wave + 16 * n + col, r.pairs, quarter);
+    if (pl.g_begin < pl.g_end) {
+        convert(pl.g_begin, 0);
+        fetch(pl.g_begin + TG);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int g = pl.g_begin; g < pl.g_end; g += TG, buf ^= 1) {
+        if (g + TG < pl.g_end) {
+            convert(g + TG, buf ^ 1);
+            fetch(g + 2 * TG);
+        }
+#pragma unroll
+        for (int gg = 0; gg < TG; gg++) {
+            const int t0 = (g + gg) * kGroup;
+            // nothing there, or nothing that a row of this wave sees
+            if (!__builtin_amdgcn_readfirstlane(have[buf][gg]) || t0 >= hi_any || t0 + kGroup <= lo_any) continue;
+            f32x4 st[NT][2];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) st[n][half] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const half8 k = kf[buf][gg][half * NB + b][lane];
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+#pragma unroll
+                        for (int p = 0; p < P; p++) st[n][half] = mfma16(k, t[n].q[p][b], st[n][half]);
+                    }
+                }
+            }
+            if (t0 < lo_all || t0 + kGroup > hi_all) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) t[n].hide(st[n], t0, quarter);
+            }
+            half8 w[NT][P];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                t[n].weigh(st[n], w[n]);
+#pragma unroll
+                for (int p = 0; p < P; p++) t[n].l = mfma16(ones8(), w[n][p], t[n].l);
+            }
+#pragma unroll
+            for (int j = 0; j < 2 * NB; j++) {
+                const half8 v = vf[buf][gg][j][lane];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int p = 0; p < P; p++) t[n].acc[j] = mfma16(v, w[n][p], t[n].acc[j]);
+                }
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int f = f_wave + 16 * n + col;
+        if (f >= r.pairs) continue;
+#pragma unroll
+        for (int j = 0; j < 2 * NB; j++) {
+            float o[4] = {t[n].acc[j][0], t[n].acc[j][1], t[n].acc[j][2], t[n].acc[j][3]};
+            store_pair(a, r, pl.h, f, pl.part, j * 16 + quarter * 4, t[n].m, t[n].l[0], o);
         }
     }
 }
 
-// The shares of a (row, head) joined: a quarter wave of hd / 4 lanes each.
-__global__ void __launch_bounds__(256) kv_q4_join_kernel(Q4Attn a, int rows) {
-    const int hd = a.b.hd, quads = hd / 4;
-    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t pr = u / quads;
-    const int d4 = (int)(u - pr * quads) * 4;
-    if (pr >= (int64_t)rows * a.n_heads) return;
-    const int row = (int)(pr / a.n_heads), head = (int)(pr - (int64_t)row * a.n_heads);
-    const int s = seq_of(a.b, row);
-    if (s < 0 || row - a.b.starts[s] >= a.max_rows) return;
-    const float* ml = a.part_ml + pr * a.nsplit * 2;
-    const float* pa = a.part_acc + pr * a.nsplit * hd + d4;
-    float m = -__builtin_inff();  // never NaN: a NaN score is in the sums alone
-    for (int i = 0; i < a.nsplit; i++) m = fmaxf(m, ml[2 * i]);
-    const float m_ref = m == -__builtin_inff() ? 0.f : m;
-    float l = 0.f, o[4] = {};
-    for (int i = 0; i < a.nsplit; i++) {
-        const float e = exp2f(ml[2 * i] - m_ref);
-        l += e * ml[2 * i + 1];
-        const f32x4 x = *(const f32x4*)(pa + (int64_t)i * hd);
-#pragma unroll
-        for (int j = 0; j < 4; j++) o[j] = fmaf(e, x[j], o[j]);
+// The parts of a (row, head) joined by one wave: lane i weighs part i (there
+// are at most 64), then the lanes take four values each of 256 / hd parts at a
+// time. `shares`: workgroups of the even shares.
+constexpr int kMaxSplit = 64;
+__global__ void __launch_bounds__(256) kv_q4_join_kernel(Q4Attn a, int shares) {
+    const int hd = a.b.hd, lane = threadIdx.x & 63;
+    const int64_t pr = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (pr >= (int64_t)a.rows * a.n_heads) return;
+    const int row = udiv((int)pr, a.n_heads), head = (int)pr - row * a.n_heads;  // rows times heads fits 31 bits
+    const int s = __builtin_amdgcn_readfirstlane(wave_search(a.b.n_seq, lane, row, [&](int i) { return a.b.starts[i]; }));
+    const int i = row - a.b.starts[s];
+    Q4Rows r;
+    if (i < 0 || row >= a.b.starts[s + 1] || !rows_of(a, s, &r)) return;
+    const int f = i * a.gq + head - udiv(head, a.gq) * a.gq;
+    if (f >= r.pairs) return;
+    int n;
+    if (a.chunk == 0) {
+        const Q4Cut c = cut_of(a, lane, shares);
+        int base = 0, lo, groups = c.n, before = c.before, run = 0;
+        for (; s >= base + 64; base += 64) {
+            run += lane_value(before + groups, 63);
+            seq_groups(a, base + 64 + lane, &lo, &groups);
+            before = wave_before(groups, lane);
+        }
+        groups = lane_value(groups, s - base);
+        const int x = (run + lane_value(before, s - base)) * a.b.n_kv + udiv(head, a.gq) * groups;
+        n = groups == 0 ? 0 : udiv(x + groups - 1, c.size) - udiv(x, c.size) + 1;
+        if (n == 1) return;  // stored already
+    } else {
+        const int f0 = f - f % a.tile_pairs;
+        int g_lo, g_hi;
+        tile_groups(r.see, row_of(a, f0), row_of(a, min(f0 + a.tile_pairs, r.pairs) - 1), &g_lo, &g_hi);
+        n = min((max(g_hi - g_lo, 0) + a.chunk - 1) / a.chunk, a.nsplit);
     }
+    const float* ml = a.part_ml + pr * a.nsplit * 2;
+    const float m_i = lane < n ? ml[2 * lane] : -__builtin_inff();
+    const float l_i = lane < n ? ml[2 * lane + 1] : 0.f;
+    const int quads = hd / 4, per = 64 / quads;  // hd 96 and 192: lanes past the last quad repeat one
+    const int d4 = lane % quads * 4, first = min(lane / quads, per - 1);
+    float o[4] = {};
+    const float* pa = a.part_acc + pr * a.nsplit * hd + d4;
+    const float m = wave_max(m_i);
+    const float e_i = __builtin_amdgcn_exp2f(m_i - (m == -__builtin_inff() ? 0.f : m));  // 0 from part n on
+    const float l = wave_sum(e_i * l_i);
+    for (int j = 0; j < n; j += 8 * per) {
+        f32x4 x[8];
+#pragma unroll
+        for (int c = 0; c < 8; c++) x[c] = *(const f32x4*)(pa + (int64_t)min(j + c * per + first, n - 1) * hd);
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            const int k = j + c * per + first;
+            const float e = __shfl(e_i, min(k, 63), 64);
+#pragma unroll
+            for (int d = 0; d < 4; d++) o[d] = fmaf(k < n ? e : 0.f, x[c][d], o[d]);
+        }
+    }
+    // sum over the parts' lanes
+    for (int c = 0; c < 4; c++) {
+        float v = o[c];
+        for (int k = 1; k < per; k++) v += __shfl(o[c], min(lane + k * quads, 63), 64);
+        o[c] = v;
+    }
+    if (lane >= quads) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < 4; e++) o[e] *= inv;
+    for (int c = 0; c < 4; c++) o[c] *= inv;
     store_o4(a, (int64_t)row * a.o_row + head * a.o_head + d4, o);
 }
 
@@ -713,24 +1381,61 @@ int32_t make_batch(Q4Batch* b, const uint8_t* cache, size_t cache_len, size_t n_
     if ((uintptr_t)pages % 4 || (uintptr_t)starts % 4 || (uintptr_t)lens % 4)
         return set_error(MIVI_ERR_INVALID_ARGUMENT, "table, starts or lens not 4-byte aligned");
     *b = Q4Batch{(uint8_t*)cache, pages,     starts,        lens,    (int64_t)pages_stride, (int64_t)n_pages,
-                 (int64_t)page_bytes, (int)n_seq, (int)n_kv, (int)hd, (int)(page_tokens / kGroup), (int)cap};
+                 (int64_t)page_bytes, (int)n_seq, (int)n_kv, (int)hd, (int)(page_tokens / kGroup),
+                 0, (int)cap};
+    if (b->gpp > 1) b->gpp_inv = (uint32_t)((1ull << 32) / b->gpp + 1);
     return MIVI_OK;
 }
 
-// Shares of a sequence's groups: enough workgroups for the card where rows and
-// heads make few.
-int split_count(size_t n_seq, size_t max_rows, size_t gq, size_t n_kv, size_t cap) {
-    const size_t tiles = (max_rows * gq + 15) / 16;
-    const size_t wgs = std::max<size_t>(1, n_seq * n_kv * tiles);
-    const size_t groups = (cap + kGroup - 1) / kGroup;
-    const size_t want = (4 * (size_t)num_cus() + wgs - 1) / wgs;
-    return (int)std::max<size_t>(1, std::min<size_t>({want, (groups + 3) / 4, 64}));
+// How an attention call is laid out.
+struct Q4Plan {
+    int nt;  // row tiles of 16 a wave of kv_q4_rows_kernel, 0: kv_q4_step_kernel
+    size_t tile_pairs, tiles, chunk, nsplit, shares, share_min, grid;
+};
+
+Q4Plan attn_plan(size_t n_seq, size_t max_rows, size_t gq, size_t n_kv, size_t cap, size_t window) {
+    Q4Plan p = {};
+    const size_t pairs = max_rows * gq;
+    p.nt = pairs <= 16 ? 0 : pairs <= 64 ? 1 : 2;
+    p.tile_pairs = p.nt ? 64 * p.nt : 16;
+    p.tiles = (pairs + p.tile_pairs - 1) / p.tile_pairs;
+    // groups that a tile can see
+    size_t tokens = cap;
+    if (window) tokens = std::min(cap, std::min(window, cap) + p.tile_pairs / gq + 1 + 2 * kGroup);
+    const size_t groups = std::max<size_t>(1, (tokens + kGroup - 1) / kGroup), cus = (size_t)num_cus();
+    size_t all, heads;  // of one tile a sequence
+    if (__builtin_mul_overflow(n_seq, n_kv, &heads) || __builtin_mul_overflow(heads, groups, &all)) all = SIZE_MAX;
+    if (p.tiles == 1 && all <= (size_t)INT32_MAX / 2) {
+        // even shares: four workgroups a CU, each at least one step of every wave
+        p.share_min = 4;
+        p.shares = std::min(cus * 4, std::max<size_t>((all + p.share_min - 1) / p.share_min, 1));
+        p.nsplit = std::min<size_t>({(size_t)kMaxSplit, p.shares / n_kv + 2, groups / p.share_min + 2});
+        p.grid = p.shares + heads;
+        return p;
+    }
+    // tiles by themselves; shares of their groups where they are too few for the card
+    const size_t goal = 2 * cus;
+    size_t wgs;
+    if (__builtin_mul_overflow(heads, p.tiles, &wgs)) wgs = SIZE_MAX;
+    size_t chunk = wgs >= goal ? groups : (wgs * groups + goal - 1) / goal;
+    chunk = std::max(chunk, (groups + kMaxSplit - 1) / kMaxSplit);
+    p.chunk = (chunk + 3) / 4 * 4;
+    p.nsplit = (groups + p.chunk - 1) / p.chunk;
+    if (__builtin_mul_overflow(wgs, p.nsplit, &p.grid)) p.grid = SIZE_MAX;
+    return p;
 }
 
+template <int NB, int P>
+void launch_attn(const Q4Attn& a, unsigned grid, int shares, int nt, hipStream_t s) {
+    constexpr int TG = NB <= 4 ? 2 : 1;
+    if (nt == 0) kv_q4_step_kernel<NB, P><<<grid, 256, 0, s>>>(a, shares);
+    else if (nt == 1) kv_q4_rows_kernel<NB, P, 1, 1><<<grid, 256, 0, s>>>(a, shares);
+    else kv_q4_rows_kernel<NB, P, 2, TG><<<grid, 256, 0, s>>>(a, shares);
+}
 template <int NB>
-void launch_attn(const Q4Attn& a, unsigned grid, int planes, hipStream_t s) {
-    if (planes == 2) kv_q4_attn_kernel<NB, 2><<<grid, 256, 0, s>>>(a);
-    else kv_q4_attn_kernel<NB, 1><<<grid, 256, 0, s>>>(a);
+void launch_attn(const Q4Attn& a, unsigned grid, const Q4Plan& p, int planes, hipStream_t s) {
+    if (planes == 2) launch_attn<NB, 2>(a, grid, (int)p.shares, p.nt, s);
+    else launch_attn<NB, 1>(a, grid, (int)p.shares, p.nt, s);
 }
 
 }  // namespace
@@ -760,11 +1465,16 @@ extern "C" int32_t mivi_hip_kv_q4_append(uint8_t* cache, size_t cache_len, size_
     clear_error();
     const size_t e = type_bytes(type);
     const int wk = wide_ok(k, k_row_stride, k_head_stride, e, 16), wv = wide_ok(v, v_row_stride, v_head_stride, e, 16);
-    const dim3 grid((unsigned)blocks, 2);
     hipStream_t s = (hipStream_t)stream;
-#define APPEND(T)                                                                                                   \
-    kv_q4_append_kernel<T><<<grid, 256, 0, s>>>(b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride,             \
-                                                (int64_t)v_row_stride, (int64_t)v_head_stride, (int)rows, wk, wv)
+    // A wave a group where the call has 8 rows a sequence or more, else 8 values
+    // a lane wherever they lie.
+    const bool by_group = rows >= 8 * n_seq;
+    const dim3 grid = by_group ? dim3((unsigned)(rows / kGroup + 2 * n_seq), (unsigned)((2 * n_kv_heads + 3) / 4))
+                               : dim3((unsigned)blocks, 2);
+#define APPEND(T)                                                                                                      \
+    (by_group ? kv_q4_append_groups_kernel<T> : kv_q4_append_kernel<T>)<<<grid, 256, 0, s>>>(                           \
+        b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride, (int64_t)v_row_stride, (int64_t)v_head_stride,       \
+        (int)rows, wk, wv)
     if (type == MIVI_GGML_F32) APPEND(MIVI_GGML_F32);
     else if (type == MIVI_GGML_F16) APPEND(MIVI_GGML_F16);
     else APPEND(MIVI_GGML_BF16);
@@ -793,11 +1503,16 @@ extern "C" int32_t mivi_hip_kv_q4_read(const uint8_t* cache, size_t cache_len, s
     clear_error();
     const size_t e = type_bytes(type);
     const int wk = wide_ok(k, k_row_stride, k_head_stride, e, 16), wv = wide_ok(v, v_row_stride, v_head_stride, e, 16);
-    const dim3 grid((unsigned)blocks, 2);
     hipStream_t s = (hipStream_t)stream;
-#define READ(T)                                                                                                   \
-    kv_q4_read_kernel<T><<<grid, 256, 0, s>>>(b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride,             \
-                                              (int64_t)v_row_stride, (int64_t)v_head_stride, (int)rows, wk, wv)
+    // A wave a group where the call has 8 rows a sequence or more, else 8 values
+    // a lane wherever they lie.
+    const bool by_group = rows >= 8 * n_seq;
+    const dim3 grid = by_group ? dim3((unsigned)(rows / kGroup + 2 * n_seq), (unsigned)((2 * n_kv_heads + 3) / 4))
+                               : dim3((unsigned)blocks, 2);
+#define READ(T)                                                                                                      \
+    (by_group ? kv_q4_read_groups_kernel<T> : kv_q4_read_kernel<T>)<<<grid, 256, 0, s>>>(                           \
+        b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride, (int64_t)v_row_stride, (int64_t)v_head_stride,       \
+        (int)rows, wk, wv)
     if (type == MIVI_GGML_F32) READ(MIVI_GGML_F32);
     else if (type == MIVI_GGML_F16) READ(MIVI_GGML_F16);
     else READ(MIVI_GGML_BF16);
@@ -807,11 +1522,11 @@ extern "C" int32_t mivi_hip_kv_q4_read(const uint8_t* cache, size_t cache_len, s
 }
 
 extern "C" size_t mivi_hip_kv_q4_attention_workspace(size_t n_seq, size_t rows, size_t max_rows, size_t n_heads,
-                                                     size_t n_kv_heads, size_t head_dim, size_t max_tokens) {
-    if (n_kv_heads == 0 || n_heads == 0 || n_heads % n_kv_heads || rows == 0 || n_seq == 0) return 0;
-    max_rows = std::min(max_rows, rows);
-    const int ns = split_count(n_seq, max_rows, n_heads / n_kv_heads, n_kv_heads, max_tokens);
-    return ns == 1 ? 0 : rows * n_heads * ns * (head_dim + 2) * sizeof(float);
+                                                     size_t n_kv_heads, size_t head_dim, size_t max_tokens,
+                                                     size_t window) {
+    if (n_kv_heads == 0 || n_heads == 0 || n_heads % n_kv_heads || rows == 0 || n_seq == 0 || max_rows == 0) return 0;
+    const Q4Plan p = attn_plan(n_seq, std::min(max_rows, rows), n_heads / n_kv_heads, n_kv_heads, max_tokens, window);
+    return p.nsplit == 1 ? 0 : rows * n_heads * p.nsplit * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int32_t mivi_hip_kv_q4_attention(
@@ -832,18 +1547,16 @@ extern "C" int32_t mivi_hip_kv_q4_attention(
         (rc = check_tensor("out", out, out_len, type, rows, out_row_stride, n_heads, out_head_stride, head_dim, true)))
         return rc;
     max_rows = std::min(max_rows, rows);
-    const size_t gq = n_heads / n_kv_heads;
-    size_t cap = pages_per_seq * page_tokens;
-    const size_t need = mivi_hip_kv_q4_attention_workspace(n_seq, rows, max_rows, n_heads, n_kv_heads, head_dim, cap);
+    const size_t gq = n_heads / n_kv_heads, cap = pages_per_seq * page_tokens;
+    const int planes = type == MIVI_GGML_F32 ? 2 : 1;
+    const Q4Plan p = attn_plan(n_seq, max_rows, gq, n_kv_heads, cap, window);
+    const size_t need =
+        mivi_hip_kv_q4_attention_workspace(n_seq, rows, max_rows, n_heads, n_kv_heads, head_dim, cap, window);
     if (workspace_bytes < need) return err_buffer_too_small(need, workspace_bytes);
     if (need && !workspace) return set_error(MIVI_ERR_INVALID_ARGUMENT, "null workspace");
     if (need && (uintptr_t)workspace % 16)
         return set_error(MIVI_ERR_INVALID_ARGUMENT, "workspace not 16-byte aligned");
-    const int ns = split_count(n_seq, max_rows, gq, n_kv_heads, cap);
-    const size_t tiles = (max_rows * gq + 15) / 16;
-    const size_t grid = tiles * n_seq * n_kv_heads * ns;
-    const size_t join = (rows * n_heads * (head_dim / 4) + 255) / 256;
-    if (grid > (size_t)INT32_MAX || join > (size_t)INT32_MAX) return err_overflow();
+    if (p.grid > (size_t)INT32_MAX || rows * n_heads > (size_t)INT32_MAX - 4096) return err_overflow();
     clear_error();
     a.q = q, a.out = out;
     a.q_row = (int64_t)q_row_stride, a.q_head = (int64_t)q_head_stride;
@@ -853,25 +1566,25 @@ extern "C" int32_t mivi_hip_kv_q4_attention(
     a.wide_q = wide_ok(q, q_row_stride, q_head_stride, e, 16);
     a.wide_o = wide_ok(out, out_row_stride, out_head_stride, e, 4 * e);
     a.n_heads = (int)n_heads, a.gq = (int)gq;
-    a.rows = (int)rows, a.max_rows = (int)max_rows, a.tiles = (int)tiles;
-    a.nsplit = ns;
+    a.rows = (int)rows, a.max_rows = (int)max_rows;
+    a.tiles = (int)p.tiles, a.tile_pairs = (int)p.tile_pairs;
+    a.nsplit = (int)p.nsplit, a.chunk = (int)p.chunk, a.share_min = (int)p.share_min;
     a.window = (int)std::min<size_t>(window, (size_t)INT32_MAX);
     a.scale = scale;
     a.part_acc = (float*)workspace;
-    a.part_ml = a.part_acc + rows * n_heads * ns * head_dim;
+    a.part_ml = a.part_acc + rows * n_heads * p.nsplit * head_dim;
     hipStream_t s = (hipStream_t)stream;
-    const int planes = type == MIVI_GGML_F32 ? 2 : 1;
     switch (head_dim / 32) {
-        case 1: launch_attn<1>(a, (unsigned)grid, planes, s); break;
-        case 2: launch_attn<2>(a, (unsigned)grid, planes, s); break;
-        case 3: launch_attn<3>(a, (unsigned)grid, planes, s); break;
-        case 4: launch_attn<4>(a, (unsigned)grid, planes, s); break;
-        case 6: launch_attn<6>(a, (unsigned)grid, planes, s); break;
-        default: launch_attn<8>(a, (unsigned)grid, planes, s); break;
+        case 1: launch_attn<1>(a, (unsigned)p.grid, p, planes, s); break;
+        case 2: launch_attn<2>(a, (unsigned)p.grid, p, planes, s); break;
+        case 3: launch_attn<3>(a, (unsigned)p.grid, p, planes, s); break;
+        case 4: launch_attn<4>(a, (unsigned)p.grid, p, planes, s); break;
+        case 6: launch_attn<6>(a, (unsigned)p.grid, p, planes, s); break;
+        default: launch_attn<8>(a, (unsigned)p.grid, p, planes, s); break;
     }
     MIVI_HIP_CHECK(hipGetLastError());
-    if (ns > 1) {
-        kv_q4_join_kernel<<<(unsigned)join, 256, 0, s>>>(a, (int)rows);
+    if (p.nsplit > 1) {
+        kv_q4_join_kernel<<<(unsigned)((rows * n_heads + 3) / 4), 256, 0, s>>>(a, (int)p.shares);
         MIVI_HIP_CHECK(hipGetLastError());
     }
     return MIVI_OK;

@@ -158,7 +158,7 @@ pub mod ffi {
             k_row_stride: usize, k_head_stride: usize, v: *mut c_void, v_len: usize, v_row_stride: usize,
             v_head_stride: usize, rows: usize, stream: *mut c_void) -> i32;
         pub fn mivi_hip_kv_q4_attention_workspace(n_seq: usize, rows: usize, max_rows: usize, n_heads: usize,
-            n_kv_heads: usize, head_dim: usize, max_tokens: usize) -> usize;
+            n_kv_heads: usize, head_dim: usize, max_tokens: usize, window: usize) -> usize;
         pub fn mivi_hip_kv_q4_attention(type_: i32, out: *mut c_void, out_len: usize, out_row_stride: usize,
             out_head_stride: usize, q: *const c_void, q_len: usize, q_row_stride: usize, q_head_stride: usize,
             rows: usize, max_rows: usize, n_heads: usize, scale: f32, window: usize, cache: *const u8, cache_len: usize, n_kv_heads: usize,

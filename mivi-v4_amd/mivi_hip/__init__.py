@@ -127,7 +127,7 @@ _sig = {
     "mivi_hip_kv_q4_page_bytes": ([_S, _S, _S], _S),
     "mivi_hip_kv_q4_append": (_kv_q4 + [_I, _P, _S, _S, _S, _P, _S, _S, _S, _S, _P], _I),
     "mivi_hip_kv_q4_read": (_kv_q4 + [_I, _P, _S, _S, _S, _P, _S, _S, _S, _S, _P], _I),
-    "mivi_hip_kv_q4_attention_workspace": ([_S] * 7, _S),
+    "mivi_hip_kv_q4_attention_workspace": ([_S] * 8, _S),
     "mivi_hip_kv_q4_attention": ([_I, _P, _S, _S, _S, _P, _S, _S, _S, _S, _S, _S, C.c_float, _S] + _kv_q4
                                  + [_P, _S, _P], _I),
     "mivi_hip_model_create": ([_P, _S, _S, _I, _S, C.POINTER(_P)], _I),

@@ -8,13 +8,10 @@ model appends its rows' K and V, then attends with the same starts and lens.
 """
 from __future__ import annotations
 
-import ctypes as C
-
-import torch
-
 from . import _check, _lib
 
-_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # GgmlType
+torch = None  # imported by the first cache: the rest of the package works without it
+_TYPES = {}   # torch dtype -> GgmlType
 _append = _lib.mivi_hip_kv_q4_append
 _read = _lib.mivi_hip_kv_q4_read
 _attention = _lib.mivi_hip_kv_q4_attention
@@ -33,65 +30,73 @@ class KvCacheQ4:
     `set_pages`). Both stay the caller's."""
 
     def __init__(self, data, pages, n_kv_heads: int, head_dim: int, page_tokens: int):
+        global torch
+        if torch is None:
+            import torch as t
+            _TYPES.update({t.float32: 0, t.float16: 1, t.bfloat16: 30})
+            torch = t
         if data.dtype != torch.uint8 or not data.is_contiguous() or not data.is_cuda:
             raise ValueError("data is a contiguous u8 GPU tensor")
         self.data, self.n_kv_heads, self.head_dim, self.page_tokens = data, n_kv_heads, head_dim, page_tokens
+        self.device = data.device
         self._geometry = (data.data_ptr(), data.numel(), n_kv_heads, head_dim, page_tokens)
         self.set_pages(pages)
 
     def set_pages(self, pages):
         if pages.dtype != torch.int32 or pages.dim() != 2 or (pages.shape[1] > 1 and pages.stride(1) != 1):
             raise ValueError("pages is a 2-D int32 tensor with contiguous rows")
-        if pages.device != self.data.device:
+        if pages.device != self.device:
             raise ValueError("pages and data are on different devices")
         self.pages = pages
         self._table = (pages.data_ptr(), pages.stride(0), pages.shape[1], pages.shape[0])
 
     def _batch(self, starts, lens):
-        n = self.pages.shape[0]
+        n = self._table[3]
         if starts.dtype != torch.int32 or lens.dtype != torch.int32 or not starts.is_contiguous() \
                 or not lens.is_contiguous():
             raise ValueError("starts and lens are contiguous int32 tensors")
         if starts.numel() != n + 1 or lens.numel() != n:
             raise ValueError(f"{n} sequences: starts has {starts.numel()} values, lens {lens.numel()}")
-        dev = self.data.device
-        if starts.device != dev or lens.device != dev:
+        if starts.device != self.device or lens.device != self.device:
             raise ValueError("starts, lens and the cache are on different devices")
         return self._geometry + self._table + (starts.data_ptr(), lens.data_ptr())
 
     def _rows(self, t, heads: int, what: str):
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim or t.stride(2) != 1:
+        shape, strides = t.shape, t.stride()
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or strides[2] != 1:
             raise ValueError(f"{what} is [rows, {heads}, {self.head_dim}] with a contiguous last dimension")
-        if t.device != self.data.device:
+        if t.device != self.device:
             raise ValueError(f"{what} and the cache are on different devices")
-        rs, hs = t.stride(0), t.stride(1)
+        rs, hs = strides[0], strides[1]
         # the elements from the first to the last: what a strided view spans
-        span = (t.shape[0] - 1) * rs + (heads - 1) * hs + self.head_dim if t.shape[0] else 0
+        span = (shape[0] - 1) * rs + (heads - 1) * hs + self.head_dim if shape[0] else 0
         return t.data_ptr(), span, rs, hs
 
 
-def _type(*tensors):
-    dt = tensors[0].dtype
-    if dt not in _TYPES or any(t.dtype != dt for t in tensors):
+def _type(a, b):
+    t = _TYPES.get(a.dtype)
+    if t is None or b.dtype != a.dtype:
         raise ValueError("tensors of one type: float32, float16 or bfloat16")
-    return _TYPES[dt]
+    return t
 
 
 def _call(fn, args, device, stream):
     """fn(*args, stream) on `device`: the given stream, or the current one there."""
     if stream is None:
-        raw = torch.cuda.current_stream(device).cuda_stream
+        raw = torch._C._cuda_getCurrentRawStream(device.index)
     elif isinstance(stream, int):
         raw = stream
     else:
         if stream.device != device:
             raise ValueError("the stream is on another device than the cache")
         raw = stream.cuda_stream
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            _check(fn(*args, raw))
+    if torch._C._cuda_getDevice() == device.index:
+        rc = fn(*args, raw)
     else:
-        _check(fn(*args, raw))
+        with torch.cuda.device(device):
+            rc = fn(*args, raw)
+    if rc:
+        _check(rc)
 
 
 def _kv(fn, cache, k, v, starts, lens, stream):
@@ -99,7 +104,7 @@ def _kv(fn, cache, k, v, starts, lens, stream):
         raise ValueError("k and v are of one shape")
     args = cache._batch(starts, lens) + (_type(k, v),) + cache._rows(k, cache.n_kv_heads, "k") \
         + cache._rows(v, cache.n_kv_heads, "v") + (k.shape[0],)
-    _call(fn, args, cache.data.device, stream)
+    _call(fn, args, cache.device, stream)
 
 
 def kv_q4_append(cache: KvCacheQ4, k, v, starts, lens, stream=None):
@@ -123,18 +128,17 @@ def kv_q4_attention(out, q, cache: KvCacheQ4, starts, lens, max_rows: int | None
     head_dim ** -0.5. workspace: a u8 GPU tensor of at least the bytes that
     mivi_hip_kv_q4_attention_workspace names (allocated here by default); calls
     that may overlap need their own. Returns out."""
-    if q.shape != out.shape:
-        raise ValueError("q and out are of one shape")
-    if q.dim() != 3:
-        raise ValueError("q is [rows, n_heads, head_dim]")
-    rows, heads = q.shape[0], q.shape[1]
+    shape = q.shape
+    if shape != out.shape or len(shape) != 3:
+        raise ValueError("q and out are [rows, n_heads, head_dim]")
+    rows, heads, _ = shape
     max_rows = rows if max_rows is None else min(max_rows, rows)
     if window < 0 or max_rows < 0:
         raise ValueError("window and max_rows are not negative")
     batch = cache._batch(starts, lens)
-    need = _workspace(cache.pages.shape[0], rows, max_rows, heads, cache.n_kv_heads, cache.head_dim,
-                      cache.pages.shape[1] * cache.page_tokens)
-    device = cache.data.device
+    need = _workspace(cache._table[3], rows, max_rows, heads, cache.n_kv_heads, cache.head_dim,
+                      cache._table[2] * cache.page_tokens, window)
+    device = cache.device
     if workspace is None and need:
         if stream is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=device)

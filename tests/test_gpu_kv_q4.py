@@ -529,7 +529,7 @@ def test_captured_steps_follow_their_lengths(hip):
     for _ in range(2):
         qkv = torch.randn((2, heads + 2 * kv, hd), generator=g).cuda()
         out = torch.empty((2, heads, hd), device="cuda")
-        need = hip.lib().mivi_hip_kv_q4_attention_workspace(2, 2, 1, heads, kv, hd, b.pages.shape[1] * page)
+        need = hip.lib().mivi_hip_kv_q4_attention_workspace(2, 2, 1, heads, kv, hd, b.pages.shape[1] * page, 0)
         ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
 
         def step():

@@ -93,7 +93,7 @@ def test_attention_refusals():
     full = rows_args(kv=4)
     assert attn(q=[A, full[1] - 1] + full[2:]) == 2
     assert attn(out=[None] + full[1:]) == 101
-    need = LIB.mivi_hip_kv_q4_attention_workspace(3, 7, 7, 4, 2, 64, 256)
+    need = LIB.mivi_hip_kv_q4_attention_workspace(3, 7, 7, 4, 2, 64, 256, 0)
     if need:
         assert attn(ws_bytes=need - 1) == 2 and mivi_hip.last_error().expected == need
         assert attn(ws=None, ws_bytes=need) == 101
@@ -109,9 +109,9 @@ def test_nothing_to_do_is_ok():
 
 def test_workspace_grows_with_the_batch():
     f = LIB.mivi_hip_kv_q4_attention_workspace
-    assert f(0, 7, 7, 4, 2, 64, 256) == 0 and f(1, 0, 0, 4, 2, 64, 256) == 0
-    assert f(1, 1, 1, 5, 2, 64, 256) == 0 and f(1, 1, 1, 4, 0, 64, 256) == 0
-    assert f(1, 1, 1, 32, 8, 64, 4096) > 0
+    assert f(0, 7, 7, 4, 2, 64, 256, 0) == 0 and f(1, 0, 0, 4, 2, 64, 256, 0) == 0
+    assert f(1, 1, 1, 5, 2, 64, 256, 0) == 0 and f(1, 1, 1, 4, 0, 64, 256, 0) == 0
+    assert f(1, 1, 1, 32, 8, 64, 4096, 0) > 0
 
 
 def test_python_refusals_on_host_tensors():

@@ -119,6 +119,36 @@ __device__ __forceinline__ uint32_t half_type_bits(float v) {
     else return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v);
 }
 
+// 8 values from element i on, as they lie; `wide`: the address is 16-byte aligned.
+template <int T>
+constexpr int kWords8 = T == MIVI_GGML_F32 ? 8 : 4;
+template <int T>
+__device__ __forceinline__ void load8_words(const void* p, int64_t i, bool wide, uint32_t (&w)[kWords8<T>]) {
+    const uint8_t* at = (const uint8_t*)p + i * (T == MIVI_GGML_F32 ? 4 : 2);
+    if (wide) {
+#pragma unroll
+        for (int e = 0; e < kWords8<T>; e += 4) {
+            const u32x4 x = *(const u32x4*)(at + 4 * e);
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[e + j] = x[j];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < kWords8<T>; e++)
+            w[e] = T == MIVI_GGML_F32 ? ((const uint32_t*)at)[e]
+                                      : ((const uint16_t*)at)[2 * e] | (uint32_t)((const uint16_t*)at)[2 * e + 1] << 16;
+    }
+}
+template <int T>
+__device__ __forceinline__ void words_to_f32(const uint32_t (&w)[kWords8<T>], float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        if constexpr (T == MIVI_GGML_F32) x[e] = __uint_as_float(w[e]);
+        else if constexpr (T == MIVI_GGML_F16) x[e] = half_bits_to_f32(w[e / 2] >> (e % 2 * 16));
+        else x[e] = bf16_bits_to_f32(w[e / 2] >> (e % 2 * 16));
+    }
+}
+
 // 8 values from element i on; `wide`: the address is 16-byte aligned.
 template <int T>
 __device__ __forceinline__ void load8(const void* p, int64_t i, bool wide, float (&x)[8]) {
@@ -184,48 +214,87 @@ __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
 
 // Largest over the four lanes of a block: a quad, or the quarters l mod 16 + 16 j.
 template <bool QUAD>
-__device__ __forceinline__ float block_max(float v) {
+__device__ __forceinline__ uint32_t block_max(uint32_t v) {
     if constexpr (QUAD) {
-        v = fmaxf(v, dpp_mov<0xB1>(v));
-        return fmaxf(v, dpp_mov<0x4E>(v));
+        v = max(v, dpp_u32<0xB1>(v));
+        return max(v, dpp_u32<0x4E>(v));
     } else {
-        return quarters_max(v);
+        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max(a[0], a[1]);
+        const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return max(b[0], b[1]);
     }
 }
 
-// The codes of 8 values of a block whose other 24 three more lanes hold, each
-// 0..15, and the block's scale as fp16 bits.
-template <bool QUAD>
-__device__ __forceinline__ uint32_t quantise8(const float (&in)[8], int (&code)[8]) {
-    float x[8];
+// Codes of 8 values of a block whose other 24 three more lanes hold, and the
+// block's scale as fp16 bits. The codes come as one dword of nibbles: value e at
+// nibble e (V), or 2 i at nibble i and 2 i + 1 at nibble 4 + i (K).
+//
+// Magnitudes are compared as integers: of the bit patterns the largest signed
+// one is the largest positive value, the largest unsigned one the negative value
+// of largest magnitude, and a NaN or a value past the limit shows in either, so
+// that only blocks with one pay for the limits.
+//
+// c - 8 = rint(x / d), ties to even: t = x / d by the reciprocal and one
+// correction is exact wherever x / d is an fp32 number, so at every tie, and a
+// sum with 1.5 * 2^23 rounds it. For fp16 and bf16 values nothing else lies so
+// near a tie that t could round to it (x / d is no nearer to a half than 2^-15,
+// d having 8 bits and x 11). An fp32 x may: there the remainder x - n d, exact in
+// one fma, decides.
+template <int T, bool QUAD>
+__device__ __forceinline__ uint32_t quantise8(float (&x)[8], bool v_order, uint32_t* scale) {
+    uint32_t pos = 0, neg = 0;
+    const uint32_t most = __float_as_uint(kMaxValue);
+    auto extent = [&] {
+        int p = 0;
+        uint32_t n = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            p = max(p, max((int)__float_as_uint(x[e]), (int)__float_as_uint(x[e + 1])));
+            n = max(n, max(__float_as_uint(x[e]), __float_as_uint(x[e + 1])));
+        }
+        pos = block_max<QUAD>((uint32_t)p);
+        n = block_max<QUAD>(n);
+        neg = n & 0x80000000u ? n & 0x7FFFFFFFu : 0u;
+    };
+    extent();
+    if (__any(max(pos, neg) > most)) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = x[e] == x[e] ? fminf(fmaxf(x[e], -kMaxValue), kMaxValue) : 0.f;
+        extent();
+    }
+    const float m = pos >= neg ? __uint_as_float(pos) : -__uint_as_float(neg);
+    const uint32_t dh = f32_to_half_bits((float)(__bf16)(m * -0.125f));
+    *scale = dh;
+    const float d = half_bits_to_f32(dh), r = d != 0.f ? __builtin_amdgcn_rcpf(d) : 0.f;
+    constexpr uint32_t kZero = 0x4B400008u;  // bits of 1.5 * 2^23 + 8: the code is the low nibble
+    const float half_d = d != 0.f ? 0.5f * fabsf(d) : __builtin_inff();
+    uint32_t u[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        x[e] = in[e] == in[e] ? fminf(fmaxf(in[e], -kMaxValue), kMaxValue) : 0.f;
+        const float t = x[e] * r, q = fmaf(fmaf(-t, d, x[e]), r, t);
+        const float sum = q + __uint_as_float(kZero);
+        u[e] = __float_as_uint(sum);
+        if constexpr (T == MIVI_GGML_F32) {
+            const float n = sum - __uint_as_float(kZero);
+            const float rem = fmaf(-n, d, x[e]);
+            // past the half, or on it at an odd code: the code beside it
+            const float edge = __uint_as_float(__float_as_uint(half_d) - (u[e] & 1));
+            const int way = (int)(__float_as_uint(rem) ^ __float_as_uint(d)) >> 31 | 1;
+            if (fabsf(rem) > edge) u[e] += way;
+        }
+        u[e] = min(max(u[e], kZero - 8), kZero + 7);
     }
-    float hi = x[0], lo = x[0];
+    // nibbles from the top: each step 16 times the last, the constants out at the end
+    uint32_t w = 0;
+    if (v_order) {
 #pragma unroll
-    for (int e = 1; e < 8; e++) hi = fmaxf(hi, x[e]), lo = fminf(lo, x[e]);
-    hi = block_max<QUAD>(hi);
-    lo = -block_max<QUAD>(-lo);
-    const float m = hi >= -lo ? hi : lo;
-    const float y = fminf(fmaxf(m * -0.125f, -kMaxScale), kMaxScale);
-    const uint32_t dh = f32_to_half_bits((float)(__bf16)y);
-    const float d = half_bits_to_f32(dh);
-    // rint(x / d): the estimate from the reciprocal is at most one off, and the
-    // remainder x - n d says which way (one fma: exact enough that its sign
-    // against +- d / 2 is right, d / 2 being representable); ties to even
-    const float r = d != 0.f ? 1.0f / d : 0.f, half = 0.5f * fabsf(d);
-    const float step = d < 0.f ? -1.f : 1.f;
+        for (int i = 7; i >= 0; i--) w = (w << 4) + u[i];
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        float n = rintf(x[e] * r);
-        const float rem = fmaf(-n, d, x[e]);
-        const float ar = fabsf(rem);
-        if (ar > half || (ar == half && ((int)n & 1))) n += rem > 0.f ? step : -step;
-        n = d != 0.f ? fminf(fmaxf(n, -8.f), 7.f) : 0.f;
-        code[e] = (int)n + 8;
+        for (int i = 7; i >= 0; i--) w = (w << 4) + u[i < 4 ? 2 * i : 2 * i - 7];
     }
-    return dh;
+    return w - (kZero - 8) * 0x11111111u;
 }
 
 // One lane 8 dimensions (a block's quarter) of one row and head, K or V
@@ -248,22 +317,16 @@ __global__ void __launch_bounds__(256) kv_q4_append_kernel(Q4Batch a, const void
     const bool is_v = blockIdx.y != 0;
     const int t = pos % kGroup;
     float x[8];
-    int code[8];
+    uint32_t d;
     load8<T>(is_v ? v : k, (int64_t)row * (is_v ? v_row : k_row) + h * (is_v ? v_head : k_head) + b * 32 + c * 8,
              is_v ? wide_v : wide_k, x);
-    const uint32_t d = quantise8<true>(x, code);
+    const uint32_t w = quantise8<T, true>(x, is_v, &d);
     if (!is_v) {
-        uint32_t w = 0;
-#pragma unroll
-        for (int e = 0; e < 8; e++) w |= (uint32_t)code[e] << (4 * (e / 2) + 16 * (e % 2));
         *(uint32_t*)(g + q4_at(nb, b, t % 16 + 16 * c) + t / 16 * 4) = w;
         if (c == 0) *(uint16_t*)(g + 32 * hd + 2 * (t % 16 * 2 * nb + t / 16 * nb + b)) = (uint16_t)d;
     } else {
         // lanes 0 and 1 hold dimensions 0..15 of the block, lanes 2 and 3 the
         // ones 16 further: a lane stores four of the eight pairs it can form
-        uint32_t w = 0;
-#pragma unroll
-        for (int e = 0; e < 8; e++) w |= (uint32_t)code[e] << (4 * e);
         const uint32_t o = dpp_u32<0x4E>(w);  // lane ^ 2
         const uint32_t lo = c < 2 ? w : o, hi = c < 2 ? o : w;
         const int byte = 16 * hd + t / 16 * 4 + ((t & 1) * 2 | (t >> 1 & 1));
@@ -316,13 +379,111 @@ __global__ void __launch_bounds__(256) kv_q4_read_kernel(Q4Batch a, void* k, voi
                   is_v ? wide_v : wide_k, x);
 }
 
+// ------------------------------------------------------ codes to values
+// Codes of one dword as four fp16 pairs 16 + c: nibbles (0, 4), (1, 5), (2, 6),
+// (3, 7) into the top mantissa bits of 16.0. The constants are held in
+// registers that the compiler does not see through: as literals they cost two
+// instructions (and, or) in place of one.
+struct Q4Bits {
+    uint32_t mask = 0x03C003C0u, sixteen = 0x4C004C00u;
+    __device__ __forceinline__ Q4Bits() {
+        asm("" : "+s"(mask));
+        asm("" : "+v"(sixteen));
+    }
+    __device__ __forceinline__ half2v pair(uint32_t w, int i) const {
+        const uint32_t x = i == 0 ? w << 6 : i == 1 ? w << 2 : i == 2 ? w >> 2 : w >> 6;
+        return __builtin_bit_cast(half2v, (x & mask) | sixteen);
+    }
+};
+// (16 + c) d - 24 d = (c - 8) d, exact; dm = -24 d (10 significant bits, exact)
+__device__ __forceinline__ half2v held(half2v x, half2v d, half2v dm) { return __builtin_elementwise_fma(x, d, dm); }
+
+__device__ __forceinline__ half2v as_half2(uint32_t w) { return __builtin_bit_cast(half2v, w); }
+__device__ __forceinline__ half8 join8(half2v a, half2v b, half2v c, half2v d) {
+    return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// K codes of a token's eight dimensions: the A operand of its block.
+__device__ __forceinline__ half8 held_k(const Q4Bits& q, uint32_t w, _Float16 ds) {
+    const half2v d = {ds, ds}, dm = d * (_Float16)-24;
+    return join8(held(q.pair(w, 0), d, dm), held(q.pair(w, 1), d, dm), held(q.pair(w, 2), d, dm),
+                 held(q.pair(w, 3), d, dm));
+}
+// V codes of eight tokens: the A operands of the block's two halves of 16
+// dimensions; sc: the tokens' four scale pairs.
+__device__ __forceinline__ void held_v(const Q4Bits& q, uint32_t w0, uint32_t w1, const uint32_t* sc, half8 (&v)[2]) {
+    half2v d[4], dm[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) d[j] = as_half2(sc[j]), dm[j] = d[j] * (_Float16)-24;
+#pragma unroll
+    for (int z = 0; z < 2; z++)
+        v[z] = join8(held(q.pair(w0, z), d[0], dm[0]), held(q.pair(w0, z + 2), d[1], dm[1]),
+                     held(q.pair(w1, z), d[2], dm[2]), held(q.pair(w1, z + 2), d[3], dm[3]));
+}
+
+// A group's codes and scales as lane l loads them: K or V codes of all blocks,
+// the K scales of token l mod 16 in both halves, the V scales of the quarter.
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {  // 4-byte aligned
+    if constexpr (N >= 4) {
+        const u32x4_a4 x = *(const u32x4_a4*)p;
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = x[i];
+        load_words<N - 4>(p + 16, w + 4);
+    } else if constexpr (N >= 2) {
+        const u32x2_a4 x = *(const u32x2_a4*)p;
+        w[0] = x[0], w[1] = x[1];
+        load_words<N - 2>(p + 8, w + 2);
+    } else if constexpr (N == 1) {
+        w[0] = *(const uint32_t*)p;
+    }
+}
+template <int NB, int B0 = 0, int B1 = NB>  // blocks B0 .. B1 - 1, B0 even
+__device__ __forceinline__ void load_codes(const uint8_t* p, int lane, uint32_t* w) {
+#pragma unroll
+    for (int b = B0; b < B1; b += 2) {
+        if (b + 1 < NB) {
+            const u32x4 x = __builtin_nontemporal_load((const u32x4*)(p + b / 2 * 1024 + lane * 16));
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[2 * (b - B0) + j] = x[j];
+        } else {
+            const u32x2 x = *(const u32x2*)(p + b / 2 * 1024 + lane * 8);
+            w[2 * (b - B0)] = x[0], w[2 * (b - B0) + 1] = x[1];
+        }
+    }
+}
+template <int NB>
+__device__ __forceinline__ void load_k(const uint8_t* g, int lane, uint32_t (&k)[2 * NB], uint32_t (&ks)[NB]) {
+    load_codes<NB>(g, lane, k);
+    load_words<NB>(g + 1024 * NB + lane % 16 * 4 * NB, ks);
+}
+template <int NB, int B0 = 0, int B1 = NB>
+__device__ __forceinline__ void load_v(const uint8_t* g, int lane, uint32_t* v, uint32_t* vs) {
+    load_codes<NB, B0, B1>(g + 512 * NB, lane, v);
+#pragma unroll
+    for (int b = B0; b < B1; b++) {
+        const u32x4 x = *(const u32x4*)(g + 1088 * NB + (b * 4 + lane / 16) * 16);
+#pragma unroll
+        for (int j = 0; j < 4; j++) vs[4 * (b - B0) + j] = x[j];
+    }
+}
+template <int NB>
+__device__ __forceinline__ _Float16 k_scale(const uint32_t (&ks)[NB], int half, int b) {
+    const int i = half * NB + b;
+    return as_half2(ks[i / 2])[i % 2];
+}
+
 // ------------------------------------------------- whole groups at a time
-// Rows that are many: a wave takes one group of one sequence and head, K or V.
-// Sequence s has the units from U(s) = starts[s] / 32 + 2 s on: its n rows touch
-// at most (n - 2) / 32 + 2 groups, and U(s + 1) - U(s) is no less, so no sum
-// over the sequences is needed to place them.
+// Rows that are many: a workgroup takes one group of one sequence, its waves (of
+// all workgroups that share the group) one head's K or V after another, the next
+// one's loads issued before the present one is worked on. Sequence s has the
+// groups' units from U(s) = starts[s] / 32 + 2 s on: its n rows touch at most
+// (n - 2) / 32 + 2 groups, and U(s + 1) - U(s) is no less, so no sum over the
+// sequences is needed to place them.
 struct Q4Unit {
-    uint8_t* g;    // the group, null where the table has no page of the cache
+    int s, g;      // sequence and group
+    bool there;    // whether the table has a page of the cache there
+    int64_t off;   // of the group of head 0
     int64_t row0;  // row of the group's token 0
     int t0, t1;    // tokens of the group that are rows of the call
 };
@@ -342,7 +503,7 @@ __device__ __forceinline__ int wave_search(int n, int lane, int u, Key key) {
     return lo;
 }
 
-__device__ __forceinline__ bool unit_of(const Q4Batch& a, int u, int h, int rows, int lane, Q4Unit* o) {
+__device__ __forceinline__ bool unit_of(const Q4Batch& a, int u, int rows, int lane, Q4Unit* o) {
     const int s = __builtin_amdgcn_readfirstlane(
         wave_search(a.n_seq, lane, u, [&](int i) { return (a.starts[i] >> 5) + 2 * i; }));
     const int start = a.starts[s];
@@ -355,14 +516,29 @@ __device__ __forceinline__ bool unit_of(const Q4Batch& a, int u, int h, int rows
     o->row0 = start + (base - p0);
     o->t0 = (int)max<int64_t>(p0 - base, 0);
     o->t1 = (int)min<int64_t>(p0 + count - base, kGroup);
-    o->g = base >= 0 && base < a.cap ? group_ptr(a, s, h, (int)g) : nullptr;
+    o->there = base >= 0 && base < a.cap;
+    o->off = 0;
+    if (o->there) {
+        const int pi = page_index(a, (int)g), page = a.pages[(int64_t)s * a.page_stride + pi];
+        o->there = page >= 0 && page < a.n_pages;
+        o->off = (int64_t)page * a.page_bytes + ((int)g - pi * a.gpp) * (36 * a.hd);
+    }
     return true;
 }
 
-// Byte of a group's V codes in its LDS image: 16 bytes more every 256, so that
-// the quarters of the tokens are in different banks.
-__device__ __forceinline__ int image_at(int byte) { return byte + (byte >> 8 << 4); }
-constexpr int kImage = 16 * 256 / 256 * 272;  // bytes of the largest
+// A wave's LDS is its own: its writes before its reads, in the compiler's order
+// too.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A group's V codes in LDS: 16 bytes more a quarter of the tokens, so that the
+// quarters are in different banks. Pair of blocks i at 1088 i, an odd last block
+// alone behind them; lane n + 16 quarter of it at n * size + quarter * (16 size +
+// 16) with 16 or 8 bytes a lane.
+constexpr int kImage = 4 * 1088;  // bytes of the largest (8 blocks)
 
 template <int T>
 __global__ void __launch_bounds__(256) kv_q4_append_groups_kernel(Q4Batch a, const void* k, const void* v,
@@ -370,137 +546,176 @@ __global__ void __launch_bounds__(256) kv_q4_append_groups_kernel(Q4Batch a, con
                                                                   int64_t v_head, int rows, int wide_k, int wide_v) {
     __shared__ __attribute__((aligned(16))) uint8_t image[4][kImage];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int which = blockIdx.y * 4 + wave, h = which >> 1;
-    const bool is_v = which & 1;
-    if (h >= a.n_kv) return;
     Q4Unit u;
-    if (!unit_of(a, blockIdx.x, h, rows, lane, &u) || !u.g) return;
+    if (!unit_of(a, blockIdx.x, rows, lane, &u) || !u.there) return;
+    const bool is_v = wave & 1;
     const int hd = a.hd, nb = hd / 32, t16 = lane & 15, c = lane >> 4;
     const void* x = is_v ? v : k;
-    const int64_t rs = is_v ? v_row : k_row;
-    const int wide = is_v ? wide_v : wide_k;
-    const int64_t base = (u.row0 + t16) * rs + h * (is_v ? v_head : k_head) + c * 8;
+    const int64_t rs = is_v ? v_row : k_row, hs = is_v ? v_head : k_head;
+    const int wide = is_v ? wide_v : wide_k, step = gridDim.y * 2;
+    const int64_t base = (u.row0 + t16) * rs + c * 8;
     const bool in[2] = {t16 >= u.t0 && t16 < u.t1, t16 + 16 >= u.t0 && t16 + 16 < u.t1};
     const bool whole = u.t1 - u.t0 == kGroup;
     uint8_t* img = image[wave];
-    for (int b = 0; b < nb; b += 2) {
-        const bool two = b + 1 < nb;
-        float val[4][8];  // [block of the pair][half]
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) val[i][e] = 0.f;
-            if (in[i % 2] && (i < 2 || two)) load8<T>(x, base + i % 2 * 16 * rs + (b + i / 2) * 32, wide, val[i]);
-        }
-        uint32_t w[4], d[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            int code[8];
-            d[i] = quantise8<false>(val[i], code);
-            w[i] = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++) w[i] |= (uint32_t)code[e] << (is_v ? 4 * e : 4 * (e / 2) + 16 * (e % 2));
-        }
-        const int off = q4_at(nb, b, lane);  // of the lane's dwords: [block][half]
-        if (!is_v) {
-            if (whole) {
-                if (two) *(u32x4*)(u.g + off) = u32x4{w[0], w[1], w[2], w[3]};
-                else *(u32x2*)(u.g + off) = u32x2{w[0], w[1]};
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (in[i % 2] && (i < 2 || two)) *(uint32_t*)(u.g + off + 4 * i) = w[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (c == 0 && in[i % 2] && (i < 2 || two))
-                    *(uint16_t*)(u.g + 32 * hd + 2 * (t16 * 2 * nb + i % 2 * nb + b + i / 2)) = (uint16_t)d[i];
-        } else {
+    auto work = [&](auto kind) {
+        constexpr bool kIsV = decltype(kind)::value;
+        uint32_t next[4][kWords8<T>];  // [block of the pair][half]
+        auto fetch = [&](int h, int b) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (i >= 2 && !two) break;
-                // lanes of quarters 0 and 1 hold dimensions 0..15 of the block,
-                // 2 and 3 the ones 16 further: a lane stores four of the eight
-                // pairs that it can form with the lane 32 away
-                float a0, a1;
-                swap32(__uint_as_float(w[i]), a0, a1);
-                const uint32_t lo = __float_as_uint(a0), hi = __float_as_uint(a1);
-                const int byte = i % 2 * 4 + ((t16 & 1) * 2 | (t16 >> 1 & 1));
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int e = (c >> 1) * 4 + j, n = (c & 1) * 8 + e;
-                    const uint8_t pair = (uint8_t)((lo >> (4 * e) & 15) | (hi >> (4 * e) & 15) << 4);
-                    const int at = q4_at(nb, b + i / 2, n + 16 * (t16 / 4)) + byte;
-                    if (whole) img[image_at(at)] = pair;
-                    else if (in[i % 2]) u.g[16 * hd + at] = pair;
+                for (int e = 0; e < kWords8<T>; e++) next[i][e] = 0;
+                if (in[i % 2] && b + i / 2 < nb) load8_words<T>(x, base + h * hs + i % 2 * 16 * rs + (b + i / 2) * 32, wide, next[i]);
+            }
+        };
+        const int h0 = blockIdx.y * 2 + (wave >> 1);
+        if (h0 < a.n_kv) fetch(h0, 0);
+        for (int h = h0; h < a.n_kv; h += step) {
+            uint8_t* g = a.cache + u.off + (int64_t)h * a.gpp * (36 * hd);
+            for (int b = 0; b < nb; b += 2) {
+                const bool two = b + 1 < nb;
+                float val[4][8];
+#pragma unroll
+                for (int i = 0; i < 4; i++) words_to_f32<T>(next[i], val[i]);
+                if (b + 2 < nb) fetch(h, b + 2);
+                else if (h + step < a.n_kv) fetch(h + step, 0);
+                uint32_t w[4], d[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = quantise8<T, false>(val[i], kIsV, &d[i]);
+                const int off = q4_at(nb, b, lane);  // of the lane's dwords: [block][half]
+                if (!kIsV) {
+                    if (whole) {
+                        if (two) *(u32x4*)(g + off) = u32x4{w[0], w[1], w[2], w[3]};
+                        else *(u32x2*)(g + off) = u32x2{w[0], w[1]};
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (in[i % 2] && (i < 2 || two)) *(uint32_t*)(g + off + 4 * i) = w[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (c == 0 && in[i % 2] && (i < 2 || two))
+                            *(uint16_t*)(g + 32 * hd + 2 * (t16 * 2 * nb + i % 2 * nb + b + i / 2)) = (uint16_t)d[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (i >= 2 && !two) break;
+                        // lanes of quarters 0 and 1 hold dimensions 0..15 of the
+                        // block, 2 and 3 the ones 16 further: with the lane 32 away a
+                        // lane forms four of the eight pairs: n = n0 + j
+                        const auto other = __builtin_amdgcn_permlane32_swap(w[i], w[i], false, false);
+                        const uint32_t lo = other[0] >> (c >> 1) * 16, hi = other[1] >> (c >> 1) * 16;
+                        const uint32_t even = (lo & 0x0F0Fu) | (hi & 0x0F0Fu) << 4;        // j = 0, 2
+                        const uint32_t odd = (lo >> 4 & 0x0F0Fu) | (hi & 0xF0F0u);         // j = 1, 3
+                        const int n0 = (c & 1) * 8 + (c >> 1) * 4, size = two ? 16 : 8;
+                        const int byte = i / 2 * 8 + i % 2 * 4 + ((t16 & 1) * 2 | (t16 >> 1 & 1));
+                        auto put = [&](uint8_t* at) {
+                            at[0] = (uint8_t)even, at[2 * size] = (uint8_t)(even >> 8);
+                            at[size] = (uint8_t)odd, at[3 * size] = (uint8_t)(odd >> 8);
+                        };
+                        if (whole) put(img + b / 2 * 1088 + n0 * size + t16 / 4 * (16 * size + 16) + byte);
+                        else if (in[i % 2]) put(g + 16 * hd + b / 2 * 1024 + (n0 + t16 / 4 * 16) * size + byte);
+                        if (c == 0 && in[i % 2])
+                            *(uint16_t*)(g + 34 * hd + 2 * ((b + i / 2) * 32 + t16 / 4 * 8 + i % 2 * 4 + t16 % 4)) = (uint16_t)d[i];
+                    }
                 }
-                if (c == 0 && in[i % 2])
-                    *(uint16_t*)(u.g + 34 * hd + 2 * ((b + i / 2) * 32 + t16 / 4 * 8 + i % 2 * 4 + t16 % 4)) = (uint16_t)d[i];
+            }
+            if (kIsV && whole) {
+                wave_sync();
+                for (int i = 0; i < nb / 2; i++)
+                    *(u32x4*)(g + 16 * hd + i * 1024 + lane * 16) =
+                        *(const u32x4*)(img + i * 1088 + lane % 16 * 16 + lane / 16 * 272);
+                if (nb % 2)
+                    *(u32x2*)(g + 16 * hd + nb / 2 * 1024 + lane * 8) =
+                        *(const u32x2*)(img + nb / 2 * 1088 + lane % 16 * 8 + lane / 16 * 144);
+                wave_sync();
             }
         }
-    }
-    if (is_v && whole) {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        for (int i = lane * 16; i < 16 * hd; i += 1024) *(u32x4*)(u.g + 16 * hd + i) = *(const u32x4*)(img + image_at(i));
-    }
+    };
+    if (is_v) work(std::true_type{});
+    else work(std::false_type{});
 }
 
+// 8 fp16 values (4 dwords) as values of type T to element i on.
 template <int T>
+__device__ __forceinline__ void store8_half(void* p, int64_t i, bool wide, u32x4 w) {
+    if (T == MIVI_GGML_F16 && wide) {
+        __builtin_nontemporal_store(w, (u32x4*)((uint16_t*)p + i));
+        return;
+    }
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = half_bits_to_f32(w[e / 2] >> (e % 2 * 16));
+    store_n<T, 8>(p, i, wide, x);
+}
+
+// The held values are fp16 numbers: they are formed as the attention forms them
+// and widened. K comes out in rows; V goes through LDS, a row of hd values and 8
+// bytes more a token (the quarters of the tokens in different banks).
+template <int T, int NB>
 __global__ void __launch_bounds__(256) kv_q4_read_groups_kernel(Q4Batch a, void* k, void* v, int64_t k_row,
                                                                 int64_t k_head, int64_t v_row, int64_t v_head,
                                                                 int rows, int wide_k, int wide_v) {
-    __shared__ __attribute__((aligned(16))) uint8_t image[4][kImage];
+    constexpr int hd = 32 * NB, kRow = hd + 4;
+    __shared__ __attribute__((aligned(16))) _Float16 tile[2][32 * kRow];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int which = blockIdx.y * 4 + wave, h = which >> 1;
-    const bool is_v = which & 1;
-    if (h >= a.n_kv) return;
     Q4Unit u;
-    if (!unit_of(a, blockIdx.x, h, rows, lane, &u)) return;
-    const int hd = a.hd, nb = hd / 32, t16 = lane & 15, c = lane >> 4;
-    void* x = is_v ? v : k;
-    const int64_t rs = is_v ? v_row : k_row;
-    const int wide = is_v ? wide_v : wide_k;
-    const int64_t base = (u.row0 + t16) * rs + h * (is_v ? v_head : k_head) + c * 8;
-    const bool in[2] = {t16 >= u.t0 && t16 < u.t1, t16 + 16 >= u.t0 && t16 + 16 < u.t1};
-    uint8_t* img = image[wave];
-    if (is_v && u.g) {
-        for (int i = lane * 16; i < 16 * hd; i += 1024) *(u32x4*)(img + image_at(i)) = *(const u32x4*)(u.g + 16 * hd + i);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
-    for (int b = 0; b < nb; b += 2) {
-        const bool two = b + 1 < nb;
-        u32x4 w = {0, 0, 0, 0};  // K codes [block of the pair][half]
-        if (!is_v && u.g) {
-            if (two) {
-                w = *(const u32x4*)(u.g + q4_at(nb, b, lane));
-            } else {
-                const u32x2 y = *(const u32x2*)(u.g + q4_at(nb, b, lane));
-                w[0] = y[0], w[1] = y[1];
-            }
+    if (!unit_of(a, blockIdx.x, rows, lane, &u)) return;
+    const bool is_v = wave & 1;
+    const int t16 = lane & 15, c = lane >> 4, step = gridDim.y * 2, h0 = blockIdx.y * 2 + (wave >> 1);
+    const Q4Bits bits;
+    const uint8_t* g0 = a.cache + u.off;
+    const int64_t hs = (int64_t)a.gpp * (36 * hd);
+    uint32_t w[2 * NB], sc[4 * NB];
+#pragma unroll
+    for (int i = 0; i < 2 * NB; i++) w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 4 * NB; i++) sc[i] = 0;  // no page: zeros
+    if (!is_v) {
+        uint32_t(&ks)[NB] = *(uint32_t(*)[NB]) sc;
+        const int64_t base = (u.row0 + t16) * k_row + c * 8;
+        const bool in[2] = {t16 >= u.t0 && t16 < u.t1, t16 + 16 >= u.t0 && t16 + 16 < u.t1};
+        if (u.there && h0 < a.n_kv) load_k<NB>(g0 + h0 * hs, lane, w, ks);
+        for (int h = h0; h < a.n_kv; h += step) {
+            u32x4 out[2 * NB];
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int half = 0; half < 2; half++)
+                    out[2 * b + half] = __builtin_bit_cast(u32x4, held_k(bits, w[2 * b + half], k_scale<NB>(ks, half, b)));
+            if (u.there && h + step < a.n_kv) load_k<NB>(g0 + (h + step) * hs, lane, w, ks);
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int half = 0; half < 2; half++)
+                    if (in[half]) store8_half<T>(k, base + h * k_head + half * 16 * k_row + b * 32, wide_k, out[2 * b + half]);
         }
+    } else {
+        _Float16* own = tile[wave >> 1];
+        if (u.there && h0 < a.n_kv) load_v<NB>(g0 + h0 * hs, lane, w, sc);
+        for (int h = h0; h < a.n_kv; h += step) {
+            // lane: dimension t16 of each half block, tokens 4 c + i of each half group
+            _Float16* at = own + 4 * c * kRow + t16;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (!in[i % 2] || (i >= 2 && !two)) continue;
-            float out[8] = {};
-            if (u.g) {
-                const int at = is_v ? 34 * hd + 2 * ((b + i / 2) * 32 + t16 / 4 * 8 + i % 2 * 4 + t16 % 4)
-                                    : 32 * hd + 2 * (t16 * 2 * nb + i % 2 * nb + b + i / 2);
-                const float d = half_bits_to_f32(*(const uint16_t*)(u.g + at));
-                const int byte = i % 2 * 4 + ((t16 & 1) * 2 | (t16 >> 1 & 1));
-                const int first = q4_at(nb, b + i / 2, (c & 1) * 8 + 16 * (t16 / 4)) + byte;
-                const int step = b + i / 2 < nb / 2 * 2 ? 16 : 8;
+            for (int b = 0; b < NB; b++) {
+                half8 vv[2];
+                held_v(bits, w[2 * b], w[2 * b + 1], &sc[4 * b], vv);
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const uint32_t code = is_v ? img[image_at(first + e * step)] >> (c / 2 * 4) & 15
-                                               : w[i] >> (4 * (e / 2) + 16 * (e % 2)) & 15;
-                    out[e] = (float)((int)code - 8) * d;
-                }
+                for (int z = 0; z < 2; z++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        at[(i / 4 * 16 + i % 4) * kRow + b * 32 + z * 16] = vv[z][i];
             }
-            store_n<T, 8>(x, base + i % 2 * 16 * rs + (b + i / 2) * 32, wide, out);
+            if (u.there && h + step < a.n_kv) load_v<NB>(g0 + (h + step) * hs, lane, w, sc);
+            wave_sync();
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) {
+                const int piece = i * 64 + lane, t = piece / (4 * NB), d = piece % (4 * NB) * 8;
+                const u32x2 lo = *(const u32x2*)(own + t * kRow + d), hi = *(const u32x2*)(own + t * kRow + d + 4);
+                if (t >= u.t0 && t < u.t1)
+                    store8_half<T>(v, (u.row0 + t) * v_row + h * v_head + d, wide_v, u32x4{lo[0], lo[1], hi[0], hi[1]});
+            }
+            wave_sync();
         }
     }
 }
@@ -526,24 +741,6 @@ struct Q4Attn {
 
 // Row of a pair.
 __device__ __forceinline__ int row_of(const Q4Attn& a, int f) { return (int)((uint32_t)f / (uint32_t)a.gq); }
-
-// Codes of one dword as four fp16 pairs 16 + c: nibbles (0, 4), (1, 5), (2, 6),
-// (3, 7) into the top mantissa bits of 16.0. The constants are held in
-// registers that the compiler does not see through: as literals they cost two
-// instructions (and, or) in place of one.
-struct Q4Bits {
-    uint32_t mask = 0x03C003C0u, sixteen = 0x4C004C00u;
-    __device__ __forceinline__ Q4Bits() {
-        asm("" : "+s"(mask));
-        asm("" : "+v"(sixteen));
-    }
-    __device__ __forceinline__ half2v pair(uint32_t w, int i) const {
-        const uint32_t x = i == 0 ? w << 6 : i == 1 ? w << 2 : i == 2 ? w >> 2 : w >> 6;
-        return __builtin_bit_cast(half2v, (x & mask) | sixteen);
-    }
-};
-// (16 + c) d - 24 d = (c - 8) d, exact; dm = -24 d (10 significant bits, exact)
-__device__ __forceinline__ half2v held(half2v x, half2v d, half2v dm) { return __builtin_elementwise_fma(x, d, dm); }
 
 // A query row's blocks, 8 values each at i + 32 b: every load before any use.
 template <int NB>
@@ -608,29 +805,6 @@ __device__ __forceinline__ void tile_groups(const Q4Seen& see, int i0, int i1, i
     *g_hi = (see.hi(i1) + kGroup - 1) / kGroup;
 }
 
-__device__ __forceinline__ half2v as_half2(uint32_t w) { return __builtin_bit_cast(half2v, w); }
-__device__ __forceinline__ half8 join8(half2v a, half2v b, half2v c, half2v d) {
-    return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
-
-// K codes of a token's eight dimensions: the A operand of its block.
-__device__ __forceinline__ half8 held_k(const Q4Bits& q, uint32_t w, _Float16 ds) {
-    const half2v d = {ds, ds}, dm = d * (_Float16)-24;
-    return join8(held(q.pair(w, 0), d, dm), held(q.pair(w, 1), d, dm), held(q.pair(w, 2), d, dm),
-                 held(q.pair(w, 3), d, dm));
-}
-// V codes of eight tokens: the A operands of the block's two halves of 16
-// dimensions; sc: the tokens' four scale pairs.
-__device__ __forceinline__ void held_v(const Q4Bits& q, uint32_t w0, uint32_t w1, const uint32_t* sc, half8 (&v)[2]) {
-    half2v d[4], dm[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) d[j] = as_half2(sc[j]), dm[j] = d[j] * (_Float16)-24;
-#pragma unroll
-    for (int z = 0; z < 2; z++)
-        v[z] = join8(held(q.pair(w0, z), d[0], dm[0]), held(q.pair(w0, z + 2), d[1], dm[1]),
-                     held(q.pair(w1, z), d[2], dm[2]), held(q.pair(w1, z + 2), d[3], dm[3]));
-}
-
 // A V scale pair j (of 4) of the lane's quarter in a group at t0, without the
 // tokens from `valid` on: what lies behind the sequence's end is anything, and
 // 0 * NaN is NaN.
@@ -639,7 +813,10 @@ __device__ __forceinline__ uint32_t keep_mask(int t0, int quarter, int j, int va
     return (t < valid ? 0xFFFFu : 0u) | (t + 1 < valid ? 0xFFFF0000u : 0u);
 }
 
-constexpr float kPShift = 15;  // weights are held times 2^15: fp16 reaches 2^-40 of the largest
+// A row's reference exponent follows its largest score only when that is more
+// than kSlack above it: weights are held times 2^kPShift and reach 2^15; fp16
+// then resolves 2^-36 of the largest.
+constexpr float kPShift = 11, kSlack = 4;
 
 // 16 (row, query head) pairs as the columns of the products; lane l works on
 // column l mod 16.
@@ -647,7 +824,7 @@ template <int NB, int P>
 struct Q4Tile {
     half8 q[P][NB];      // B operands: block b, dimensions 8 quarter .. + 7
     float sc;            // a raw score times sc is the exponent to base 2
-    float m, nm;         // largest exponent so far; kPShift - m, the exponent's offset
+    float m, nm;         // reference exponent; kPShift - m, the exponents' offset
     f32x4 acc[2 * NB];   // sums of w V: dimensions 16 j + 4 quarter + i
     f32x4 l;             // sums of w, the same in all four
     int lo, hi;          // positions seen
@@ -692,12 +869,12 @@ struct Q4Tile {
 
     // The scores of a group (tokens 4 quarter + i of each half) to weights, the
     // B operands of the sums. The maximum over the quarters is formed only when
-    // some lane has a larger score than its row had.
+    // some lane has a score so much larger than its row's reference.
     __device__ __forceinline__ void weigh(const f32x4 (&st)[2], half8 (&w)[P]) {
         float mx = st[0][0];
 #pragma unroll
         for (int i = 1; i < 8; i++) mx = fmaxf(mx, st[i / 4][i % 4]);
-        if (__any(mx * sc > m)) {
+        if (__any(mx * sc > m + kSlack)) {
             const float m_new = fmaxf(m, quarters_max(mx) * sc);
             const float f = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
             m = m_new;
@@ -736,58 +913,6 @@ __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
 __device__ __forceinline__ half8 ones8() {
     const _Float16 o = 1;
     return half8{o, o, o, o, o, o, o, o};
-}
-
-// A group's codes and scales as lane l loads them: K or V codes of all blocks,
-// the K scales of token l mod 16 in both halves, the V scales of the quarter.
-template <int N>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {  // 4-byte aligned
-    if constexpr (N >= 4) {
-        const u32x4_a4 x = *(const u32x4_a4*)p;
-#pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = x[i];
-        load_words<N - 4>(p + 16, w + 4);
-    } else if constexpr (N >= 2) {
-        const u32x2_a4 x = *(const u32x2_a4*)p;
-        w[0] = x[0], w[1] = x[1];
-        load_words<N - 2>(p + 8, w + 2);
-    } else if constexpr (N == 1) {
-        w[0] = *(const uint32_t*)p;
-    }
-}
-template <int NB, int B0 = 0, int B1 = NB>  // blocks B0 .. B1 - 1, B0 even
-__device__ __forceinline__ void load_codes(const uint8_t* p, int lane, uint32_t* w) {
-#pragma unroll
-    for (int b = B0; b < B1; b += 2) {
-        if (b + 1 < NB) {
-            const u32x4 x = __builtin_nontemporal_load((const u32x4*)(p + b / 2 * 1024 + lane * 16));
-#pragma unroll
-            for (int j = 0; j < 4; j++) w[2 * (b - B0) + j] = x[j];
-        } else {
-            const u32x2 x = *(const u32x2*)(p + b / 2 * 1024 + lane * 8);
-            w[2 * (b - B0)] = x[0], w[2 * (b - B0) + 1] = x[1];
-        }
-    }
-}
-template <int NB>
-__device__ __forceinline__ void load_k(const uint8_t* g, int lane, uint32_t (&k)[2 * NB], uint32_t (&ks)[NB]) {
-    load_codes<NB>(g, lane, k);
-    load_words<NB>(g + 1024 * NB + lane % 16 * 4 * NB, ks);
-}
-template <int NB, int B0 = 0, int B1 = NB>
-__device__ __forceinline__ void load_v(const uint8_t* g, int lane, uint32_t* v, uint32_t* vs) {
-    load_codes<NB, B0, B1>(g + 512 * NB, lane, v);
-#pragma unroll
-    for (int b = B0; b < B1; b++) {
-        const u32x4 x = *(const u32x4*)(g + 1088 * NB + (b * 4 + lane / 16) * 16);
-#pragma unroll
-        for (int j = 0; j < 4; j++) vs[4 * (b - B0) + j] = x[j];
-    }
-}
-template <int NB>
-__device__ __forceinline__ _Float16 k_scale(const uint32_t (&ks)[NB], int half, int b) {
-    const int i = half * NB + b;
-    return as_half2(ks[i / 2])[i % 2];
 }
 
 // What a workgroup knows of its sequence's rows.
@@ -861,18 +986,20 @@ __device__ __forceinline__ bool place_of(const Q4Attn& a, int split, int tile, i
 }
 
 // Even shares, where a sequence's pairs are one tile: the groups of all
-// sequences and heads in one row (sequence by sequence, head by head), cut at
+// sequences and heads in one row, sequence by sequence and head by head, cut at
 // every `size` and between heads. Each piece is one workgroup's, so that no
-// workgroup has more than `size` whatever the lengths. The head and sequence i
-// at x has the workgroups from x / size + i on (the next one's first is past its
-// last). Every wave forms the cut by itself, 64 sequences a look.
-// (All positions fit 31 bits: the plan takes other shares where they might not.)
+// workgroup has more than `size` whatever the lengths. The head that starts at
+// x, with i heads before it, has the workgroups from x / size + i on (the next
+// one's first is past its last). Every wave forms the cut by itself, 64
+// sequences a look. (All positions fit 31 bits: the plan takes other shares
+// where they might not.)
 struct Q4Cut {
     int total;   // groups of all sequences and heads
     int size;    // of a share
     int lo, n;   // this lane's sequence of the first 64: its first group, its groups
     int before;  // groups of a head of the sequences before it
 };
+__device__ __forceinline__ int udiv(int a, int b) { return (int)((uint32_t)a / (uint32_t)b); }
 __device__ __forceinline__ void seq_groups(const Q4Attn& a, int s, int* lo, int* n) {
     Q4Rows r;
     *lo = *n = 0;
@@ -891,7 +1018,6 @@ __device__ __forceinline__ int wave_before(int v, int lane) {  // sum of the lan
     return x - v;
 }
 __device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
-__device__ __forceinline__ int udiv(int a, int b) { return (int)((uint32_t)a / (uint32_t)b); }
 
 __device__ __forceinline__ Q4Cut cut_of(const Q4Attn& a, int lane, int shares) {
     Q4Cut c;
@@ -1077,15 +1203,17 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
     }
 }
 
-// Many pairs: a workgroup's four waves take 16 NT pairs each and share the held
+// Many pairs: a workgroup's NW waves take 16 NT pairs each and share the held
 // values of TG groups at a time, converted once into LDS in operand order (one
-// 16-byte piece a lane, read and written without bank conflicts); two buffers,
-// the next groups converted into one and the ones after on their way from
-// memory while the other is worked on. Each wave converts K or V, of one
-// group (TG 2) or of a part of the blocks (TG 1).
-template <int NB, int P, int NT, int TG>
-__global__ void __launch_bounds__(256) kv_q4_rows_kernel(Q4Attn a, int shares) {
-    constexpr int B0 = TG == 2 || NB < 2 ? NB : (NB / 2 + 1) / 2 * 2;  // blocks of the first wave of a kind
+// 16-byte piece a lane, read and written without bank conflicts). Two buffers:
+// one is worked on while the next groups are converted into the other, and the
+// two steps after are on their way from memory. Each wave converts K or V of
+// some blocks of one group.
+template <int NB, int P, int NT, int NW, int TG>
+__global__ void __launch_bounds__(64 * NW) kv_q4_rows_kernel(Q4Attn a, int shares) {
+    constexpr int kPer = NW / 2 / TG;                             // waves of a group, K or V
+    constexpr int kBlocks = ((NB + 1) / 2 + kPer - 1) / kPer * 2;  // blocks of one of them, an even number
+    constexpr int kHave = kBlocks < NB ? kBlocks : NB;
     __shared__ half8 kf[2][TG][2 * NB][64], vf[2][TG][2 * NB][64];
     __shared__ int have[2][TG];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1104,85 +1232,104 @@ __global__ void __launch_bounds__(256) kv_q4_rows_kernel(Q4Attn a, int shares) {
     }
     const Q4Groups groups(a, pl.s, pl.h, pl.g_end);
     const bool is_v = wave & 1;
-    const int part = wave >> 1;  // group of the step (TG 2), part of the blocks (TG 1)
+    const int part = (wave >> 1) % kPer, mine = (wave >> 1) / kPer;  // blocks from kBlocks part on of group `mine`
 
-    uint32_t c[2 * B0], sc[4 * B0 > NB ? 4 * B0 : NB];
-    const uint8_t* gp = nullptr;
-    int page = -1;              // page id of this wave's group of the next fetch
-    auto fetch = [&](int g) {  // this wave's share of the step at g, and the id for the one after
-        const int gg = TG == 2 ? g + part : g;
-        gp = groups.at(a, gg, page);
-        page = groups.id(a, gg + TG);
-        if (!gp) return;
-        if (is_v) {
-            if (TG == 2 || part == 0) load_v<NB, 0, B0>(gp, lane, c, sc);
-            else if constexpr (B0 < NB) load_v<NB, B0, NB>(gp, lane, c, sc);
-        } else {
-            load_words<NB>(gp + 1024 * NB + lane % 16 * 4 * NB, sc);
-            if (TG == 2 || part == 0) load_codes<NB, 0, B0>(gp, lane, c);
-            else if constexpr (B0 < NB) load_codes<NB, B0, NB>(gp, lane, c);
-        }
-    };
-    auto put_v = [&](half8 (*to)[64], int b, int n) {
+    // two steps' words on their way: codes, and the V scales of the blocks or
+    // the K scales of all blocks
+    uint32_t c[2][2 * kBlocks], sc[2][4 * kHave > NB ? 4 * kHave : NB];
+    const uint8_t* gp[2] = {nullptr, nullptr};
+    int page = -1;  // page id of this wave's group of the next fetch
+    // f(first block, number of blocks), constants, of this wave's part
+    auto with_blocks = [&](auto f) {
 #pragma unroll
-        for (int i = 0; i < B0; i++) {
-            if (i >= n) break;
-            half8 vv[2];
-            held_v(bits, c[2 * i], c[2 * i + 1], &sc[4 * i], vv);
-            to[2 * (b + i)][lane] = vv[0];
-            to[2 * (b + i) + 1][lane] = vv[1];
-        }
-    };
-    auto put_k = [&](half8 (*to)[64], auto first, auto count) {
-        constexpr int b = decltype(first)::value, n = decltype(count)::value;
-#pragma unroll
-        for (int i = 0; i < n; i++) {
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const int si = half * NB + b + i;
-                to[half * NB + b + i][lane] = held_k(bits, c[2 * i + half], as_half2(sc[si / 2])[si % 2]);
+        for (int p = 0; p < kPer; p++) {
+            if (p != part) continue;
+            if (p == 0) f(std::integral_constant<int, 0>{}, std::integral_constant<int, kHave>{});
+            if constexpr (kPer > 1 && kBlocks < NB) {
+                if (p == 1) f(std::integral_constant<int, kBlocks>{}, std::integral_constant<int, (NB < 2 * kBlocks ? NB : 2 * kBlocks) - kBlocks>{});
+            }
+            if constexpr (kPer > 2 && 2 * kBlocks < NB) {
+                if (p == 2) f(std::integral_constant<int, 2 * kBlocks>{}, std::integral_constant<int, (NB < 3 * kBlocks ? NB : 3 * kBlocks) - 2 * kBlocks>{});
+            }
+            if constexpr (kPer > 3 && 3 * kBlocks < NB) {
+                if (p == 3) f(std::integral_constant<int, 3 * kBlocks>{}, std::integral_constant<int, NB - 3 * kBlocks>{});
             }
         }
     };
-    auto convert = [&](int g, int buf) {
-        const int gg = TG == 2 ? part : 0;
-        if (is_v && (TG == 2 || part == 0) && lane == 0) have[buf][gg] = gp != nullptr;
-        if (!gp) return;
-        if (is_v) {
-            const int t0 = (g + gg) * kGroup;
-            if (t0 + kGroup > r.valid) {
+    auto fetch = [&](int g, auto slot) {  // this wave's share of the step at g, and the page id for the one after
+        constexpr int i = decltype(slot)::value;
+        gp[i] = groups.at(a, g + mine, page);
+        page = groups.id(a, g + mine + TG);
+        if (!gp[i]) return;
+        with_blocks([&](auto first, auto count) {
+            constexpr int b = decltype(first)::value, n = decltype(count)::value;
+            if (is_v) {
+                load_v<NB, b, b + n>(gp[i], lane, c[i], sc[i]);
+            } else {
+                load_words<NB>(gp[i] + 1024 * NB + lane % 16 * 4 * NB, sc[i]);
+                load_codes<NB, b, b + n>(gp[i], lane, c[i]);
+            }
+        });
+    };
+    auto convert = [&](int g, auto slot) {  // into the buffer of the slot's number
+        constexpr int i = decltype(slot)::value;
+        if (is_v && part == 0 && lane == 0) have[i][mine] = gp[i] != nullptr;
+        if (!gp[i]) return;
+        with_blocks([&](auto first, auto count) {
+            constexpr int b = decltype(first)::value, n = decltype(count)::value;
+            if (is_v) {
+                const int t0 = (g + mine) * kGroup;
+                if (t0 + kGroup > r.valid) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t keep = keep_mask(t0, quarter, j, r.valid);
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t keep = keep_mask(t0, quarter, j, r.valid);
 #pragma unroll
-                    for (int b = 0; b < B0; b++) sc[4 * b + j] &= keep;
+                        for (int e = 0; e < n; e++) sc[i][4 * e + j] &= keep;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < n; e++) {
+                    half8 vv[2];
+                    held_v(bits, c[i][2 * e], c[i][2 * e + 1], &sc[i][4 * e], vv);
+                    vf[i][mine][2 * (b + e)][lane] = vv[0];
+                    vf[i][mine][2 * (b + e) + 1][lane] = vv[1];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < n; e++) {
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        const int si = half * NB + b + e;
+                        kf[i][mine][si][lane] = held_k(bits, c[i][2 * e + half], as_half2(sc[i][si / 2])[si % 2]);
+                    }
                 }
             }
-            if (TG == 2 || part == 0) put_v(vf[buf][gg], 0, B0);
-            else put_v(vf[buf][gg], B0, NB - B0);
-        } else {
-            if (TG == 2 || part == 0) put_k(kf[buf][gg], std::integral_constant<int, 0>{}, std::integral_constant<int, B0>{});
-            else put_k(kf[buf][gg], std::integral_constant<int, B0>{}, std::integral_constant<int, NB - B0>{});
-        }
+        });
     };
 
-    if (pl.g_begin < pl.g_end) {
-        page = groups.id(a, TG == 2 ? pl.g_begin + part : pl.g_begin);
-        fetch(pl.g_begin);
+    constexpr std::integral_constant<int, 0> s0{};
+    constexpr std::integral_constant<int, 1> s1{};
+    const int g_begin = pl.g_begin, g_end = pl.g_end;
+    if (g_begin < g_end) {
+        page = groups.id(a, g_begin + mine);
+        fetch(g_begin, s0);
+        fetch(g_begin + TG, s1);
     }
     Q4Tile<NB, P> t[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) t[n].init(a, r.see, r.start, pl.h, f_wave + 16 * n + col, r.pairs, quarter);
-    if (pl.g_begin < pl.g_end) {
-        convert(pl.g_begin, 0);
-        fetch(pl.g_begin + TG);
+    if (g_begin < g_end) {
+        convert(g_begin, s0);
+        fetch(g_begin + 2 * TG, s0);
     }
     __syncthreads();
-    int buf = 0;
-    for (int g = pl.g_begin; g < pl.g_end; g += TG, buf ^= 1) {
-        if (g + TG < pl.g_end) {
-            convert(g + TG, buf ^ 1);
-            fetch(g + 2 * TG);
+    // one step: the next one's groups into the other buffer, the loads of the
+    // one two further, then the scores and sums of this one's
+    auto step = [&](int g, auto slot, auto other) {
+        constexpr int buf = decltype(slot)::value;
+        if (g + TG < g_end) {
+            convert(g + TG, other);
+            fetch(g + 3 * TG, other);
         }
 #pragma unroll
         for (int gg = 0; gg < TG; gg++) {
@@ -1226,6 +1373,10 @@ __global__ void __launch_bounds__(256) kv_q4_rows_kernel(Q4Attn a, int shares) {
             }
         }
         __syncthreads();
+    };
+    for (int g = g_begin; g < g_end; g += 2 * TG) {
+        step(g, s0, s1);
+        if (g + TG < g_end) step(g + TG, s1, s0);
     }
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -1263,8 +1414,9 @@ __global__ void __launch_bounds__(256) kv_q4_join_kernel(Q4Attn a, int shares) {
             seq_groups(a, base + 64 + lane, &lo, &groups);
             before = wave_before(groups, lane);
         }
-        groups = lane_value(groups, s - base);
-        const int x = (run + lane_value(before, s - base)) * a.b.n_kv + udiv(head, a.gq) * groups;
+        const int own = s - base;
+        const int x = (run + lane_value(before, own)) * a.b.n_kv + udiv(head, a.gq) * lane_value(groups, own);
+        groups = lane_value(groups, own);
         n = groups == 0 ? 0 : udiv(x + groups - 1, c.size) - udiv(x, c.size) + 1;
         if (n == 1) return;  // stored already
     } else {
@@ -1387,55 +1539,98 @@ int32_t make_batch(Q4Batch* b, const uint8_t* cache, size_t cache_len, size_t n_
     return MIVI_OK;
 }
 
+// Grid of the kernels that take whole groups: units times as many workgroups a
+// unit as fill the card (each wave at least one head's K or V); none (x = 0)
+// where the call has fewer than 8 rows a sequence: those go 8 values a lane.
+dim3 group_grid(size_t rows, size_t n_seq, size_t n_kv) {
+    if (rows < 8 * n_seq) return dim3(0, 0);
+    const size_t units = rows / kGroup + 2 * n_seq, most = (n_kv + 1) / 2;
+    const size_t want = (8 * (size_t)num_cus() + units - 1) / units;
+    return dim3((unsigned)units, (unsigned)std::min(most, want));
+}
+
+template <int T, class... Args>
+void launch_read_groups(size_t nb, dim3 grid, hipStream_t s, Args... args) {
+    switch (nb) {
+        case 1: kv_q4_read_groups_kernel<T, 1><<<grid, 256, 0, s>>>(args...); break;
+        case 2: kv_q4_read_groups_kernel<T, 2><<<grid, 256, 0, s>>>(args...); break;
+        case 3: kv_q4_read_groups_kernel<T, 3><<<grid, 256, 0, s>>>(args...); break;
+        case 4: kv_q4_read_groups_kernel<T, 4><<<grid, 256, 0, s>>>(args...); break;
+        case 6: kv_q4_read_groups_kernel<T, 6><<<grid, 256, 0, s>>>(args...); break;
+        default: kv_q4_read_groups_kernel<T, 8><<<grid, 256, 0, s>>>(args...); break;
+    }
+}
+
 // How an attention call is laid out.
 struct Q4Plan {
-    int nt;  // row tiles of 16 a wave of kv_q4_rows_kernel, 0: kv_q4_step_kernel
+    // kv_q4_step_kernel; kv_q4_rows_kernel of 64 pairs a workgroup (four waves
+    // of 16), of 128 (eight of 16, four of 32), of 256 (eight of 32)
+    enum { kStep, kFew, kSome, kMid, kMany } form;
     size_t tile_pairs, tiles, chunk, nsplit, shares, share_min, grid;
 };
 
-Q4Plan attn_plan(size_t n_seq, size_t max_rows, size_t gq, size_t n_kv, size_t cap, size_t window) {
+Q4Plan attn_plan(size_t n_seq, size_t max_rows, size_t gq, size_t n_kv, size_t hd, int planes, size_t cap,
+                 size_t window) {
     Q4Plan p = {};
-    const size_t pairs = max_rows * gq;
-    p.nt = pairs <= 16 ? 0 : pairs <= 64 ? 1 : 2;
-    p.tile_pairs = p.nt ? 64 * p.nt : 16;
+    const size_t pairs = max_rows * gq, cus = (size_t)num_cus();
+    size_t heads;
+    if (__builtin_mul_overflow(n_seq, n_kv, &heads)) heads = SIZE_MAX;
+    p.form = pairs <= 16    ? Q4Plan::kStep
+             : pairs <= 128 ? Q4Plan::kFew
+             : hd > 128     ? Q4Plan::kSome
+             : hd <= 96     ? Q4Plan::kMid
+             : planes == 2 || heads >= 2 * cus || heads * ((pairs + 255) / 256) >= 2 * cus ? Q4Plan::kMany
+                                                                                          : Q4Plan::kSome;
+    p.tile_pairs = p.form == Q4Plan::kStep ? 16 : p.form == Q4Plan::kFew ? 64 : p.form == Q4Plan::kMany ? 256 : 128;
     p.tiles = (pairs + p.tile_pairs - 1) / p.tile_pairs;
     // groups that a tile can see
     size_t tokens = cap;
     if (window) tokens = std::min(cap, std::min(window, cap) + p.tile_pairs / gq + 1 + 2 * kGroup);
-    const size_t groups = std::max<size_t>(1, (tokens + kGroup - 1) / kGroup), cus = (size_t)num_cus();
-    size_t all, heads;  // of one tile a sequence
-    if (__builtin_mul_overflow(n_seq, n_kv, &heads) || __builtin_mul_overflow(heads, groups, &all)) all = SIZE_MAX;
+    const size_t groups = std::max<size_t>(1, (tokens + kGroup - 1) / kGroup);
+    size_t all, wgs;
+    if (__builtin_mul_overflow(heads, groups, &all)) all = SIZE_MAX;
     if (p.tiles == 1 && all <= (size_t)INT32_MAX / 2) {
         // even shares: four workgroups a CU, each at least one step of every wave
         p.share_min = 4;
-        p.shares = std::min(cus * 4, std::max<size_t>((all + p.share_min - 1) / p.share_min, 1));
+        p.shares = std::min(cus * 4, (all + p.share_min - 1) / p.share_min);
         p.nsplit = std::min<size_t>({(size_t)kMaxSplit, p.shares / n_kv + 2, groups / p.share_min + 2});
         p.grid = p.shares + heads;
         return p;
     }
-    // tiles by themselves; shares of their groups where they are too few for the card
-    const size_t goal = 2 * cus;
-    size_t wgs;
+    // Tiles by themselves, their groups in shares where that fills the card
+    // better: the rounds that the workgroups take, one to three a CU, times a share's groups at about 1.1 us, against the join's 10 us and
+    // its traffic, twice the parts at 4 TB/s.
     if (__builtin_mul_overflow(heads, p.tiles, &wgs)) wgs = SIZE_MAX;
-    size_t chunk = wgs >= goal ? groups : (wgs * groups + goal - 1) / goal;
-    chunk = std::max(chunk, (groups + kMaxSplit - 1) / kMaxSplit);
-    p.chunk = (chunk + 3) / 4 * 4;
-    p.nsplit = (groups + p.chunk - 1) / p.chunk;
+    const size_t slots = cus * (p.form == Q4Plan::kFew ? 3 : p.form == Q4Plan::kMid ? 2 : 1);
+    double best = 0;
+    for (size_t ns = 1; ns <= (size_t)kMaxSplit && (ns == 1 || wgs < 4 * slots); ns++) {
+        const size_t chunk = ((groups + ns - 1) / ns + 3) / 4 * 4, n = (groups + chunk - 1) / chunk;
+        const size_t rounds = wgs == SIZE_MAX ? 1 : (wgs * n + slots - 1) / slots;
+        const double parts = (double)n_seq * max_rows * gq * n_kv * n * (hd + 2) * 4;
+        const double us = (double)rounds * chunk * 1.1 + (n > 1 ? 10 + 2 * parts / 4e6 : 0);
+        if (ns == 1 || us < best) best = us, p.chunk = chunk, p.nsplit = n;
+    }
     if (__builtin_mul_overflow(wgs, p.nsplit, &p.grid)) p.grid = SIZE_MAX;
     return p;
 }
 
 template <int NB, int P>
-void launch_attn(const Q4Attn& a, unsigned grid, int shares, int nt, hipStream_t s) {
+void launch_attn(const Q4Attn& a, const Q4Plan& p, hipStream_t s) {
+    const unsigned grid = (unsigned)p.grid;
+    const int shares = (int)p.shares;
     constexpr int TG = NB <= 4 ? 2 : 1;
-    if (nt == 0) kv_q4_step_kernel<NB, P><<<grid, 256, 0, s>>>(a, shares);
-    else if (nt == 1) kv_q4_rows_kernel<NB, P, 1, 1><<<grid, 256, 0, s>>>(a, shares);
-    else kv_q4_rows_kernel<NB, P, 2, TG><<<grid, 256, 0, s>>>(a, shares);
+    if (p.form == Q4Plan::kStep) kv_q4_step_kernel<NB, P><<<grid, 256, 0, s>>>(a, shares);
+    else if (p.form == Q4Plan::kFew) kv_q4_rows_kernel<NB, P, 1, 4, 1><<<grid, 256, 0, s>>>(a, shares);
+    else if (p.form == Q4Plan::kSome) kv_q4_rows_kernel<NB, P, 1, 8, 1><<<grid, 512, 0, s>>>(a, shares);
+    else if constexpr (NB <= 4) {
+        if (p.form == Q4Plan::kMid) kv_q4_rows_kernel<NB, P, 2, 4, TG><<<grid, 256, 0, s>>>(a, shares);
+        else kv_q4_rows_kernel<NB, P, 2, 8, TG><<<grid, 512, 0, s>>>(a, shares);
+    }
 }
 template <int NB>
-void launch_attn(const Q4Attn& a, unsigned grid, const Q4Plan& p, int planes, hipStream_t s) {
-    if (planes == 2) launch_attn<NB, 2>(a, grid, (int)p.shares, p.nt, s);
-    else launch_attn<NB, 1>(a, grid, (int)p.shares, p.nt, s);
+void launch_attn(const Q4Attn& a, const Q4Plan& p, int planes, hipStream_t s) {
+    if (planes == 2) launch_attn<NB, 2>(a, p, s);
+    else launch_attn<NB, 1>(a, p, s);
 }
 
 }  // namespace
@@ -1466,18 +1661,19 @@ extern "C" int32_t mivi_hip_kv_q4_append(uint8_t* cache, size_t cache_len, size_
     const size_t e = type_bytes(type);
     const int wk = wide_ok(k, k_row_stride, k_head_stride, e, 16), wv = wide_ok(v, v_row_stride, v_head_stride, e, 16);
     hipStream_t s = (hipStream_t)stream;
-    // A wave a group where the call has 8 rows a sequence or more, else 8 values
-    // a lane wherever they lie.
-    const bool by_group = rows >= 8 * n_seq;
-    const dim3 grid = by_group ? dim3((unsigned)(rows / kGroup + 2 * n_seq), (unsigned)((2 * n_kv_heads + 3) / 4))
-                               : dim3((unsigned)blocks, 2);
-#define APPEND(T)                                                                                                      \
-    (by_group ? kv_q4_append_groups_kernel<T> : kv_q4_append_kernel<T>)<<<grid, 256, 0, s>>>(                           \
-        b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride, (int64_t)v_row_stride, (int64_t)v_head_stride,       \
-        (int)rows, wk, wv)
-    if (type == MIVI_GGML_F32) APPEND(MIVI_GGML_F32);
-    else if (type == MIVI_GGML_F16) APPEND(MIVI_GGML_F16);
-    else APPEND(MIVI_GGML_BF16);
+    const dim3 grid = group_grid(rows, n_seq, n_kv_heads);
+#define APPEND(T)                                                                                                    \
+    if (grid.x)                                                                                                      \
+        kv_q4_append_groups_kernel<T><<<grid, 256, 0, s>>>(b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride,   \
+                                                           (int64_t)v_row_stride, (int64_t)v_head_stride, (int)rows, \
+                                                           wk, wv);                                                  \
+    else                                                                                                             \
+        kv_q4_append_kernel<T><<<dim3((unsigned)blocks, 2), 256, 0, s>>>(                                            \
+            b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride, (int64_t)v_row_stride, (int64_t)v_head_stride,   \
+            (int)rows, wk, wv)
+    if (type == MIVI_GGML_F32) { APPEND(MIVI_GGML_F32); }
+    else if (type == MIVI_GGML_F16) { APPEND(MIVI_GGML_F16); }
+    else { APPEND(MIVI_GGML_BF16); }
 #undef APPEND
     MIVI_HIP_CHECK(hipGetLastError());
     return MIVI_OK;
@@ -1504,18 +1700,18 @@ extern "C" int32_t mivi_hip_kv_q4_read(const uint8_t* cache, size_t cache_len, s
     const size_t e = type_bytes(type);
     const int wk = wide_ok(k, k_row_stride, k_head_stride, e, 16), wv = wide_ok(v, v_row_stride, v_head_stride, e, 16);
     hipStream_t s = (hipStream_t)stream;
-    // A wave a group where the call has 8 rows a sequence or more, else 8 values
-    // a lane wherever they lie.
-    const bool by_group = rows >= 8 * n_seq;
-    const dim3 grid = by_group ? dim3((unsigned)(rows / kGroup + 2 * n_seq), (unsigned)((2 * n_kv_heads + 3) / 4))
-                               : dim3((unsigned)blocks, 2);
+    const dim3 grid = group_grid(rows, n_seq, n_kv_heads);
 #define READ(T)                                                                                                      \
-    (by_group ? kv_q4_read_groups_kernel<T> : kv_q4_read_kernel<T>)<<<grid, 256, 0, s>>>(                           \
-        b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride, (int64_t)v_row_stride, (int64_t)v_head_stride,       \
-        (int)rows, wk, wv)
-    if (type == MIVI_GGML_F32) READ(MIVI_GGML_F32);
-    else if (type == MIVI_GGML_F16) READ(MIVI_GGML_F16);
-    else READ(MIVI_GGML_BF16);
+    if (grid.x)                                                                                                      \
+        launch_read_groups<T>(head_dim / 32, grid, s, b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride,        \
+                              (int64_t)v_row_stride, (int64_t)v_head_stride, (int)rows, wk, wv);                     \
+    else                                                                                                             \
+        kv_q4_read_kernel<T><<<dim3((unsigned)blocks, 2), 256, 0, s>>>(                                              \
+            b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride, (int64_t)v_row_stride, (int64_t)v_head_stride,   \
+            (int)rows, wk, wv)
+    if (type == MIVI_GGML_F32) { READ(MIVI_GGML_F32); }
+    else if (type == MIVI_GGML_F16) { READ(MIVI_GGML_F16); }
+    else { READ(MIVI_GGML_BF16); }
 #undef READ
     MIVI_HIP_CHECK(hipGetLastError());
     return MIVI_OK;
@@ -1525,8 +1721,11 @@ extern "C" size_t mivi_hip_kv_q4_attention_workspace(size_t n_seq, size_t rows, 
                                                      size_t n_kv_heads, size_t head_dim, size_t max_tokens,
                                                      size_t window) {
     if (n_kv_heads == 0 || n_heads == 0 || n_heads % n_kv_heads || rows == 0 || n_seq == 0 || max_rows == 0) return 0;
-    const Q4Plan p = attn_plan(n_seq, std::min(max_rows, rows), n_heads / n_kv_heads, n_kv_heads, max_tokens, window);
-    return p.nsplit == 1 ? 0 : rows * n_heads * p.nsplit * (head_dim + 2) * sizeof(float);
+    size_t parts = 1;
+    for (int planes = 1; planes <= 2; planes++)
+        parts = std::max(parts, attn_plan(n_seq, std::min(max_rows, rows), n_heads / n_kv_heads, n_kv_heads, head_dim,
+                                          planes, max_tokens, window).nsplit);
+    return parts == 1 ? 0 : rows * n_heads * parts * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int32_t mivi_hip_kv_q4_attention(
@@ -1549,7 +1748,7 @@ extern "C" int32_t mivi_hip_kv_q4_attention(
     max_rows = std::min(max_rows, rows);
     const size_t gq = n_heads / n_kv_heads, cap = pages_per_seq * page_tokens;
     const int planes = type == MIVI_GGML_F32 ? 2 : 1;
-    const Q4Plan p = attn_plan(n_seq, max_rows, gq, n_kv_heads, cap, window);
+    const Q4Plan p = attn_plan(n_seq, max_rows, gq, n_kv_heads, head_dim, planes, cap, window);
     const size_t need =
         mivi_hip_kv_q4_attention_workspace(n_seq, rows, max_rows, n_heads, n_kv_heads, head_dim, cap, window);
     if (workspace_bytes < need) return err_buffer_too_small(need, workspace_bytes);
@@ -1575,12 +1774,12 @@ extern "C" int32_t mivi_hip_kv_q4_attention(
     a.part_ml = a.part_acc + rows * n_heads * p.nsplit * head_dim;
     hipStream_t s = (hipStream_t)stream;
     switch (head_dim / 32) {
-        case 1: launch_attn<1>(a, (unsigned)p.grid, p, planes, s); break;
-        case 2: launch_attn<2>(a, (unsigned)p.grid, p, planes, s); break;
-        case 3: launch_attn<3>(a, (unsigned)p.grid, p, planes, s); break;
-        case 4: launch_attn<4>(a, (unsigned)p.grid, p, planes, s); break;
-        case 6: launch_attn<6>(a, (unsigned)p.grid, p, planes, s); break;
-        default: launch_attn<8>(a, (unsigned)p.grid, p, planes, s); break;
+        case 1: launch_attn<1>(a, p, planes, s); break;
+        case 2: launch_attn<2>(a, p, planes, s); break;
+        case 3: launch_attn<3>(a, p, planes, s); break;
+        case 4: launch_attn<4>(a, p, planes, s); break;
+        case 6: launch_attn<6>(a, p, planes, s); break;
+        default: launch_attn<8>(a, p, planes, s); break;
     }
     MIVI_HIP_CHECK(hipGetLastError());
     if (p.nsplit > 1) {

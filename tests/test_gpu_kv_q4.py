@@ -94,16 +94,16 @@ def check_attention(got, want, mag, top, dtype, hd, longest, big=6.0):
     relative to itself, plus 2^-22 of the exponential, plus 2^-11 where weights
     are one fp16 plane and 2^-22 where two. Numerator and denominator: twice
     that. Sums over the tokens: no chain is longer than one in four of them
-    plus the joins. A weight is an fp16 number times 2^-15 of the row's largest
-    so far: the last plane of one so small that it is a denormal is off by half
-    of 2^-24 there, 2^-40 of the largest and so of the denominator; over
-    `longest` tokens of values up to `big` that is longest * 2^-40 * big. Then
-    half a step of the output's type."""
+    plus the joins. A weight is an fp16 number times 2^-11 of the row's reference,
+    which is no larger than its largest weight: the last plane of one so small
+    that it is a denormal is off by half of 2^-24 there, 2^-36 of the largest and
+    so of the denominator; over `longest` tokens of values up to `big` that is
+    longest * 2^-36 * big. Then half a step of the output's type."""
     u = 2.0 ** -24
     planes = 2.0 ** -22 if dtype == torch.float32 else 0.0
     eps = top[..., None] * ((hd + 8) * u + planes) + 2.0 ** -21
     eps = eps + (2.0 ** -22 if dtype == torch.float32 else 2.0 ** -11)
-    bound = mag * (2 * eps + (longest / 4 + 64) * u) + longest * 2.0 ** -40 * big
+    bound = mag * (2 * eps + (longest / 4 + 64) * u) + longest * 2.0 ** -36 * big
     bound = bound + (want.abs() + bound) * (torch.finfo(dtype).eps / 2) + torch.finfo(dtype).tiny
     err = (got.double().cpu() - want).abs()
     assert torch.isfinite(got).all()

@@ -1103,9 +1103,9 @@ constexpr int step_waves(int nb, int p) {
 }
 template <int NB, int P>
 __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4Attn a, int shares) {
-    constexpr int hd = 32 * NB;
-    __shared__ float red_ml[4][16][2];
-    __shared__ float red_acc[4][16][hd + 4];
+    constexpr int hd = 32 * NB, NW = 4;
+    __shared__ float red_ml[NW][16][2];
+    __shared__ float red_acc[NW][16][hd + 4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quarter = lane >> 4;
     Q4Place pl;
@@ -1120,9 +1120,9 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
     const uint8_t *gp = nullptr, *next = nullptr;
     int id = -1;  // page id of the group after next
     if (g < pl.g_end) {
-        const int id0 = groups.id(a, g), id1 = groups.id(a, g + 4);
-        id = groups.id(a, g + 8);
-        gp = groups.at(a, g, id0), next = groups.at(a, g + 4, id1);
+        const int id0 = groups.id(a, g), id1 = groups.id(a, g + NW);
+        id = groups.id(a, g + 2 * NW);
+        gp = groups.at(a, g, id0), next = groups.at(a, g + NW, id1);
         // loads go somewhere in any case: a group that is not there is read as
         // the cache's first, and hidden
         load_k<NB>(gp ? gp : a.b.cache, lane, k, ks);
@@ -1130,10 +1130,10 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
     }
     t.init(a, r.see, r.start, pl.h, col, r.pairs, quarter);
 
-    for (; g < pl.g_end; g += 4) {
+    for (; g < pl.g_end; g += NW) {
         const uint8_t* from = next ? next : a.b.cache;
-        const uint8_t* after = groups.at(a, g + 8, id);
-        id = groups.id(a, g + 12);
+        const uint8_t* after = groups.at(a, g + 2 * NW, id);
+        id = groups.id(a, g + 3 * NW);
         // scores: rows tokens, columns query rows
         f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -1177,7 +1177,7 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
         gp = next, next = after;
     }
 
-    // join the four waves
+    // join the waves
     constexpr int kQuads = hd / 4;
     if (quarter == 0) red_ml[wave][col][0] = t.m, red_ml[wave][col][1] = t.l[0];
 #pragma unroll
@@ -1188,11 +1188,11 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
         if (f >= r.pairs) continue;
         float m = -__builtin_inff();  // never NaN: a NaN score is in the sums alone
 #pragma unroll
-        for (int w = 0; w < 4; w++) m = fmaxf(m, red_ml[w][f][0]);
+        for (int w = 0; w < NW; w++) m = fmaxf(m, red_ml[w][f][0]);
         const float m_ref = m == -__builtin_inff() ? 0.f : m;
         float l = 0.f, o[4] = {};
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < NW; w++) {
             const float e = __builtin_amdgcn_exp2f(red_ml[w][f][0] - m_ref);
             l = fmaf(e, red_ml[w][f][1], l);
             const f32x4 x = *(const f32x4*)&red_acc[w][f][d4];
@@ -1390,6 +1390,19 @@ __global__ void __launch_bounds__(64 * NW) kv_q4_rows_kernel(Q4Attn a, int share
     }
 }
 
+// wave_max without LDS traffic, as xsum_all64.
+__device__ __forceinline__ float xmax_all64(float v) {
+    float a, b;
+    swap32(v, a, b);
+    v = fmaxf(a, b);
+    swap16(v, a, b);
+    v = fmaxf(a, b);
+    v = fmaxf(v, dpp_mov<0x128>(v));
+    v = fmaxf(v, xor4_mov(v));
+    v = fmaxf(v, dpp_mov<0x4E>(v));
+    return fmaxf(v, dpp_mov<0xB1>(v));
+}
+
 // The parts of a (row, head) joined by one wave: lane i weighs part i (there
 // are at most 64), then the lanes take four values each of 256 / hd parts at a
 // time. `shares`: workgroups of the even shares.
@@ -1425,20 +1438,27 @@ __global__ void __launch_bounds__(256) kv_q4_join_kernel(Q4Attn a, int shares) {
         tile_groups(r.see, row_of(a, f0), row_of(a, min(f0 + a.tile_pairs, r.pairs) - 1), &g_lo, &g_hi);
         n = min((max(g_hi - g_lo, 0) + a.chunk - 1) / a.chunk, a.nsplit);
     }
-    const float* ml = a.part_ml + pr * a.nsplit * 2;
-    const float m_i = lane < n ? ml[2 * lane] : -__builtin_inff();
-    const float l_i = lane < n ? ml[2 * lane + 1] : 0.f;
     const int quads = hd / 4, per = 64 / quads;  // hd 96 and 192: lanes past the last quad repeat one
     const int d4 = lane % quads * 4, first = min(lane / quads, per - 1);
-    float o[4] = {};
     const float* pa = a.part_acc + pr * a.nsplit * hd + d4;
-    const float m = wave_max(m_i);
-    const float e_i = __builtin_amdgcn_exp2f(m_i - (m == -__builtin_inff() ? 0.f : m));  // 0 from part n on
-    const float l = wave_sum(e_i * l_i);
-    for (int j = 0; j < n; j += 8 * per) {
-        f32x4 x[8];
+    const float* ml = a.part_ml + pr * a.nsplit * 2;
+    // all loads of up to 8 per parts, before any use
+    f32x4 x[8];
+    auto fetch = [&](int j) {
 #pragma unroll
         for (int c = 0; c < 8; c++) x[c] = *(const f32x4*)(pa + (int64_t)min(j + c * per + first, n - 1) * hd);
+    };
+    float m_i = -__builtin_inff(), l_i = 0.f;
+    if (n) {
+        if (lane < n) m_i = ml[2 * lane], l_i = ml[2 * lane + 1];
+        fetch(0);
+    }
+    float o[4] = {};
+    const float m = xmax_all64(m_i);
+    const float e_i = __builtin_amdgcn_exp2f(m_i - (m == -__builtin_inff() ? 0.f : m));  // 0 from part n on
+    const float l = xsum_all64(e_i * l_i);
+    for (int j = 0; j < n; j += 8 * per) {
+        if (j) fetch(j);
 #pragma unroll
         for (int c = 0; c < 8; c++) {
             const int k = j + c * per + first;
@@ -1589,6 +1609,15 @@ Q4Plan attn_plan(size_t n_seq, size_t max_rows, size_t gq, size_t n_kv, size_t h
     const size_t groups = std::max<size_t>(1, (tokens + kGroup - 1) / kGroup);
     size_t all, wgs;
     if (__builtin_mul_overflow(heads, groups, &all)) all = SIZE_MAX;
+    // One part a head, which needs no second kernel, where it is short: 8 groups
+    // a wave, 4 of more than 128 dimensions, 8 groups in all of more rows. (One
+    // token, 8 heads of 64, f32: at 1024 tokens 9.9 us against 12.9 in shares and
+    // a join, 14.7 at 2048; 64 sequences at 1024 18.7 against 22.8; 4 heads of
+    // 256 at 512 13.0 and 13.8; 16 rows at 256 10.5 and 14.)
+    if (p.tiles == 1 && groups <= (p.form == Q4Plan::kStep ? hd <= 128 ? 32 : 16 : 8)) {
+        p.chunk = groups, p.nsplit = 1, p.grid = heads;
+        return p;
+    }
     if (p.tiles == 1 && all <= (size_t)INT32_MAX / 2) {
         // even shares: four workgroups a CU, each at least one step of every wave
         p.share_min = 4;
@@ -1741,6 +1770,8 @@ extern "C" int32_t mivi_hip_kv_q4_attention(
     if (rc) return rc;
     if (n_heads == 0 || n_heads % n_kv_heads || n_heads > 65535)
         return set_error(MIVI_ERR_INVALID_ARGUMENT, "%zu heads over %zu kv heads", n_heads, n_kv_heads);
+    if (!(scale >= -3.402823466e38f && scale <= 3.402823466e38f))
+        return set_error(MIVI_ERR_INVALID_ARGUMENT, "scale %g is not finite", (double)scale);
     if (rows == 0 || n_seq == 0 || max_rows == 0) return clear_error();
     if ((rc = check_tensor("q", q, q_len, type, rows, q_row_stride, n_heads, q_head_stride, head_dim, false)) ||
         (rc = check_tensor("out", out, out_len, type, rows, out_row_stride, n_heads, out_head_stride, head_dim, true)))

@@ -12,6 +12,7 @@ from . import _check, _lib
 
 torch = None  # imported by the first cache: the rest of the package works without it
 _TYPES = {}   # torch dtype -> GgmlType
+_needs = {}   # a call's sizes -> the bytes of its workspace
 _append = _lib.mivi_hip_kv_q4_append
 _read = _lib.mivi_hip_kv_q4_read
 _attention = _lib.mivi_hip_kv_q4_attention
@@ -136,8 +137,13 @@ def kv_q4_attention(out, q, cache: KvCacheQ4, starts, lens, max_rows: int | None
     if window < 0 or max_rows < 0:
         raise ValueError("window and max_rows are not negative")
     batch = cache._batch(starts, lens)
-    need = _workspace(cache._table[3], rows, max_rows, heads, cache.n_kv_heads, cache.head_dim,
-                      cache._table[2] * cache.page_tokens, window)
+    sizes = (cache._table[3], rows, max_rows, heads, cache.n_kv_heads, cache.head_dim,
+             cache._table[2] * cache.page_tokens, window)
+    need = _needs.get(sizes)
+    if need is None:
+        if len(_needs) >= 1024:
+            _needs.clear()
+        need = _needs[sizes] = _workspace(*sizes)
     device = cache.device
     if workspace is None and need:
         if stream is None:

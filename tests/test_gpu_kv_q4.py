@@ -481,6 +481,95 @@ def test_a_cache_past_four_gigabytes(hip):
     check_attention(out, want, mag, top, torch.float32, hd, t)
 
 
+@pytest.mark.parametrize("n,kv,heads,most,few", [
+    (70, 2, 8, 400, 1),      # more sequences than a wave has lanes
+    (300, 1, 1, 130, 1),
+    (65, 3, 6, 3000, 1),
+    (130, 2, 16, 90, 5),
+    (3, 70, 70, 1500, 1),    # more heads than a wave has lanes
+    (2, 66, 132, 2100, 9),
+])
+def test_attention_of_many_sequences_and_heads(hip, n, kv, heads, most, few):
+    """Ragged batches over tables of different spare room: lengths of zero, one
+    and the table's, sequences without rows."""
+    r = np.random.RandomState(n)
+    lens = r.randint(0, most + 1, n)
+    lens[r.randint(0, n, 2)] = most
+    lens[n // 2], lens[n - 1] = 0, 1
+    rows = r.randint(0, few + 1, n) if few > 1 else np.where(r.rand(n) < 0.2, 0, 1)
+    rows[0] = few
+    for cap in (most, 4 * most):
+        b = Batch(hip, rows.tolist(), lens.tolist(), kv, 32, 32, cap=cap, seed=n)
+        kvs = b.fill(hip)
+        q = torch.randn((int(rows.sum()), heads, 32), generator=torch.Generator().manual_seed(n))
+        for window in (0, 50):
+            out = torch.full(q.shape, 5.0, device="cuda")
+            hip.kv_q4_attention(out, q.cuda(), b.cache, b.starts_t, b.lens_t, few, 0.2, window)
+            want, mag, top = reference(q, kvs, rows.tolist(), lens.tolist(), 0.2, window)
+            check_attention(out, want, mag, top, torch.float32, 32, most)
+
+
+@pytest.mark.parametrize("n,rows_of", [(70, lambda r, n: r.randint(0, 40, n)), (200, lambda r, n: r.randint(5, 15, n)),
+                                       (200, lambda r, n: np.where(r.rand(n) < 0.3, 0, 1))])
+def test_rows_of_many_sequences_written_and_read_back(hip, n, rows_of):
+    r = np.random.RandomState(n)
+    rows = rows_of(r, n)
+    lens = rows + r.randint(0, 100, n)
+    b = Batch(hip, rows.tolist(), lens.tolist(), 3, 32, 64, seed=n)
+    x = torch.randn((int(rows.sum()), 6, 32), generator=torch.Generator().manual_seed(n)).cuda()
+    hip.kv_q4_append(b.cache, x[:, :3], x[:, 3:], b.starts_t, b.lens_t)
+    ko, vo = (torch.full((x.shape[0], 3, 32), 9.0, device="cuda") for _ in range(2))
+    hip.kv_q4_read(b.cache, ko, vo, b.starts_t, b.lens_t)
+    assert torch.equal(ko.cpu().double(), held(x[:, :3])) and torch.equal(vo.cpu().double(), held(x[:, 3:]))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 30, 60])
+def test_attention_negative_and_zero_scales(hip, rows):
+    heads, kv, hd = 8, 2, 64
+    b = Batch(hip, [rows], [1500], kv, hd, 64)
+    kvs = b.fill(hip)
+    q = torch.randn((rows, heads, hd), generator=torch.Generator().manual_seed(4))
+    out = torch.empty(q.shape, device="cuda")
+    for scale in (-0.3, 0.0, 1e-38):
+        hip.kv_q4_attention(out, q.cuda(), b.cache, b.starts_t, b.lens_t, rows, scale)
+        want, mag, top = reference(q, kvs, [rows], [1500], scale)
+        check_attention(out, want, mag, top, torch.float32, hd, 1500)
+
+
+@pytest.mark.parametrize("hd,kv,heads", [(64, 2, 16), (128, 1, 8), (256, 1, 4)])
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_attention_of_every_form(hip, name, hd, kv, heads):
+    """Row counts on both sides of each form's limits, over a table of 40 groups
+    and a window that starts inside one."""
+    dt = TYPES[name]
+    g = heads // kv
+    for pairs in (16, 24, 64, 72, 128, 136, 256, 520):
+        rows = -(-pairs // g)
+        b = Batch(hip, [rows, 1], [1280, 700], kv, hd, 32)
+        kvs = b.fill(hip)
+        q = torch.randn((rows + 1, heads, hd), generator=torch.Generator().manual_seed(pairs)).to(dt)
+        for window in (0, 333):
+            out = torch.empty(q.shape, dtype=dt, device="cuda")
+            hip.kv_q4_attention(out, q.cuda(), b.cache, b.starts_t, b.lens_t, rows, None, window)
+            want, mag, top = reference(q, kvs, [rows, 1], [1280, 700], hd ** -0.5, window)
+            check_attention(out, want, mag, top, dt, hd, 1280)
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_attention_rows_of_many_heads(hip, name):
+    """Enough heads for the largest workgroups of 16-bit types; the second tile
+    of a head has a few rows only."""
+    dt = TYPES[name]
+    heads, kv, hd, rows, lens = 64, 64, 128, [260] + [1] * 7, [300] + [33] * 7
+    b = Batch(hip, rows, lens, kv, hd, 64)
+    kvs = b.fill(hip)
+    q = torch.randn((sum(rows), heads, hd), generator=torch.Generator().manual_seed(4)).to(dt)
+    out = torch.empty(q.shape, dtype=dt, device="cuda")
+    hip.kv_q4_attention(out, q.cuda(), b.cache, b.starts_t, b.lens_t, 260)
+    want, mag, top = reference(q, kvs, rows, lens, hd ** -0.5)
+    check_attention(out, want, mag, top, dt, hd, 300)
+
+
 # ------------------------------------------------------- as they are used
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 def test_prompts_in_passes_then_single_tokens(hip, name):

@@ -26,9 +26,10 @@ def kv_call(fn, geo=None, k=None, v=None, typ=0, rows=7):
     return fn(*(geo or geometry()), typ, *(k or rows_args()), *(v or rows_args()), rows, None)
 
 
-def attn(geo=None, out=None, q=None, typ=0, rows=7, max_rows=7, heads=4, window=0, ws=A, ws_bytes=1 << 40):
+def attn(geo=None, out=None, q=None, typ=0, rows=7, max_rows=7, heads=4, window=0, ws=A, ws_bytes=1 << 40,
+         scale=0.125):
     return LIB.mivi_hip_kv_q4_attention(typ, *(out or rows_args(kv=4)), *(q or rows_args(kv=4)), rows, max_rows, heads,
-                                        0.125, window, *(geo or geometry()), ws, ws_bytes, None)
+                                        scale, window, *(geo or geometry()), ws, ws_bytes, None)
 
 
 CALLS = [lambda **k: kv_call(LIB.mivi_hip_kv_q4_append, **k), lambda **k: kv_call(LIB.mivi_hip_kv_q4_read, **k), attn]
@@ -90,14 +91,17 @@ def test_written_rows_may_not_overlap():
 
 def test_attention_refusals():
     assert attn(heads=5) == 101 and attn(heads=0) == 101
+    for scale in (float("inf"), float("-inf"), float("nan")):
+        assert attn(scale=scale) == 101
     full = rows_args(kv=4)
     assert attn(q=[A, full[1] - 1] + full[2:]) == 2
     assert attn(out=[None] + full[1:]) == 101
-    need = LIB.mivi_hip_kv_q4_attention_workspace(3, 7, 7, 4, 2, 64, 256, 0)
-    if need:
-        assert attn(ws_bytes=need - 1) == 2 and mivi_hip.last_error().expected == need
-        assert attn(ws=None, ws_bytes=need) == 101
-        assert attn(ws=A + 4, ws_bytes=need) == 101
+    geo = geometry(page=1024, pstride=64, per=64)
+    need = LIB.mivi_hip_kv_q4_attention_workspace(3, 7, 7, 4, 2, 64, 64 * 1024, 0)
+    assert need > 0
+    assert attn(geo=geo, ws_bytes=need - 1) == 2 and mivi_hip.last_error().expected == need
+    assert attn(geo=geo, ws=None, ws_bytes=need) == 101
+    assert attn(geo=geo, ws=A + 4, ws_bytes=need) == 101
 
 
 def test_nothing_to_do_is_ok():

@@ -212,7 +212,8 @@ int32_t mivi_hip_dot_q8_0_f32(const float* q, size_t q_len, const uint8_t* k_blo
  * of head_dim (32, 64, 96, 128, 192 or 256). Its inner order is the library's.
  * `pages`: page ids on the device, n_seq rows of pages_per_seq, pages_stride
  * apart: token t of sequence s is in page pages[s * pages_stride + t /
- * page_tokens]. Sequences may share pages that none of them writes.
+ * page_tokens]. Sequences may share pages; a page that a call writes belongs to
+ * one place of the table.
  * `starts` [n_seq + 1], `lens` [n_seq] on the device: rows starts[s] ..
  * starts[s + 1] - 1 of a call's tensors belong to sequence s and are its last
  * positions: row i of its n is at position lens[s] - n + i (lens counts them).

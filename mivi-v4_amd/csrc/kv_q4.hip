@@ -44,11 +44,9 @@ using namespace mivi;
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2_a4 __attribute__((ext_vector_type(2), aligned(4)));
-typedef uint32_t u32x4_a8 __attribute__((ext_vector_type(4), aligned(8)));
 
 constexpr int kGroup = 32;         // tokens of a group
 constexpr float kMaxScale = 2720;  // 170 * 2^4 (8 significant bits): 24 times it is an fp16 number
@@ -480,6 +478,11 @@ __device__ __forceinline__ _Float16 k_scale(const uint32_t (&ks)[NB], int half, 
 // groups' units from U(s) = starts[s] / 32 + 2 s on: its n rows touch at most
 // (n - 2) / 32 + 2 groups, and U(s + 1) - U(s) is no less, so no sum over the
 // sequences is needed to place them.
+//
+// 24 bf16 prompts of up to 701 rows, 8 heads of 128 (52 MB in, 15 out): written
+// in 23.6 us, 17 vector instructions an element and 64 lanes, read in 14.9; 8
+// values a lane wherever they lie took 48 and 36. 8 x 32768 rows of 8 heads of 64
+// to fp16 (688 MB): 165 us, 4.2 TB/s, 81 % of a copy's rate.
 struct Q4Unit {
     int s, g;      // sequence and group
     bool there;    // whether the table has a page of the cache there
@@ -1095,6 +1098,14 @@ __device__ __forceinline__ bool head_place(const Q4Attn& a, int lane, int shares
 // weights). K of the next group is on its way during the sums, V during the
 // scores, and page ids two groups ahead of that.
 //
+// Bound: about 200 (hd 64, two planes) to 290 (hd 128, one) vector instructions
+// a group, half of them codes to values, 60 % of the cycles; the loads alone take
+// 28 us where the kernel takes 41 (8 sequences of 32768 tokens, 8 heads of 64,
+// f32: 151 MB, 3.6 TB/s). 64 ragged sequences of up to 8192, 8 heads of 128, bf16:
+// 71 us, 297 MB, 4.2 TB/s. No faster: the next group's scores formed beside this
+// one's sums (46 us), five waves a SIMD (45), four groups' scores in sets of four
+// columns (fewer exponentials, two waves a SIMD: 41).
+//
 // Waves a SIMD that the registers are held to: 17 nb words of codes, scales and
 // sums and 4 nb a plane of queries beside about 40 others.
 constexpr int step_waves(int nb, int p) {
@@ -1209,6 +1220,13 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
 // one is worked on while the next groups are converted into the other, and the
 // two steps after are on their way from memory. Each wave converts K or V of
 // some blocks of one group.
+//
+// Bound: vector instructions and matrix instructions of a SIMD in turn. 2 x 2048
+// bf16 rows at 32768 tokens, 32 / 8 heads of 128 (NT 2, NW 8): 2.22 ms, 905
+// TFLOP/s, matrix pipe busy 40 %, vector pipe 43; with four waves a conversion
+// 2.48 ms. 2048 f32 rows at 4096, heads of 64: 132 us, the planes doubling both
+// products. 16 x 5 bf16 rows at up to 12000 tokens, 4 heads of 128 (NT 1): 36 us,
+// the chain of barrier, scores, weights and sums of one tile a wave.
 template <int NB, int P, int NT, int NW, int TG>
 __global__ void __launch_bounds__(64 * NW) kv_q4_rows_kernel(Q4Attn a, int shares) {
     constexpr int kPer = NW / 2 / TG;                             // waves of a group, K or V
@@ -1595,6 +1613,13 @@ Q4Plan attn_plan(size_t n_seq, size_t max_rows, size_t gq, size_t n_kv, size_t h
     const size_t pairs = max_rows * gq, cus = (size_t)num_cus();
     size_t heads;
     if (__builtin_mul_overflow(n_seq, n_kv, &heads)) heads = SIZE_MAX;
+    // By registers: two tiles a wave and two or three workgroups a CU up to 96
+    // dimensions, one tile a wave past 128; at 128 the 256 pairs that share a
+    // conversion need two workgroups a CU's worth of tiles to end evenly (2 x
+    // 2048 bf16 rows at 32768: 2210 us, with 128 pairs 2420; 2048 rows of one
+    // prompt from its start 84 and 67), and two planes do not fit one tile a wave
+    // twice on a CU (2 x 700 f32 rows at 32768: 1290 and 1670). 65 to 128 pairs
+    // as two tiles of 64: 8 x 25 f32 rows at 4096 57.6 us, as one of 128 109.
     p.form = pairs <= 16    ? Q4Plan::kStep
              : pairs <= 128 ? Q4Plan::kFew
              : hd > 128     ? Q4Plan::kSome
@@ -1647,13 +1672,24 @@ template <int NB, int P>
 void launch_attn(const Q4Attn& a, const Q4Plan& p, hipStream_t s) {
     const unsigned grid = (unsigned)p.grid;
     const int shares = (int)p.shares;
-    constexpr int TG = NB <= 4 ? 2 : 1;
-    if (p.form == Q4Plan::kStep) kv_q4_step_kernel<NB, P><<<grid, 256, 0, s>>>(a, shares);
-    else if (p.form == Q4Plan::kFew) kv_q4_rows_kernel<NB, P, 1, 4, 1><<<grid, 256, 0, s>>>(a, shares);
-    else if (p.form == Q4Plan::kSome) kv_q4_rows_kernel<NB, P, 1, 8, 1><<<grid, 512, 0, s>>>(a, shares);
-    else if constexpr (NB <= 4) {
-        if (p.form == Q4Plan::kMid) kv_q4_rows_kernel<NB, P, 2, 4, TG><<<grid, 256, 0, s>>>(a, shares);
-        else kv_q4_rows_kernel<NB, P, 2, 8, TG><<<grid, 512, 0, s>>>(a, shares);
+    if (p.form == Q4Plan::kStep) {
+        kv_q4_step_kernel<NB, P><<<grid, 256, 0, s>>>(a, shares);
+    } else if (p.form == Q4Plan::kFew) {
+        // two groups a step at 64 dimensions (16 x 5 rows 44.7 -> 39.3 us); at 128
+        // their LDS halves the workgroups of a CU (57 -> 63)
+        kv_q4_rows_kernel<NB, P, 1, 4, NB <= 2 ? 2 : 1><<<grid, 256, 0, s>>>(a, shares);
+    } else if constexpr (NB <= 3) {
+        kv_q4_rows_kernel<NB, P, 2, 4, 2><<<grid, 256, 0, s>>>(a, shares);
+    } else if constexpr (NB == 4) {
+        if constexpr (P == 1) {
+            if (p.form == Q4Plan::kSome) {
+                kv_q4_rows_kernel<NB, P, 1, 8, 1><<<grid, 512, 0, s>>>(a, shares);
+                return;
+            }
+        }
+        kv_q4_rows_kernel<NB, P, 2, 8, 2><<<grid, 512, 0, s>>>(a, shares);
+    } else {
+        kv_q4_rows_kernel<NB, P, 1, 8, 1><<<grid, 512, 0, s>>>(a, shares);
     }
 }
 template <int NB>

@@ -482,7 +482,7 @@ __device__ __forceinline__ _Float16 k_scale(const uint32_t (&ks)[NB], int half, 
 // 24 bf16 prompts of up to 701 rows, 8 heads of 128 (52 MB in, 15 out): written
 // in 23.6 us, 17 vector instructions an element and 64 lanes, read in 14.9; 8
 // values a lane wherever they lie took 48 and 36. 8 x 32768 rows of 8 heads of 64
-// to fp16 (688 MB): 165 us, 4.2 TB/s, 81 % of a copy's rate.
+// to fp16 (688 MB): 148 us, 4.6 TB/s, 90 % of a copy's rate.
 struct Q4Unit {
     int s, g;      // sequence and group
     bool there;    // whether the table has a page of the cache there
@@ -639,11 +639,15 @@ __global__ void __launch_bounds__(256) kv_q4_append_groups_kernel(Q4Batch a, con
     else work(std::false_type{});
 }
 
-// 8 fp16 values (4 dwords) as values of type T to element i on.
-template <int T>
+// 8 fp16 values (4 dwords) as values of type T to element i on. LINES: the wave
+// stores whole rows, around the caches; pieces of 64 bytes (K) go through L2,
+// which joins them (8 x 32768 rows of 64 to fp16: 148 us; all around the caches
+// 165, all through them 154).
+template <int T, bool LINES>
 __device__ __forceinline__ void store8_half(void* p, int64_t i, bool wide, u32x4 w) {
     if (T == MIVI_GGML_F16 && wide) {
-        __builtin_nontemporal_store(w, (u32x4*)((uint16_t*)p + i));
+        if (LINES) __builtin_nontemporal_store(w, (u32x4*)((uint16_t*)p + i));
+        else *(u32x4*)((uint16_t*)p + i) = w;
         return;
     }
     float x[8];
@@ -691,7 +695,7 @@ __global__ void __launch_bounds__(256) kv_q4_read_groups_kernel(Q4Batch a, void*
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int half = 0; half < 2; half++)
-                    if (in[half]) store8_half<T>(k, base + h * k_head + half * 16 * k_row + b * 32, wide_k, out[2 * b + half]);
+                    if (in[half]) store8_half<T, false>(k, base + h * k_head + half * 16 * k_row + b * 32, wide_k, out[2 * b + half]);
         }
     } else {
         _Float16* own = tile[wave >> 1];
@@ -716,7 +720,7 @@ __global__ void __launch_bounds__(256) kv_q4_read_groups_kernel(Q4Batch a, void*
                 const int piece = i * 64 + lane, t = piece / (4 * NB), d = piece % (4 * NB) * 8;
                 const u32x2 lo = *(const u32x2*)(own + t * kRow + d), hi = *(const u32x2*)(own + t * kRow + d + 4);
                 if (t >= u.t0 && t < u.t1)
-                    store8_half<T>(v, (u.row0 + t) * v_row + h * v_head + d, wide_v, u32x4{lo[0], lo[1], hi[0], hi[1]});
+                    store8_half<T, true>(v, (u.row0 + t) * v_row + h * v_head + d, wide_v, u32x4{lo[0], lo[1], hi[0], hi[1]});
             }
             wave_sync();
         }
@@ -1099,7 +1103,7 @@ __device__ __forceinline__ bool head_place(const Q4Attn& a, int lane, int shares
 // scores, and page ids two groups ahead of that.
 //
 // Bound: about 200 (hd 64, two planes) to 290 (hd 128, one) vector instructions
-// a group, half of them codes to values, 60 % of the cycles; the loads alone take
+// a group, half of them codes to values, 73 and 62 % of the cycles; the loads alone take
 // 28 us where the kernel takes 41 (8 sequences of 32768 tokens, 8 heads of 64,
 // f32: 151 MB, 3.6 TB/s). 64 ragged sequences of up to 8192, 8 heads of 128, bf16:
 // 71 us, 297 MB, 4.2 TB/s. No faster: the next group's scores formed beside this

@@ -260,7 +260,8 @@ size_t mivi_hip_kv_q4_attention_workspace(size_t n_seq, size_t rows, size_t max_
 /* out = softmax(scale q K^T) V for every row and head over the cache, which
  * holds the rows' own tokens already: a row at position p sees the positions
  * 0 .. p, or with window > 0 the last `window` of them; query head j reads kv
- * head j / (n_heads / n_kv_heads). A row that sees nothing is zero. max_rows:
+ * head j / (n_heads / n_kv_heads). What no row sees need never have been
+ * written. A row that sees nothing is zero. max_rows:
  * at least the rows of any one sequence; a sequence's rows past it are not
  * computed. F32 queries and softmax weights enter the products as two fp16
  * planes (22 bits), F16 and BF16 ones as one (queries exactly, weights to 11

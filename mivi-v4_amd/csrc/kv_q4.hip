@@ -813,11 +813,11 @@ __device__ __forceinline__ void tile_groups(const Q4Seen& see, int i0, int i1, i
 }
 
 // A V scale pair j (of 4) of the lane's quarter in a group at t0, without the
-// tokens from `valid` on: what lies behind the sequence's end is anything, and
-// 0 * NaN is NaN.
-__device__ __forceinline__ uint32_t keep_mask(int t0, int quarter, int j, int valid) {
+// tokens before `from` and from `valid` on: what lies before the first row's
+// window or behind the last row is anything, and 0 * NaN is NaN.
+__device__ __forceinline__ uint32_t keep_mask(int t0, int quarter, int j, int from, int valid) {
     const int t = t0 + j / 2 * 16 + quarter * 4 + j % 2 * 2;
-    return (t < valid ? 0xFFFFu : 0u) | (t + 1 < valid ? 0xFFFF0000u : 0u);
+    return (t >= from && t < valid ? 0xFFFFu : 0u) | (t + 1 >= from && t + 1 < valid ? 0xFFFF0000u : 0u);
 }
 
 // A row's reference exponent follows its largest score only when that is more
@@ -924,17 +924,18 @@ __device__ __forceinline__ half8 ones8() {
 
 // What a workgroup knows of its sequence's rows.
 struct Q4Rows {
-    int start, valid, pairs;
+    int start, pairs;
+    int from, valid;  // positions that may be seen by a row
     Q4Seen see;
 };
 __device__ __forceinline__ bool rows_of(const Q4Attn& a, int s, Q4Rows* r) {
     const int start = a.b.starts[s], len = a.b.lens[s];
     const int64_t count = (int64_t)a.b.starts[s + 1] - start;
     r->start = start;
-    // rows times heads fits 31 bits
-    r->pairs = start < 0 || start >= a.rows ? 0 : (int)min<int64_t>(count, min(a.max_rows, a.rows - start)) * a.gq;
+    const int n = start < 0 || start >= a.rows ? 0 : (int)min<int64_t>(count, min(a.max_rows, a.rows - start));
+    r->pairs = n * a.gq;  // rows times heads fits 31 bits
     r->see = Q4Seen{(int)max<int64_t>(len - count, INT32_MIN), a.b.cap, a.window};
-    r->valid = min(max(len, 0), a.b.cap);
+    r->from = r->see.lo(0), r->valid = r->see.hi(n - 1);
     return r->pairs > 0;
 }
 
@@ -1165,10 +1166,10 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
         if (!gp || t0 < lo_all || t0 + kGroup > hi_all) {  // some row sees only a part
             t.hide(st, gp ? t0 : -1 - kGroup, quarter);
             const int valid = gp ? r.valid : 0;
-            if (t0 + kGroup > valid) {
+            if (t0 < r.from || t0 + kGroup > valid) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const uint32_t keep = keep_mask(t0, quarter, j, valid);
+                    const uint32_t keep = keep_mask(t0, quarter, j, r.from, valid);
 #pragma unroll
                     for (int b = 0; b < NB; b++) vs[4 * b + j] &= keep;
                 }
@@ -1301,10 +1302,10 @@ __global__ void __launch_bounds__(64 * NW) kv_q4_rows_kernel(Q4Attn a, int share
             constexpr int b = decltype(first)::value, n = decltype(count)::value;
             if (is_v) {
                 const int t0 = (g + mine) * kGroup;
-                if (t0 + kGroup > r.valid) {
+                if (t0 < r.from || t0 + kGroup > r.valid) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const uint32_t keep = keep_mask(t0, quarter, j, r.valid);
+                        const uint32_t keep = keep_mask(t0, quarter, j, r.from, r.valid);
 #pragma unroll
                         for (int e = 0; e < n; e++) sc[i][4 * e + j] &= keep;
                     }

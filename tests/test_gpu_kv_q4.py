@@ -401,6 +401,30 @@ def test_attention_pages_that_are_missing(hip, rows):
         assert (out[i].cpu().double() - want).abs().max() < 1e-5  # sums of 200 terms of order one in f32
 
 
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv,hd", [(4, 2, 64), (8, 1, 128), (2, 1, 256)])
+@pytest.mark.parametrize("rows", [[1, 2], [20, 3], [150, 40]])
+def test_attention_positions_before_every_window(hip, name, heads, kv, hd, rows):
+    """What no row's window reaches may never have been written (NaN scales here),
+    also where it shares a group of 32 with what some row sees."""
+    dt, page, lens, window = TYPES[name], 64, [307, 117], 45
+    b = Batch(hip, rows, lens, kv, hd, page)
+    have = [min(n + window - 1, t) for n, t in zip(rows, lens)]  # positions that some row sees
+    g = torch.Generator().manual_seed(11)
+    k, v = (torch.randn((sum(have), kv, hd), generator=g) for _ in range(2))
+    hip.kv_q4_append(b.cache, k.cuda(), v.cuda(), *Batch.tensors(have, lens))
+    kvs, at = [], 0
+    for n, t in zip(have, lens):
+        kvs.append([torch.cat([torch.zeros(kv, t - n, hd, dtype=torch.float64), held(x[at:at + n]).transpose(0, 1)], 1)
+                    for x in (k, v)])
+        at += n
+    q = torch.randn((sum(rows), heads, hd), generator=g).to(dt)
+    out = torch.empty_like(q, device="cuda")
+    hip.kv_q4_attention(out, q.cuda(), b.cache, b.starts_t, b.lens_t, max(rows), hd ** -0.5, window)
+    want, mag, top = reference(q, kvs, rows, lens, hd ** -0.5, window)
+    check_attention(out, want, mag, top, dt, hd, window)
+
+
 @pytest.mark.parametrize("rows", [[1, 1, 1], [40, 1, 20]])
 def test_attention_lengths_past_the_table_and_rows_past_the_limit(hip, rows):
     heads, kv, hd, page = 4, 2, 64, 32

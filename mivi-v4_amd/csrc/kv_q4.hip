@@ -1657,8 +1657,9 @@ Q4Plan attn_plan(size_t n_seq, size_t max_rows, size_t gq, size_t n_kv, size_t h
         return p;
     }
     // Tiles by themselves, their groups in shares where that fills the card
-    // better: the rounds that the workgroups take, one to three a CU, times a share's groups at about 1.1 us, against the join's 10 us and
-    // its traffic, twice the parts at 4 TB/s.
+    // better: the rounds that the workgroups take, one to three a CU, times a
+    // share's groups at about 1.1 us, against the join's 10 us and its traffic,
+    // twice the parts at 4 TB/s.
     if (__builtin_mul_overflow(heads, p.tiles, &wgs)) wgs = SIZE_MAX;
     const size_t slots = cus * (p.form == Q4Plan::kFew ? 3 : p.form == Q4Plan::kMid ? 2 : 1);
     double best = 0;

@@ -1570,7 +1570,7 @@ int32_t make_batch(Q4Batch* b, const uint8_t* cache, size_t cache_len, size_t n_
         return err_overflow();
     if (n_seq > 1 && pages_stride < pages_per_seq)
         return set_error(MIVI_ERR_INVALID_ARGUMENT, "pages_stride %zu < pages_per_seq %zu", pages_stride, pages_per_seq);
-    if (!cache || (pages_per_seq && !pages) || !starts || !lens)
+    if (!cache || !starts || (n_seq && (!lens || (pages_per_seq && !pages))))
         return set_error(MIVI_ERR_INVALID_ARGUMENT, "null argument");
     if ((uintptr_t)cache % 16) return set_error(MIVI_ERR_INVALID_ARGUMENT, "cache not 16-byte aligned");
     if ((uintptr_t)pages % 4 || (uintptr_t)starts % 4 || (uintptr_t)lens % 4)

@@ -726,3 +726,17 @@ def test_python_refusals(hip):
         hip.kv_q4_read(b.cache, x.expand(3, 2, 64), x.expand(3, 2, 64), b.starts_t, b.lens_t)
     assert hip.kv_q4_attention(torch.empty((0, 4, 64), device="cuda"), torch.empty((0, 4, 64), device="cuda"), b.cache,
                                b.starts_t, b.lens_t).shape[0] == 0
+
+
+def test_a_batch_of_no_sequences(hip):
+    b = Batch(hip, [1], [10], 2, 64, 32)
+    b.cache.set_pages(torch.empty((0, 4), dtype=torch.int32, device="cuda"))
+    starts, lens = Batch.tensors([], [])
+    for rows in (0, 3):  # rows of no sequence are left alone
+        x = torch.full((rows, 2, 64), 5.0, device="cuda")
+        before = b.data.clone()
+        hip.kv_q4_append(b.cache, x, x, starts, lens)
+        hip.kv_q4_read(b.cache, x, torch.empty_like(x), starts, lens)
+        out = torch.full((rows, 4, 64), 5.0, device="cuda")
+        hip.kv_q4_attention(out, torch.zeros_like(out), b.cache, starts, lens)
+        assert torch.equal(b.data, before) and (x == 5).all() and (out == 5).all()

@@ -111,6 +111,12 @@ def test_nothing_to_do_is_ok():
     assert attn(max_rows=0) == 0
 
 
+@pytest.mark.parametrize("call", CALLS)
+def test_no_sequences_need_no_table(call):
+    assert call(geo=geometry(nseq=0, pages=None, lens=None)) == 0  # what an empty tensor's address is
+    assert call(geo=geometry(nseq=0, starts=None)) == 101
+
+
 def test_workspace_grows_with_the_batch():
     f = LIB.mivi_hip_kv_q4_attention_workspace
     assert f(0, 7, 7, 4, 2, 64, 256, 0) == 0 and f(1, 0, 0, 4, 2, 64, 256, 0) == 0

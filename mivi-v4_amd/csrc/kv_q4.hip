@@ -820,10 +820,16 @@ __device__ __forceinline__ uint32_t keep_mask(int t0, int quarter, int j, int fr
     return (t >= from && t < valid ? 0xFFFFu : 0u) | (t + 1 >= from && t + 1 < valid ? 0xFFFF0000u : 0u);
 }
 
-// A row's reference exponent follows its largest score only when that is more
-// than kSlack above it: weights are held times 2^kPShift and reach 2^15; fp16
-// then resolves 2^-36 of the largest.
-constexpr float kPShift = 11, kSlack = 4;
+// A weight is 2^(y - m), y = st sc as an fp32 number. A row's reference m moves
+// only when some y is more than kReach above it, and then lies kPShift below the
+// largest: no weight passes 2^15, and fp16 resolves 2^-36 of the largest. From
+// kFar on m is the largest y itself: kPShift less would round, by 16 at 2^27, and
+// weights of infinity or of zero alone would come of it. For the same reason the
+// exponent is formed from y, as m was, in two roundings: in one fma the product's
+// own rounding, 8 at 2^27, would stand between them. (The second instruction is
+// 1 to 2 % of a prompt's time, nothing of a single token's.)
+constexpr float kPShift = 11, kReach = 15, kFar = 1 << 20;
+constexpr float kUnseen = -3.402823466e38f;  // m of a row that has seen nothing
 
 // 16 (row, query head) pairs as the columns of the products; lane l works on
 // column l mod 16.
@@ -831,7 +837,7 @@ template <int NB, int P>
 struct Q4Tile {
     half8 q[P][NB];      // B operands: block b, dimensions 8 quarter .. + 7
     float sc;            // a raw score times sc is the exponent to base 2
-    float m, nm;         // reference exponent; kPShift - m, the exponents' offset
+    float m;             // reference exponent
     f32x4 acc[2 * NB];   // sums of w V: dimensions 16 j + 4 quarter + i
     f32x4 l;             // sums of w, the same in all four
     int lo, hi;          // positions seen
@@ -868,7 +874,7 @@ struct Q4Tile {
         // positive, so that the largest score has the largest exponent and a
         // hidden one's -inf stays that
         sc = fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -ex), 1.17549435e-38f);
-        m = -__builtin_inff(), nm = kPShift;
+        m = kUnseen;
         l = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < 2 * NB; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -878,22 +884,23 @@ struct Q4Tile {
     // B operands of the sums. The maximum over the quarters is formed only when
     // some lane has a score so much larger than its row's reference.
     __device__ __forceinline__ void weigh(const f32x4 (&st)[2], half8 (&w)[P]) {
-        float mx = st[0][0];
+        float y[8];
 #pragma unroll
-        for (int i = 1; i < 8; i++) mx = fmaxf(mx, st[i / 4][i % 4]);
-        if (__any(mx * sc > m + kSlack)) {
-            const float m_new = fmaxf(m, quarters_max(mx) * sc);
+        for (int i = 0; i < 8; i++) y[i] = st[i / 4][i % 4] * sc;
+        float mx = y[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) mx = fmaxf(mx, y[i]);
+        if (__any(mx - m > kReach)) {  // m + kReach would round
+            const float most = quarters_max(mx), m_new = fmaxf(m, most - (fabsf(most) < kFar ? kPShift : 0.f));
             const float f = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
             m = m_new;
-            nm = kPShift - (m == -__builtin_inff() ? 0.f : m);
             l *= f;
 #pragma unroll
             for (int j = 0; j < 2 * NB; j++) acc[j] *= f;
         }
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-            const f32x2 x = {__builtin_amdgcn_exp2f(fmaf(st[i / 4][i % 4], sc, nm)),
-                             __builtin_amdgcn_exp2f(fmaf(st[i / 4][i % 4 + 1], sc, nm))};
+            const f32x2 x = {__builtin_amdgcn_exp2f(y[i] - m), __builtin_amdgcn_exp2f(y[i + 1] - m)};
             const half2v top = __builtin_convertvector(x, half2v);
             w[0][i] = top.x, w[0][i + 1] = top.y;
             if constexpr (P == 2) {  // x - top, exact, in one instruction each
@@ -1202,14 +1209,13 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
     for (int u = threadIdx.x; u < 16 * kQuads; u += 256) {
         const int f = u / kQuads, d4 = u % kQuads * 4;
         if (f >= r.pairs) continue;
-        float m = -__builtin_inff();  // never NaN: a NaN score is in the sums alone
+        float m = kUnseen;  // never NaN: a NaN score is in the sums alone
 #pragma unroll
         for (int w = 0; w < NW; w++) m = fmaxf(m, red_ml[w][f][0]);
-        const float m_ref = m == -__builtin_inff() ? 0.f : m;
         float l = 0.f, o[4] = {};
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float e = __builtin_amdgcn_exp2f(red_ml[w][f][0] - m_ref);
+            const float e = __builtin_amdgcn_exp2f(red_ml[w][f][0] - m);
             l = fmaf(e, red_ml[w][f][1], l);
             const f32x4 x = *(const f32x4*)&red_acc[w][f][d4];
 #pragma unroll
@@ -1471,14 +1477,14 @@ __global__ void __launch_bounds__(256) kv_q4_join_kernel(Q4Attn a, int shares) {
 #pragma unroll
         for (int c = 0; c < 8; c++) x[c] = *(const f32x4*)(pa + (int64_t)min(j + c * per + first, n - 1) * hd);
     };
-    float m_i = -__builtin_inff(), l_i = 0.f;
+    float m_i = kUnseen, l_i = 0.f;
     if (n) {
         if (lane < n) m_i = ml[2 * lane], l_i = ml[2 * lane + 1];
         fetch(0);
     }
     float o[4] = {};
     const float m = xmax_all64(m_i);
-    const float e_i = __builtin_amdgcn_exp2f(m_i - (m == -__builtin_inff() ? 0.f : m));  // 0 from part n on
+    const float e_i = __builtin_amdgcn_exp2f(m_i - m);  // used up to part n
     const float l = xsum_all64(e_i * l_i);
     for (int j = 0; j < n; j += 8 * per) {
         if (j) fetch(j);

@@ -1,0 +1,84 @@
+"""Attention over the 4-bit cache at the ends of what its arguments can hold:
+scores far past fp32's integers, scales next to the largest float, values at
+the cache's limit; and how near 16-bit outputs come to their own rounding."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_kv_q4 import TYPES, Batch, check_attention, held, reference
+
+pytestmark = pytest.mark.gpu
+
+
+def check_hull(got, q, kvs, rows, lens, scale, dtype, longest):
+    """For scores whose f32 rounding is larger than one: softmax weighs a row's
+    tokens by scores that are off by at most e = sum |q k| scale * ((hd + 8)
+    2^-24 and 2^-22 for f32 queries in two planes), so that a token more than
+    2 e + 40 below the largest has less than e^-40 of its weight, which fp16
+    weights hold as zero, and the output lies between the least and the largest
+    value of the tokens that are left, up to the f32 sums (one in four of the
+    tokens and 64 more roundings) and half a step of the type. With one token
+    left this is its value."""
+    q = q.double().cpu()
+    hd = q.shape[-1]
+    assert torch.isfinite(got).all()
+    got = got.double().cpu()
+    at, alone = 0, 0
+    for (k, v), n, t in zip(kvs, rows, lens):
+        g = q.shape[1] // k.shape[0]
+        for i in range(n):
+            kk, vv = (x[:, :t - n + i + 1].repeat_interleave(g, 0) for x in (k, v))
+            s = (kk @ q[at + i][:, :, None])[..., 0] * scale
+            top = (kk.abs() @ q[at + i].abs()[:, :, None])[..., 0].amax(-1, keepdim=True) * abs(scale)
+            e = top * ((hd + 8) * 2.0 ** -24 + (2.0 ** -22 if dtype == torch.float32 else 0.0))
+            left = s >= s.amax(-1, keepdim=True) - 2 * e - 40
+            alone += (left.sum(-1) == 1).sum().item()
+            lo = torch.where(left[..., None], vv, math.inf).amin(1)
+            hi = torch.where(left[..., None], vv, -math.inf).amax(1)
+            room = (torch.maximum(lo.abs(), hi.abs()) * ((longest / 4 + 64) * 2.0 ** -24 + torch.finfo(dtype).eps / 2)
+                    + torch.finfo(dtype).tiny)
+            assert (got[at + i] >= lo - room).all() and (got[at + i] <= hi + room).all()
+        at += n
+    return alone
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40])
+@pytest.mark.parametrize("cap", [600, 4096])   # one part, and shares with a join
+@pytest.mark.parametrize("name,by,kscale", [
+    ("f32", 3e7, 1.0), ("f32", 1e9, 1.0), ("f32", 1e20, 1.0), ("f32", 1e36, 1.0),
+    ("bf16", 1e8, 1.0), ("bf16", 1e36, 1.0), ("f16", 1.5e4, 2e4),
+])
+def test_attention_of_scores_past_the_integers_of_fp32(hip, name, by, kscale, cap, rows):
+    """Finite queries give finite outputs, of the tokens with the largest scores."""
+    dt = TYPES[name]
+    heads, kv, hd = 8, 2, 64
+    b = Batch(hip, [rows], [600], kv, hd, 64, cap=cap)
+    kvs = b.fill(hip, scale=kscale)
+    q = (torch.randn((rows, heads, hd), generator=torch.Generator().manual_seed(4)) * by).clamp(-3e38, 3e38)
+    q = (q.clamp(-65504, 65504) if dt == torch.float16 else q).to(dt)
+    out = torch.empty((rows, heads, hd), dtype=dt, device="cuda")
+    for scale in (hd ** -0.5, -0.125):
+        hip.kv_q4_attention(out, q.cuda(), b.cache, b.starts_t, b.lens_t, rows, scale)
+        alone = check_hull(out, q, kvs, [rows], [600], scale, dt, 600)
+        assert alone > rows * heads / 2  # most rows have one token only
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_of_large_scores_leaves_the_other_rows_alone(hip, rows):
+    """Rows beside one of very large scores are as exact as ever."""
+    heads, kv, hd = 8, 2, 64
+    b = Batch(hip, [rows], [600], kv, hd, 64)
+    kvs = b.fill(hip)
+    q = torch.randn((rows, heads, hd), generator=torch.Generator().manual_seed(4))
+    far = q.clone()
+    far[0, 1] *= 1e9
+    out = torch.empty(q.shape, device="cuda")
+    hip.kv_q4_attention(out, far.cuda(), b.cache, b.starts_t, b.lens_t)
+    assert torch.isfinite(out).all()
+    want, mag, top = reference(q, kvs, [rows], [600], hd ** -0.5)
+    out[0, 1] = want[0, 1].float()
+    check_attention(out, want, mag, top, torch.float32, hd, 600)

@@ -268,7 +268,9 @@ size_t mivi_hip_kv_q4_attention_workspace(size_t n_seq, size_t rows, size_t max_
  * computed. F32 queries and softmax weights enter the products as two fp16
  * planes (22 bits), F16 and BF16 ones as one (queries exactly, weights to 11
  * bits); a weight below 2^-25 of its row's largest to 2^-36 of that; sums are
- * f32. An infinity or NaN in q stays in its row and head.
+ * f32. Finite q and scale give finite outputs, the weights being those of the
+ * scores as f32 products give them, however large. An infinity or NaN in q
+ * stays in its row and head.
  * `workspace`: 16-byte aligned, mivi_hip_kv_q4_attention_workspace bytes for
  * the call's arguments, in use until the call's work is done; calls that may
  * overlap need workspaces of their own. */

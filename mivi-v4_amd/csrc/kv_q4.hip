@@ -872,8 +872,13 @@ struct Q4Tile {
             }
         }
         // positive, so that the largest score has the largest exponent and a
-        // hidden one's -inf stays that
-        sc = fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -ex), 1.17549435e-38f);
+        // hidden one's -inf stays that; no more than 2^89, so that no exponent is
+        // infinite (raw scores are below 2^38: 256 products of 2^15 and 21760).
+        // Raw scores that differ do so by 2^-48 at least, fp16's smallest step
+        // squared: past 2^89 the largest has all the weight either way. The scale
+        // is brought into range first: log2(e) times it may have no number.
+        sc = ldexpf(fabsf(a.scale), -ex) * 1.44269504088896340736f;
+        sc = fminf(fmaxf(sc, 1.17549435e-38f), 0x1p89f);
         m = kUnseen;
         l = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll

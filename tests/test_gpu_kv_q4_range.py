@@ -82,3 +82,21 @@ def test_attention_of_large_scores_leaves_the_other_rows_alone(hip, rows):
     want, mag, top = reference(q, kvs, [rows], [600], hd ** -0.5)
     out[0, 1] = want[0, 1].float()
     check_attention(out, want, mag, top, torch.float32, hd, 600)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("scale,by", [(3.4e38, 1e-38), (3.4e38, 1e-39), (-3e38, 2e-38), (2.5e38, 1e-20), (3.4e38, 1.0),
+                                      (1e30, 1e30), (3.4e38, 0.0)])
+def test_attention_of_scales_next_to_the_largest_float(hip, rows, scale, by):
+    """scale log2(e) passes the largest float, and scale q k does."""
+    heads, kv, hd = 4, 2, 64
+    b = Batch(hip, [rows], [100], kv, hd, 64)
+    kvs = b.fill(hip)
+    q = (torch.randn((rows, heads, hd), generator=torch.Generator().manual_seed(4)) * by).clamp(-3e38, 3e38)
+    out = torch.empty((rows, heads, hd), device="cuda")
+    hip.kv_q4_attention(out, q.cuda(), b.cache, b.starts_t, b.lens_t, rows, scale)
+    if abs(scale) * by < 100:
+        want, mag, top = reference(q, kvs, [rows], [100], float(np.float32(scale)))
+        check_attention(out, want, mag, top, torch.float32, hd, 100)
+    else:
+        check_hull(out, q, kvs, [rows], [100], float(np.float32(scale)), torch.float32, 100)

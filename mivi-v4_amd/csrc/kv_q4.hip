@@ -832,10 +832,10 @@ constexpr float kPShift = 11, kReach = 15, kFar = 1 << 20;
 constexpr float kUnseen = -3.402823466e38f;  // m of a row that has seen nothing
 
 // 16 (row, query head) pairs as the columns of the products; lane l works on
-// column l mod 16.
-template <int NB, int P>
+// column l mod 16. PQ, PW: fp16 planes of the queries and of the weights.
+template <int NB, int PQ, int PW>
 struct Q4Tile {
-    half8 q[P][NB];      // B operands: block b, dimensions 8 quarter .. + 7
+    half8 q[PQ][NB];     // B operands: block b, dimensions 8 quarter .. + 7
     float sc;            // a raw score times sc is the exponent to base 2
     float m;             // reference exponent
     f32x4 acc[2 * NB];   // sums of w V: dimensions 16 j + 4 quarter + i
@@ -868,7 +868,7 @@ struct Q4Tile {
                 const float y = ldexpf(x[b][e], ex) * sign;
                 const _Float16 top = (_Float16)y;
                 q[0][b][e] = top;
-                if constexpr (P == 2) q[1][b][e] = (_Float16)(y - (float)top);
+                if constexpr (PQ == 2) q[1][b][e] = (_Float16)(y - (float)top);
             }
         }
         // positive, so that the largest score has the largest exponent and a
@@ -888,7 +888,7 @@ struct Q4Tile {
     // The scores of a group (tokens 4 quarter + i of each half) to weights, the
     // B operands of the sums. The maximum over the quarters is formed only when
     // some lane has a score so much larger than its row's reference.
-    __device__ __forceinline__ void weigh(const f32x4 (&st)[2], half8 (&w)[P]) {
+    __device__ __forceinline__ void weigh(const f32x4 (&st)[2], half8 (&w)[PW]) {
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) y[i] = st[i / 4][i % 4] * sc;
@@ -908,7 +908,7 @@ struct Q4Tile {
             const f32x2 x = {__builtin_amdgcn_exp2f(y[i] - m), __builtin_amdgcn_exp2f(y[i + 1] - m)};
             const half2v top = __builtin_convertvector(x, half2v);
             w[0][i] = top.x, w[0][i + 1] = top.y;
-            if constexpr (P == 2) {  // x - top, exact, in one instruction each
+            if constexpr (PW == 2) {  // x - top, exact, in one instruction each
                 const f32x2 rest = {fmaf((float)top.x, -1.f, x.x), fmaf((float)top.y, -1.f, x.y)};
                 const half2v low = __builtin_convertvector(rest, half2v);
                 w[1][i] = low.x, w[1][i + 1] = low.y;
@@ -1109,11 +1109,17 @@ __device__ __forceinline__ bool head_place(const Q4Attn& a, int lane, int shares
 // Up to 16 pairs of a sequence and kv head: a workgroup takes a range of their
 // groups, each of its four waves every fourth one straight from memory to
 // operands, and joins the waves at the end. One pass with the running maximum
-// and sum of the softmax. P: the fp16 planes of the query rows and of the
-// weights (2 for f32 values, 22 bits in all; 1 for fp16 and bf16 values, whose
-// queries fp16 holds exactly and whose outputs have no more bits than the
-// weights). K of the next group is on its way during the sums, V during the
-// scores, and page ids two groups ahead of that.
+// and sum of the softmax. Planes: two hold 22 bits of a value, one 11. Queries
+// of 16 bits need one (bf16 has 8 bits, and past 2^-28 of a row's largest what
+// fp16 lacks is 2^-39 of that). Weights rounded to 11 bits put an error of about
+// 2^-12 of sum w |v| / sqrt(tokens) on an output: beside an fp16 output's own
+// rounding that is 1.1 to 1.5 times its rms error, so fp16 takes two (64 ragged
+// sequences of up to 8192, 8 heads of 128: 76 -> 84 us, prompts of 32768 2.26 ->
+// 2.88 ms; the rms error is then the rounding's); beside a bf16 output's it is 1 %
+// at most, so bf16 takes one.
+//
+// K of the next group is on its way during the sums, V during the scores, and
+// page ids two groups ahead of that.
 //
 // Bound: about 200 (hd 64, two planes) to 290 (hd 128, one) vector instructions
 // a group, half of them codes to values, 73 and 62 % of the cycles; the loads alone take
@@ -1124,13 +1130,15 @@ __device__ __forceinline__ bool head_place(const Q4Attn& a, int lane, int shares
 // columns (fewer exponentials, two waves a SIMD: 41).
 //
 // Waves a SIMD that the registers are held to: 17 nb words of codes, scales and
-// sums and 4 nb a plane of queries beside about 40 others.
-constexpr int step_waves(int nb, int p) {
-    const int words = nb * (17 + 4 * p);
+// sums and 4 nb a plane of queries beside about 40 others; 4 where the weights
+// have a plane more (64 ragged fp16 sequences, 8 heads of 128: three waves 84 us,
+// four with spills 88).
+constexpr int step_waves(int nb, int pq, int pw) {
+    const int words = nb * (17 + 4 * pq) + 4 * (pw - pq);
     return words <= 84 ? 4 : words <= 102 ? 3 : 2;
 }
-template <int NB, int P>
-__global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4Attn a, int shares) {
+template <int NB, int PQ, int PW>
+__global__ void __launch_bounds__(256, step_waves(NB, PQ, PW)) kv_q4_step_kernel(Q4Attn a, int shares) {
     constexpr int hd = 32 * NB, NW = 4;
     __shared__ float red_ml[NW][16][2];
     __shared__ float red_acc[NW][16][hd + 4];
@@ -1142,7 +1150,7 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
     const int lo_all = r.see.lo(row_of(a, r.pairs - 1)), hi_all = r.see.hi(0);  // seen by every row: lo_all .. hi_all - 1
     const Q4Groups groups(a, pl.s, pl.h, pl.g_end);
     const Q4Bits bits;
-    Q4Tile<NB, P> t;
+    Q4Tile<NB, PQ, PW> t;
     uint32_t k[2 * NB], ks[NB], v[2 * NB], vs[4 * NB];
     int g = pl.g_begin + wave;
     const uint8_t *gp = nullptr, *next = nullptr;
@@ -1170,7 +1178,7 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
             for (int half = 0; half < 2; half++) {
                 const half8 kk = held_k(bits, k[2 * b + half], k_scale<NB>(ks, half, b));
 #pragma unroll
-                for (int p = 0; p < P; p++) st[half] = mfma16(kk, t.q[p][b], st[half]);
+                for (int p = 0; p < PQ; p++) st[half] = mfma16(kk, t.q[p][b], st[half]);
             }
         }
         load_k<NB>(from, lane, k, ks);
@@ -1187,10 +1195,10 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
                 }
             }
         }
-        half8 w[P];
+        half8 w[PW];
         t.weigh(st, w);
 #pragma unroll
-        for (int p = 0; p < P; p++) t.l = mfma16(ones8(), w[p], t.l);
+        for (int p = 0; p < PW; p++) t.l = mfma16(ones8(), w[p], t.l);
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             half8 vv[2];
@@ -1198,7 +1206,7 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
 #pragma unroll
             for (int z = 0; z < 2; z++) {
 #pragma unroll
-                for (int p = 0; p < P; p++) t.acc[2 * b + z] = mfma16(vv[z], w[p], t.acc[2 * b + z]);
+                for (int p = 0; p < PW; p++) t.acc[2 * b + z] = mfma16(vv[z], w[p], t.acc[2 * b + z]);
             }
         }
         load_v<NB>(from, lane, v, vs);
@@ -1243,7 +1251,7 @@ __global__ void __launch_bounds__(256, step_waves(NB, P)) kv_q4_step_kernel(Q4At
 // 2.48 ms. 2048 f32 rows at 4096, heads of 64: 132 us, the planes doubling both
 // products. 16 x 5 bf16 rows at up to 12000 tokens, 4 heads of 128 (NT 1): 36 us,
 // the chain of barrier, scores, weights and sums of one tile a wave.
-template <int NB, int P, int NT, int NW, int TG>
+template <int NB, int PQ, int PW, int NT, int NW, int TG>
 __global__ void __launch_bounds__(64 * NW) kv_q4_rows_kernel(Q4Attn a, int shares) {
     constexpr int kPer = NW / 2 / TG;                             // waves of a group, K or V
     constexpr int kBlocks = ((NB + 1) / 2 + kPer - 1) / kPer * 2;  // blocks of one of them, an even number
@@ -1349,7 +1357,7 @@ __global__ void __launch_bounds__(64 * NW) kv_q4_rows_kernel(Q4Attn a, int share
         fetch(g_begin, s0);
         fetch(g_begin + TG, s1);
     }
-    Q4Tile<NB, P> t[NT];
+    Q4Tile<NB, PQ, PW> t[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) t[n].init(a, r.see, r.start, pl.h, f_wave + 16 * n + col, r.pairs, quarter);
     if (g_begin < g_end) {
@@ -1381,7 +1389,7 @@ __global__ void __launch_bounds__(64 * NW) kv_q4_rows_kernel(Q4Attn a, int share
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
 #pragma unroll
-                        for (int p = 0; p < P; p++) st[n][half] = mfma16(k, t[n].q[p][b], st[n][half]);
+                        for (int p = 0; p < PQ; p++) st[n][half] = mfma16(k, t[n].q[p][b], st[n][half]);
                     }
                 }
             }
@@ -1389,12 +1397,12 @@ __global__ void __launch_bounds__(64 * NW) kv_q4_rows_kernel(Q4Attn a, int share
 #pragma unroll
                 for (int n = 0; n < NT; n++) t[n].hide(st[n], t0, quarter);
             }
-            half8 w[NT][P];
+            half8 w[NT][PW];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 t[n].weigh(st[n], w[n]);
 #pragma unroll
-                for (int p = 0; p < P; p++) t[n].l = mfma16(ones8(), w[n][p], t[n].l);
+                for (int p = 0; p < PW; p++) t[n].l = mfma16(ones8(), w[n][p], t[n].l);
             }
 #pragma unroll
             for (int j = 0; j < 2 * NB; j++) {
@@ -1402,7 +1410,7 @@ __global__ void __launch_bounds__(64 * NW) kv_q4_rows_kernel(Q4Attn a, int share
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
-                    for (int p = 0; p < P; p++) t[n].acc[j] = mfma16(v, w[n][p], t[n].acc[j]);
+                    for (int p = 0; p < PW; p++) t[n].acc[j] = mfma16(v, w[n][p], t[n].acc[j]);
                 }
             }
         }
@@ -1685,34 +1693,35 @@ Q4Plan attn_plan(size_t n_seq, size_t max_rows, size_t gq, size_t n_kv, size_t h
     return p;
 }
 
-template <int NB, int P>
+template <int NB, int PQ, int PW>
 void launch_attn(const Q4Attn& a, const Q4Plan& p, hipStream_t s) {
     const unsigned grid = (unsigned)p.grid;
     const int shares = (int)p.shares;
     if (p.form == Q4Plan::kStep) {
-        kv_q4_step_kernel<NB, P><<<grid, 256, 0, s>>>(a, shares);
+        kv_q4_step_kernel<NB, PQ, PW><<<grid, 256, 0, s>>>(a, shares);
     } else if (p.form == Q4Plan::kFew) {
         // two groups a step at 64 dimensions (16 x 5 rows 44.7 -> 39.3 us); at 128
         // their LDS halves the workgroups of a CU (57 -> 63)
-        kv_q4_rows_kernel<NB, P, 1, 4, NB <= 2 ? 2 : 1><<<grid, 256, 0, s>>>(a, shares);
+        kv_q4_rows_kernel<NB, PQ, PW, 1, 4, NB <= 2 ? 2 : 1><<<grid, 256, 0, s>>>(a, shares);
     } else if constexpr (NB <= 3) {
-        kv_q4_rows_kernel<NB, P, 2, 4, 2><<<grid, 256, 0, s>>>(a, shares);
+        kv_q4_rows_kernel<NB, PQ, PW, 2, 4, 2><<<grid, 256, 0, s>>>(a, shares);
     } else if constexpr (NB == 4) {
-        if constexpr (P == 1) {
+        if constexpr (PQ == 1) {
             if (p.form == Q4Plan::kSome) {
-                kv_q4_rows_kernel<NB, P, 1, 8, 1><<<grid, 512, 0, s>>>(a, shares);
+                kv_q4_rows_kernel<NB, PQ, PW, 1, 8, 1><<<grid, 512, 0, s>>>(a, shares);
                 return;
             }
         }
-        kv_q4_rows_kernel<NB, P, 2, 8, 2><<<grid, 512, 0, s>>>(a, shares);
+        kv_q4_rows_kernel<NB, PQ, PW, 2, 8, 2><<<grid, 512, 0, s>>>(a, shares);
     } else {
-        kv_q4_rows_kernel<NB, P, 1, 8, 1><<<grid, 512, 0, s>>>(a, shares);
+        kv_q4_rows_kernel<NB, PQ, PW, 1, 8, 1><<<grid, 512, 0, s>>>(a, shares);
     }
 }
 template <int NB>
-void launch_attn(const Q4Attn& a, const Q4Plan& p, int planes, hipStream_t s) {
-    if (planes == 2) launch_attn<NB, 2>(a, p, s);
-    else launch_attn<NB, 1>(a, p, s);
+void launch_attn(const Q4Attn& a, const Q4Plan& p, hipStream_t s) {
+    if (a.type == MIVI_GGML_F32) launch_attn<NB, 2, 2>(a, p, s);
+    else if (a.type == MIVI_GGML_F16) launch_attn<NB, 1, 2>(a, p, s);
+    else launch_attn<NB, 1, 1>(a, p, s);
 }
 
 }  // namespace
@@ -1858,12 +1867,12 @@ extern "C" int32_t mivi_hip_kv_q4_attention(
     a.part_ml = a.part_acc + rows * n_heads * p.nsplit * head_dim;
     hipStream_t s = (hipStream_t)stream;
     switch (head_dim / 32) {
-        case 1: launch_attn<1>(a, p, planes, s); break;
-        case 2: launch_attn<2>(a, p, planes, s); break;
-        case 3: launch_attn<3>(a, p, planes, s); break;
-        case 4: launch_attn<4>(a, p, planes, s); break;
-        case 6: launch_attn<6>(a, p, planes, s); break;
-        default: launch_attn<8>(a, p, planes, s); break;
+        case 1: launch_attn<1>(a, p, s); break;
+        case 2: launch_attn<2>(a, p, s); break;
+        case 3: launch_attn<3>(a, p, s); break;
+        case 4: launch_attn<4>(a, p, s); break;
+        case 6: launch_attn<6>(a, p, s); break;
+        default: launch_attn<8>(a, p, s); break;
     }
     MIVI_HIP_CHECK(hipGetLastError());
     if (p.nsplit > 1) {

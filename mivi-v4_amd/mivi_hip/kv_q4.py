@@ -100,6 +100,14 @@ def _call(fn, args, device, stream):
         _check(rc)
 
 
+def _stream_of(stream, device):
+    """The torch stream of an object or a handle (0: the default stream, which
+    ExternalStream would take for a new one)."""
+    if not isinstance(stream, int):
+        return stream
+    return torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)
+
+
 def _kv(fn, cache, k, v, starts, lens, stream):
     if k.shape != v.shape:
         raise ValueError("k and v are of one shape")
@@ -149,7 +157,7 @@ def kv_q4_attention(out, q, cache: KvCacheQ4, starts, lens, max_rows: int | None
         if stream is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=device)
         else:  # from that stream's memory: reused only behind its work
-            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if isinstance(stream, int) else stream):
+            with torch.cuda.stream(_stream_of(stream, device)):
                 workspace = torch.empty(need, dtype=torch.uint8, device=device)
     if workspace is not None and (workspace.device != device or not workspace.is_contiguous()):
         raise ValueError("workspace is a contiguous tensor on the cache's device")

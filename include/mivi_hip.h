@@ -252,9 +252,9 @@ int32_t mivi_hip_kv_q4_read(const uint8_t* cache, size_t cache_len, size_t n_kv_
                             size_t v_row_stride, size_t v_head_stride, size_t rows, void* stream);
 
 /* Bytes of mivi_hip_kv_q4_attention's workspace for a call of these sizes,
- * max_tokens = pages_per_seq * page_tokens (0: none is needed). A smaller call
- * may need more, as its work is cut finer: a workspace for several calls has
- * the largest of theirs. */
+ * max_tokens = pages_per_seq * page_tokens (0: none is needed, or there is no
+ * such call). A smaller call may need more, as its work is cut finer: a
+ * workspace for several calls has the largest of theirs. */
 size_t mivi_hip_kv_q4_attention_workspace(size_t n_seq, size_t rows, size_t max_rows, size_t n_heads,
                                           size_t n_kv_heads, size_t head_dim, size_t max_tokens,
                                           size_t window);

@@ -1562,6 +1562,9 @@ int wide_ok(const void* p, size_t row_stride, size_t head_stride, size_t elem, s
     return (uintptr_t)p % bytes == 0 && row_stride * elem % bytes == 0 && head_stride * elem % bytes == 0;
 }
 
+// A launch counts the threads of a dimension in 32 bits.
+bool grid_fits(size_t groups, size_t threads) { return groups <= UINT32_MAX / threads; }
+
 int32_t check_geometry(size_t n_kv, size_t hd, size_t page_tokens) {
     if (hd % 32) return err_misaligned(hd, 32);
     if (!head_dim_ok(hd))
@@ -1629,6 +1632,7 @@ struct Q4Plan {
     // of 16), of 128 (eight of 16, four of 32), of 256 (eight of 32)
     enum { kStep, kFew, kSome, kMid, kMany } form;
     size_t tile_pairs, tiles, chunk, nsplit, shares, share_min, grid;
+    size_t threads() const { return form == kSome || form == kMany ? 512 : 256; }
 };
 
 Q4Plan attn_plan(size_t n_seq, size_t max_rows, size_t gq, size_t n_kv, size_t hd, int planes, size_t cap,
@@ -1747,12 +1751,12 @@ extern "C" int32_t mivi_hip_kv_q4_append(uint8_t* cache, size_t cache_len, size_
         (rc = check_tensor("v", v, v_len, type, rows, v_row_stride, n_kv_heads, v_head_stride, head_dim, false)))
         return rc;
     const size_t blocks = (rows * n_kv_heads * (head_dim / 8) + 255) / 256;
-    if (blocks > (size_t)INT32_MAX) return err_overflow();
+    const dim3 grid = group_grid(rows, n_seq, n_kv_heads);
+    if (!grid_fits(grid.x ? grid.x : blocks, 256)) return err_overflow();
     clear_error();
     const size_t e = type_bytes(type);
     const int wk = wide_ok(k, k_row_stride, k_head_stride, e, 16), wv = wide_ok(v, v_row_stride, v_head_stride, e, 16);
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid = group_grid(rows, n_seq, n_kv_heads);
 #define APPEND(T)                                                                                                    \
     if (grid.x)                                                                                                      \
         kv_q4_append_groups_kernel<T><<<grid, 256, 0, s>>>(b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride,   \
@@ -1786,12 +1790,12 @@ extern "C" int32_t mivi_hip_kv_q4_read(const uint8_t* cache, size_t cache_len, s
         (rc = check_tensor("v", v, v_len, type, rows, v_row_stride, n_kv_heads, v_head_stride, head_dim, true)))
         return rc;
     const size_t blocks = (rows * n_kv_heads * (head_dim / 8) + 255) / 256;
-    if (blocks > (size_t)INT32_MAX) return err_overflow();
+    const dim3 grid = group_grid(rows, n_seq, n_kv_heads);
+    if (!grid_fits(grid.x ? grid.x : blocks, 256)) return err_overflow();
     clear_error();
     const size_t e = type_bytes(type);
     const int wk = wide_ok(k, k_row_stride, k_head_stride, e, 16), wv = wide_ok(v, v_row_stride, v_head_stride, e, 16);
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid = group_grid(rows, n_seq, n_kv_heads);
 #define READ(T)                                                                                                      \
     if (grid.x)                                                                                                      \
         launch_read_groups<T>(head_dim / 32, grid, s, b, k, v, (int64_t)k_row_stride, (int64_t)k_head_stride,        \
@@ -1812,6 +1816,8 @@ extern "C" size_t mivi_hip_kv_q4_attention_workspace(size_t n_seq, size_t rows, 
                                                      size_t n_kv_heads, size_t head_dim, size_t max_tokens,
                                                      size_t window) {
     if (n_kv_heads == 0 || n_heads == 0 || n_heads % n_kv_heads || rows == 0 || n_seq == 0 || max_rows == 0) return 0;
+    // no call has these: their products could wrap round
+    if (n_heads > 65535 || !head_dim_ok(head_dim) || std::max({n_seq, rows, max_tokens}) > (size_t)INT32_MAX) return 0;
     size_t parts = 1;
     for (int planes = 1; planes <= 2; planes++)
         parts = std::max(parts, attn_plan(n_seq, std::min(max_rows, rows), n_heads / n_kv_heads, n_kv_heads, head_dim,
@@ -1848,7 +1854,10 @@ extern "C" int32_t mivi_hip_kv_q4_attention(
     if (need && !workspace) return set_error(MIVI_ERR_INVALID_ARGUMENT, "null workspace");
     if (need && (uintptr_t)workspace % 16)
         return set_error(MIVI_ERR_INVALID_ARGUMENT, "workspace not 16-byte aligned");
-    if (p.grid > (size_t)INT32_MAX || rows * n_heads > (size_t)INT32_MAX - 4096) return err_overflow();
+    const size_t join_grid = (rows * n_heads + 3) / 4;  // a wave a row and head
+    if (!grid_fits(p.grid, p.threads()) || rows * n_heads > (size_t)INT32_MAX - 4096 ||
+        (p.nsplit > 1 && !grid_fits(join_grid, 256)))
+        return err_overflow();
     clear_error();
     a.q = q, a.out = out;
     a.q_row = (int64_t)q_row_stride, a.q_head = (int64_t)q_head_stride;
@@ -1876,7 +1885,7 @@ extern "C" int32_t mivi_hip_kv_q4_attention(
     }
     MIVI_HIP_CHECK(hipGetLastError());
     if (p.nsplit > 1) {
-        kv_q4_join_kernel<<<(unsigned)((rows * n_heads + 3) / 4), 256, 0, s>>>(a, (int)p.shares);
+        kv_q4_join_kernel<<<(unsigned)join_grid, 256, 0, s>>>(a, (int)p.shares);
         MIVI_HIP_CHECK(hipGetLastError());
     }
     return MIVI_OK;

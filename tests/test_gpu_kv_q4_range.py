@@ -102,6 +102,22 @@ def test_attention_of_scales_next_to_the_largest_float(hip, rows, scale, by):
         check_hull(out, q, kvs, [rows], [100], float(np.float32(scale)), torch.float32, 100)
 
 
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cap", [600, 4096])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_of_values_at_the_limit(hip, name, rows, cap):
+    """Values up to 21760, in every type: the bounds of check_attention."""
+    dt = TYPES[name]
+    heads, kv, hd = 8, 2, 64
+    b = Batch(hip, [rows], [600], kv, hd, 64, cap=cap)
+    kvs = b.fill(hip, scale=2e4)  # some at the limit
+    q = (torch.randn((rows, heads, hd), generator=torch.Generator().manual_seed(4)) * 2.0 ** -10).to(dt)
+    out = torch.empty((rows, heads, hd), dtype=dt, device="cuda")
+    hip.kv_q4_attention(out, q.cuda(), b.cache, b.starts_t, b.lens_t)
+    want, mag, top = reference(q, kvs, [rows], [600], hd ** -0.5)
+    check_attention(out, want, mag, top, dt, hd, 600, max(x.abs().max().item() for kv_ in kvs for x in kv_))
+
+
 @pytest.mark.parametrize("heads,kv,hd,rows,length,by", [
     (28, 4, 96, 1, 4097, 0.3), (8, 2, 64, 6, 100, 0.3), (8, 2, 128, 1, 8192, 0.3), (16, 2, 128, 70, 400, 0.3),
     (8, 2, 64, 40, 300, 0.0), (4, 2, 256, 9, 500, 0.3), (2, 1, 192, 60, 500, 1.0), (4, 4, 32, 120, 300, 0.3),
@@ -121,3 +137,31 @@ def test_fp16_outputs_are_as_near_as_their_rounding(hip, heads, kv, hd, rows, le
     got, best = rms(out.cpu().double() - want), rms(want.half().double() - want)
     print(heads, kv, hd, rows, length, got / best)
     assert got <= 1.1 * best
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_of_queries_of_wide_range(hip, name, rows):
+    """Dimensions of one query far apart: the large ones meet keys of zero, so
+    that the small ones decide. A query is held to 2^-39 of its row's largest
+    magnitude (half of fp16's smallest step beside 2^14), two planes or one."""
+    dt = TYPES[name]
+    heads, kv, hd, length = 4, 2, 64, 100
+    b = Batch(hip, [rows], [length], kv, hd, 64)
+    g = torch.Generator().manual_seed(3)
+    k, v = torch.randn((length, kv, hd), generator=g), torch.randn((length, kv, hd), generator=g)
+    k[..., :32] = 0.0
+    s, l = Batch.tensors([length], [length])
+    hip.kv_q4_append(b.cache, k.cuda(), v.cuda(), s, l)
+    kvs = [(held(k).transpose(0, 1), held(v).transpose(0, 1))]
+    q = torch.randn((rows, heads, hd), generator=g)
+    far = 2.0 ** 12 if dt == torch.float16 else 2.0 ** 24
+    q[..., :32] *= far
+    q = q.to(dt)
+    out = torch.empty((rows, heads, hd), dtype=dt, device="cuda")
+    hip.kv_q4_attention(out, q.cuda(), b.cache, b.starts_t, b.lens_t)
+    want, mag, top = reference(q, kvs, [rows], [length], hd ** -0.5)
+    # what the queries lack, times the keys
+    most = q.double().abs().amax(-1)
+    lack = most * 2.0 ** -39 * hd * kvs[0][0].abs().amax().item() * hd ** -0.5
+    check_attention(out, want, mag, top + lack / 2.0 ** -22, dt, hd, length)

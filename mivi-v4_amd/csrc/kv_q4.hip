@@ -105,13 +105,6 @@ __device__ __forceinline__ bool row_pos(const Q4Batch& a, int s, int r, int* pos
 
 // --------------------------------------------------------- element types
 template <int T>
-__device__ __forceinline__ float load_elem(const void* p, int64_t i) {
-    if constexpr (T == MIVI_GGML_F32) return ((const float*)p)[i];
-    else if constexpr (T == MIVI_GGML_F16) return half_bits_to_f32(((const uint16_t*)p)[i]);
-    else return bf16_bits_to_f32(((const uint16_t*)p)[i]);
-}
-
-template <int T>
 __device__ __forceinline__ uint32_t half_type_bits(float v) {
     if constexpr (T == MIVI_GGML_F16) return f32_to_half_bits(v);
     else return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v);
@@ -147,24 +140,11 @@ __device__ __forceinline__ void words_to_f32(const uint32_t (&w)[kWords8<T>], fl
     }
 }
 
-// 8 values from element i on; `wide`: the address is 16-byte aligned.
 template <int T>
 __device__ __forceinline__ void load8(const void* p, int64_t i, bool wide, float (&x)[8]) {
-    if (!wide) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = load_elem<T>(p, i + e);
-    } else if constexpr (T == MIVI_GGML_F32) {
-        const f32x4 a = *(const f32x4*)((const float*)p + i), b = *(const f32x4*)((const float*)p + i + 4);
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = a[e], x[e + 4] = b[e];
-    } else {
-        const u32x4 w = *(const u32x4*)((const uint16_t*)p + i);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            x[2 * e] = T == MIVI_GGML_F16 ? half_bits_to_f32(w[e]) : bf16_bits_to_f32(w[e]);
-            x[2 * e + 1] = T == MIVI_GGML_F16 ? half_bits_to_f32(w[e] >> 16) : bf16_bits_to_f32(w[e] >> 16);
-        }
-    }
+    uint32_t w[kWords8<T>];
+    load8_words<T>(p, i, wide, w);
+    words_to_f32<T>(w, x);
 }
 
 // N (4 or 8) values to element i on; `wide`: the address is aligned to the

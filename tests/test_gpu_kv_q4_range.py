@@ -165,3 +165,23 @@ def test_attention_of_queries_of_wide_range(hip, name, rows):
     most = q.double().abs().amax(-1)
     lack = most * 2.0 ** -39 * hd * kvs[0][0].abs().amax().item() * hd ** -0.5
     check_attention(out, want, mag, top + lack / 2.0 ** -22, dt, hd, length)
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [20, 50], [300, 2]])
+def test_a_table_without_pages(hip, rows):
+    """No row has a position: nothing is written, rows read and attend as zeros."""
+    heads, kv, hd = 4, 2, 64
+    b = Batch(hip, rows, [400, 400], kv, hd, 64)
+    b.cache.set_pages(torch.empty((2, 0), dtype=torch.int32, device="cuda"))
+    n = sum(rows)
+    x = torch.randn((n, kv, hd), device="cuda")
+    before = b.data.clone()
+    hip.kv_q4_append(b.cache, x, x, b.starts_t, b.lens_t)
+    assert torch.equal(b.data, before)
+    ko, vo = torch.full_like(x, 5.0), torch.full_like(x, 5.0)
+    hip.kv_q4_read(b.cache, ko, vo, b.starts_t, b.lens_t)
+    assert (ko == 0).all() and (vo == 0).all()
+    q = torch.randn((n, heads, hd), device="cuda")
+    out = torch.full_like(q, 5.0)
+    hip.kv_q4_attention(out, q, b.cache, b.starts_t, b.lens_t, max(rows))
+    assert (out == 0).all()

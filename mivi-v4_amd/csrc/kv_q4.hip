@@ -460,9 +460,9 @@ __device__ __forceinline__ _Float16 k_scale(const uint32_t (&ks)[NB], int half, 
 // sequences is needed to place them.
 //
 // 24 bf16 prompts of up to 701 rows, 8 heads of 128 (52 MB in, 15 out): written
-// in 23.6 us, 17 vector instructions an element and 64 lanes, read in 14.9; 8
+// in 21.8 us, 17 vector instructions an element and 64 lanes, read in 15.0; 8
 // values a lane wherever they lie took 48 and 36. 8 x 32768 rows of 8 heads of 64
-// to fp16 (688 MB): 148 us, 4.6 TB/s, 90 % of a copy's rate.
+// to fp16 (688 MB): 141 us, 4.9 TB/s, 94 % of a copy's rate.
 struct Q4Unit {
     int s, g;      // sequence and group
     bool there;    // whether the table has a page of the cache there
@@ -518,9 +518,11 @@ __device__ __forceinline__ void wave_sync() {
 }
 
 // A group's V codes in LDS: 16 bytes more a quarter of the tokens, so that the
-// quarters are in different banks. Pair of blocks i at 1088 i, an odd last block
-// alone behind them; lane n + 16 quarter of it at n * size + quarter * (16 size +
-// 16) with 16 or 8 bytes a lane.
+// quarters are in different banks. (Dimensions n and n + 8 of a pair of blocks
+// are not, at 128 bytes: a byte store takes two turns, 39 to 48 % of the LDS's
+// cycles from 64 dimensions on, which are 4 % of the kernel's.) Pair of blocks i at
+// 1088 i, an odd last block alone behind them; lane n + 16 quarter of it at
+// n * size + quarter * (16 size + 16) with 16 or 8 bytes a lane.
 constexpr int kImage = 4 * 1088;  // bytes of the largest (8 blocks)
 
 template <int T>
@@ -621,8 +623,8 @@ __global__ void __launch_bounds__(256) kv_q4_append_groups_kernel(Q4Batch a, con
 
 // 8 fp16 values (4 dwords) as values of type T to element i on. LINES: the wave
 // stores whole rows, around the caches; pieces of 64 bytes (K) go through L2,
-// which joins them (8 x 32768 rows of 64 to fp16: 148 us; all around the caches
-// 165, all through them 154).
+// which joins them (8 x 32768 rows of 64 to fp16: 142 us; all around the caches
+// 167, all through them 157).
 template <int T, bool LINES>
 __device__ __forceinline__ void store8_half(void* p, int64_t i, bool wide, u32x4 w) {
     if (T == MIVI_GGML_F16 && wide) {
@@ -638,7 +640,11 @@ __device__ __forceinline__ void store8_half(void* p, int64_t i, bool wide, u32x4
 
 // The held values are fp16 numbers: they are formed as the attention forms them
 // and widened. K comes out in rows; V goes through LDS, a row of hd values and 8
-// bytes more a token (the quarters of the tokens in different banks).
+// bytes more a token: the quarters of the tokens, which are stored together, are
+// in different banks. Reading back, 8 of 16 bytes a lane at a time, is without
+// conflicts where 16 lanes hold two tokens (64 dimensions: their rows' 8 bytes
+// interleave); elsewhere conflicts are 18 to 24 % of the LDS's cycles, 2 to 4 %
+// of the kernel's.
 template <int T, int NB>
 __global__ void __launch_bounds__(256) kv_q4_read_groups_kernel(Q4Batch a, void* k, void* v, int64_t k_row,
                                                                 int64_t k_head, int64_t v_row, int64_t v_head,
@@ -1101,13 +1107,13 @@ __device__ __forceinline__ bool head_place(const Q4Attn& a, int lane, int shares
 // K of the next group is on its way during the sums, V during the scores, and
 // page ids two groups ahead of that.
 //
-// Bound: about 200 (hd 64, two planes) to 290 (hd 128, one) vector instructions
-// a group, half of them codes to values, 73 and 62 % of the cycles; the loads alone take
-// 28 us where the kernel takes 41 (8 sequences of 32768 tokens, 8 heads of 64,
-// f32: 151 MB, 3.6 TB/s). 64 ragged sequences of up to 8192, 8 heads of 128, bf16:
-// 71 us, 297 MB, 4.2 TB/s. No faster: the next group's scores formed beside this
-// one's sums (46 us), five waves a SIMD (45), four groups' scores in sets of four
-// columns (fewer exponentials, two waves a SIMD: 41).
+// Bound: about 210 (hd 64, two planes) to 300 (hd 128, one) vector instructions
+// a group, half of them codes to values, 76 and 62 % of the cycles. 8 sequences of
+// 32768 tokens, 8 heads of 64, f32: 40 us, 151 MB, 3.8 TB/s (the loads alone took
+// 28 us of 41). 64 ragged sequences of up to 8192, 8 heads of 128, bf16:
+// 69 us, 297 MB, 4.3 TB/s. No faster: the next group's scores formed beside this
+// one's sums (46 us where the kernel took 42), five waves a SIMD (45), four groups'
+// scores in sets of four columns (fewer exponentials, two waves a SIMD: 41).
 //
 // Waves a SIMD that the registers are held to: 17 nb words of codes, scales and
 // sums and 4 nb a plane of queries beside about 40 others; 4 where the weights
@@ -1226,10 +1232,10 @@ __global__ void __launch_bounds__(256, step_waves(NB, PQ, PW)) kv_q4_step_kernel
 // some blocks of one group.
 //
 // Bound: vector instructions and matrix instructions of a SIMD in turn. 2 x 2048
-// bf16 rows at 32768 tokens, 32 / 8 heads of 128 (NT 2, NW 8): 2.22 ms, 905
-// TFLOP/s, matrix pipe busy 40 %, vector pipe 43; with four waves a conversion
-// 2.48 ms. 2048 f32 rows at 4096, heads of 64: 132 us, the planes doubling both
-// products. 16 x 5 bf16 rows at up to 12000 tokens, 4 heads of 128 (NT 1): 36 us,
+// bf16 rows at 32768 tokens, 32 / 8 heads of 128 (NT 2, NW 8): 2.25 ms, 894
+// TFLOP/s, matrix pipe busy 39 %, vector pipe 45; with four waves a conversion 12 %
+// more. 2048 f32 rows at 4096, heads of 64: 132 us, the planes doubling both
+// products. 16 x 5 bf16 rows at up to 12000 tokens, 4 heads of 128 (NT 1): 34 us,
 // the chain of barrier, scores, weights and sums of one tile a wave.
 template <int NB, int PQ, int PW, int NT, int NW, int TG>
 __global__ void __launch_bounds__(64 * NW) kv_q4_rows_kernel(Q4Attn a, int shares) {
@@ -1586,7 +1592,10 @@ int32_t make_batch(Q4Batch* b, const uint8_t* cache, size_t cache_len, size_t n_
 
 // Grid of the kernels that take whole groups: units times as many workgroups a
 // unit as fill the card (each wave at least one head's K or V); none (x = 0)
-// where the call has fewer than 8 rows a sequence: those go 8 values a lane.
+// where the call has fewer than 8 rows a sequence: those go 8 values a lane. (64
+// sequences, 8 bf16 heads of 128, written and read back by groups and 8 values a
+// lane: 4 rows each 12.5 and 9.1 us, 8 rows 12.9 and 10.8, 16 rows 14.0 and 14.3,
+// 32 rows 14.3 and 19.3.)
 dim3 group_grid(size_t rows, size_t n_seq, size_t n_kv) {
     if (rows < 8 * n_seq) return dim3(0, 0);
     const size_t units = rows / kGroup + 2 * n_seq, most = (n_kv + 1) / 2;
@@ -1623,11 +1632,13 @@ Q4Plan attn_plan(size_t n_seq, size_t max_rows, size_t gq, size_t n_kv, size_t h
     if (__builtin_mul_overflow(n_seq, n_kv, &heads)) heads = SIZE_MAX;
     // By registers: two tiles a wave and two or three workgroups a CU up to 96
     // dimensions, one tile a wave past 128; at 128 the 256 pairs that share a
-    // conversion need two workgroups a CU's worth of tiles to end evenly (2 x
-    // 2048 bf16 rows at 32768: 2210 us, with 128 pairs 2420; 2048 rows of one
-    // prompt from its start 84 and 67), and two planes do not fit one tile a wave
-    // twice on a CU (2 x 700 f32 rows at 32768: 1290 and 1670). 65 to 128 pairs
-    // as two tiles of 64: 8 x 25 f32 rows at 4096 57.6 us, as one of 128 109.
+    // conversion need two workgroups a CU's worth of tiles to end evenly (8 kv
+    // heads, 2 x 2048 bf16 rows at 32768: 2260 us, with 128 pairs 2590; 2048 rows
+    // of one prompt from its start 88 and 70), and two planes of queries do not
+    // fit one tile a wave twice on a CU (2 x 700 f32 rows at 32768: 1370 and
+    // 1720). 65 to 128 pairs as two tiles of 64: 8 x 25 f32 rows at 4096, heads
+    // of 128, 59.6 us, as one of 128 114 (bf16 49.9 and 71.5, f32 heads of 64
+    // 40.5 and 50.9).
     p.form = pairs <= 16    ? Q4Plan::kStep
              : pairs <= 128 ? Q4Plan::kFew
              : hd > 128     ? Q4Plan::kSome
@@ -1643,10 +1654,11 @@ Q4Plan attn_plan(size_t n_seq, size_t max_rows, size_t gq, size_t n_kv, size_t h
     size_t all, wgs;
     if (__builtin_mul_overflow(heads, groups, &all)) all = SIZE_MAX;
     // One part a head, which needs no second kernel, where it is short: 8 groups
-    // a wave, 4 of more than 128 dimensions, 8 groups in all of more rows. (One
-    // token, 8 heads of 64, f32: at 1024 tokens 9.9 us against 12.9 in shares and
-    // a join, 14.7 at 2048; 64 sequences at 1024 18.7 against 22.8; 4 heads of
-    // 256 at 512 13.0 and 13.8; 16 rows at 256 10.5 and 14.)
+    // a wave, 4 of more than 128 dimensions, 8 groups in all of more rows. (In one
+    // part and in shares with a join, captured: one token, 8 heads of 64, f32, at
+    // 1024 tokens 9.0 and 11.2 us, at 2048 13.6 and 11.3; 64 sequences at 1024 15.5
+    // and 26.4; 4 sequences of 4 bf16 heads of 256 at 512 12.2 and 14.1, at 1024
+    // 17.4 and 14.5; 16 rows at 256 10.2 and 13.9, at 512 15.3 and 13.9.)
     if (p.tiles == 1 && groups <= (p.form == Q4Plan::kStep ? hd <= 128 ? 32 : 16 : 8)) {
         p.chunk = groups, p.nsplit = 1, p.grid = heads;
         return p;
@@ -1684,8 +1696,9 @@ void launch_attn(const Q4Attn& a, const Q4Plan& p, hipStream_t s) {
     if (p.form == Q4Plan::kStep) {
         kv_q4_step_kernel<NB, PQ, PW><<<grid, 256, 0, s>>>(a, shares);
     } else if (p.form == Q4Plan::kFew) {
-        // two groups a step at 64 dimensions (16 x 5 rows 44.7 -> 39.3 us); at 128
-        // their LDS halves the workgroups of a CU (57 -> 63)
+        // two groups a step at 64 dimensions (16 x 5 bf16 rows at up to 12000
+        // tokens, 4 heads: 35.4 -> 32.0 us); at 128 their LDS halves the workgroups
+        // of a CU (42.4 -> 51.2)
         kv_q4_rows_kernel<NB, PQ, PW, 1, 4, NB <= 2 ? 2 : 1><<<grid, 256, 0, s>>>(a, shares);
     } else if constexpr (NB <= 3) {
         kv_q4_rows_kernel<NB, PQ, PW, 2, 4, 2><<<grid, 256, 0, s>>>(a, shares);

@@ -185,3 +185,32 @@ def test_a_table_without_pages(hip, rows):
     out = torch.full_like(q, 5.0)
     hip.kv_q4_attention(out, q, b.cache, b.starts_t, b.lens_t, max(rows))
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [9, 3]])
+def test_rows_more_than_two_billion_elements_apart(hip, rows):
+    """Offsets past 32 bits, in elements and in bytes, in every tensor."""
+    heads, kv, hd, lens = 4, 2, 64, [1500, 700]
+    n = sum(rows)
+    b = Batch(hip, rows, lens, kv, hd, 64)
+    kvs = [tuple(x.clone() for x in kv_) for kv_ in b.fill(hip, dtype=torch.bfloat16)]
+    apart = 2 ** 31 // (n - 1) + 64
+    buf = torch.empty((n - 1) * apart + 3 * heads * hd, dtype=torch.bfloat16, device="cuda")
+
+    def view(first, h):
+        return buf[first * hd:].as_strided((n, h, hd), (apart, hd, 1))
+    g = torch.Generator().manual_seed(4)
+    q, k, v = (torch.randn((n, h, hd), generator=g).to(torch.bfloat16) for h in (heads, kv, kv))
+    view(0, heads).copy_(q), view(heads, kv).copy_(k), view(heads + kv, kv).copy_(v)
+    hip.kv_q4_append(b.cache, view(heads, kv), view(heads + kv, kv), b.starts_t, b.lens_t)
+    ko, vo = view(heads + 2 * kv, kv), view(heads + 3 * kv, kv)
+    hip.kv_q4_read(b.cache, ko, vo, b.starts_t, b.lens_t)
+    assert torch.equal(ko.cpu(), held(k).to(ko.dtype)) and torch.equal(vo.cpu(), held(v).to(vo.dtype))
+    out = view(2 * heads, heads)
+    hip.kv_q4_attention(out, view(0, heads), b.cache, b.starts_t, b.lens_t, max(rows))
+    at = 0
+    for i, (r, t) in enumerate(zip(rows, lens)):
+        kvs[i][0][:, t - r:t], kvs[i][1][:, t - r:t] = (held(x[at:at + r]).transpose(0, 1) for x in (k, v))
+        at += r
+    want, mag, top = reference(q, kvs, rows, lens, hd ** -0.5)
+    check_attention(out.contiguous(), want, mag, top, torch.bfloat16, hd, max(lens))

@@ -279,3 +279,34 @@ def test_the_default_workspace_of_the_null_stream(hip, monkeypatch):
     assert seen == [0]
     want, mag, top = reference(q, kvs, [1], [3000], hd ** -0.5)
     check_attention(out, want, mag, top, torch.float32, hd, 3000)
+
+
+def test_captured_steps_on_their_default_workspaces(hip):
+    """Two captured steps that name no workspace, replayed in turn with eager
+    work and other allocations between."""
+    heads, kv, hd = 8, 2, 64
+    b = Batch(hip, [1, 2], [4096, 2000], kv, hd, 64)
+    need_of(hip, b, [1, 2], heads, 2)
+    kvs = b.fill(hip)
+    gen = torch.Generator().manual_seed(4)
+    jobs = []
+    for _ in range(2):
+        q = torch.randn((3, heads, hd), generator=gen).cuda()
+        out = torch.empty(q.shape, device="cuda")
+        hip.kv_q4_attention(out, q, b.cache, b.starts_t, b.lens_t, 2)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            hip.kv_q4_attention(out, q, b.cache, b.starts_t, b.lens_t, 2)
+        jobs.append((graph, q, out))
+    for _ in range(4):
+        for graph, q, out in jobs:
+            q.copy_(torch.randn(q.shape, generator=gen))
+            out.fill_(9.0)
+            graph.replay()
+            torch.full((1 << 20,), 7.0, device="cuda")
+            eager = torch.empty_like(out)
+            hip.kv_q4_attention(eager, q, b.cache, b.starts_t, b.lens_t, 2)
+            assert torch.equal(out, eager)
+    _, q, out = jobs[0]
+    want, mag, top = reference(q, kvs, [1, 2], [4096, 2000], hd ** -0.5)
+    check_attention(out, want, mag, top, torch.float32, hd, 4096)

@@ -265,14 +265,15 @@ size_t mivi_hip_kv_q4_attention_workspace(size_t n_seq, size_t rows, size_t max_
  * head j / (n_heads / n_kv_heads). What no row sees need never have been
  * written. A row that sees nothing is zero. max_rows:
  * at least the rows of any one sequence; a sequence's rows past it are not
- * computed. F32 queries enter the products with 22 bits, F16 and BF16 ones with
+ * computed.
+ * Precision: F32 queries enter the products with 22 bits, F16 and BF16 ones with
  * all of theirs, any of them to no less than 2^-39 of its row's largest
- * magnitude; softmax weights of F32 and F16 calls with 22 bits, of BF16 calls
- * with 11 (their rounding is then about 2^-12 of sum w |v| over the square root
- * of the tokens), and none to less than 2^-36 of its row's largest (2^-25 where
- * a score passes 2^19); sums are f32. Finite q and scale give finite outputs, the weights being those of the
- * scores as f32 products give them, however large. An infinity or NaN in q
- * stays in its row and head.
+ * magnitude. Softmax weights have 22 bits in F32 and F16 calls, 11 in BF16 ones
+ * (their rounding adds about 2^-12 of sum w |v| over the square root of the
+ * tokens), none to less than 2^-36 of its row's largest, 2^-25 where a score
+ * passes 2^19. Sums are f32. Finite q and scale give finite outputs, the weights
+ * being those of the scores as f32 products give them, however large. An
+ * infinity or NaN in q stays in its row and head.
  * `workspace`: 16-byte aligned, mivi_hip_kv_q4_attention_workspace bytes for
  * the call's arguments, in use until the call's work is done; calls that may
  * overlap need workspaces of their own. */

@@ -5,8 +5,8 @@ the verification of drafted tokens.
 norm    s = x + residual, out = s (mean s^2 + eps)^(-1/2) w over the last
         dimension, and s itself rounded to its type; or out in 8 bits: in each
         group of a row (`group` dimensions, 0 the whole row) with A = max |s w|
-        codes rint(127 s w / A), which stand for A (mean s^2 + eps)^(-1/2) / 127
-        times themselves.
+        codes rint(127 s w / A) (ties to even), which stand for A (mean s^2 +
+        eps)^(-1/2) / 127 times themselves.
 rope    pairs (a, b) of the first `rot` dimensions turned by position times
         frequency, dimensions (2 i, 2 i + 1) or (i, i + rot / 2), the others
         copied. Rows are ragged as in the cache: row i of a sequence's n is at
@@ -244,7 +244,7 @@ def _norm(s):
     y = s["x"].double() + s["r"].double() if c["residual"] else s["x"].double()
     y = (y * s["w"].double()).view(c["rows"], -1, c["group"] or c["dim"])
     top = y.abs().amax(-1, keepdim=True)
-    codes = (y * (127 / torch.where(top == 0, 1.0, top))).round_()
+    codes = (y * 127 / torch.where(top == 0, 1.0, top)).round_()
     scale = (top * f.double() / 127).float()
     return dict(out, out=(codes.float() * scale).view(c["rows"], -1))
 
@@ -354,9 +354,8 @@ def exact(case, seed):
         v = (s64 * s["w"]).unflatten(-1, (-1, case["group"] or case["dim"]))
         hi, lo = v.amax(-1), v.amin(-1)
         top = torch.maximum(hi, -lo)[..., None]
-        step = top / 127
-        codes = torch.where(top > 0, v / torch.where(top > 0, step, 1.0), 0.0).round()
-        return dict(out, out=(codes * step * f[..., None, None]).flatten(1))
+        codes = torch.where(top > 0, 127 * v / torch.where(top > 0, top, 1.0), 0.0).round()
+        return dict(out, out=(codes * (top / 127) * f[..., None, None]).flatten(1))
     if kind == "rope":
         rows, lens = _ragged(case)
         pos = np.concatenate([np.arange(t - n, t) for n, t in zip(rows, lens)])

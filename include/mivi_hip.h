@@ -287,6 +287,137 @@ int32_t mivi_hip_kv_q4_attention(int32_t type, void* out, size_t out_len, size_t
                                  void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------
+ * The parts of a step around that cache, for a host that drives its own layers
+ * (the model handles fuse these into their kernels): norms, rotary positions,
+ * products with 4-bit weights that have group scales, verification of drafted
+ * tokens. No counterparts as calls in the reference. Tensors, `type`, strides,
+ * starts, lens, streams and captures as for the 4-bit cache; nothing is
+ * allocated. A tensor may be written over the one it is made from (same address
+ * and strides); written tensors must not overlap anything else.
+ * ------------------------------------------------------------------- */
+
+/* s = x + residual (residual may be NULL), out = s w / sqrt(mean s^2 + eps) over
+ * the dim elements of every row and head; s rounded to `type` into sum (may be
+ * NULL; residual itself, usually). out is formed from s before that rounding.
+ * weight: f32. eps at least 1e-30. Squares are summed in 64 bits, the rest is
+ * f32. (crates/mivi-model/src/norm.rs is the model's own.) */
+int32_t mivi_hip_rms_norm(int32_t type, void* out, size_t out_len, size_t out_row_stride,
+                          size_t out_head_stride, const void* x, size_t x_len, size_t x_row_stride,
+                          size_t x_head_stride, const void* residual, size_t residual_len,
+                          size_t residual_row_stride, size_t residual_head_stride, void* sum,
+                          size_t sum_len, size_t sum_row_stride, size_t sum_head_stride,
+                          const float* weight, size_t weight_len, float eps, size_t rows, size_t heads,
+                          size_t dim, void* stream);
+
+/* The same in 8 bits, for mivi_hip_w4_matmul_rows_q8: codes [rows][dim] (signed
+ * bytes) and scales [rows][dim / group]; group 32, 64, 128, 256 or 512 dimensions, or 0 for
+ * one scale a row. With A the group's largest |s w|: code = 127 s w / A rounded
+ * to nearest (ties to even), scale = A / sqrt(mean s^2 + eps) / 127, so codes
+ * are those of exact arithmetic in s w. A group of zeros has scale 0; a row with
+ * an infinity or NaN in s, and a group with one in s w, has codes 0 and scale
+ * NaN. */
+int32_t mivi_hip_rms_norm_q8(int32_t type, uint8_t* codes, size_t codes_len, float* scales,
+                             size_t scales_len, size_t group, const void* x, size_t x_len,
+                             size_t x_row_stride, const void* residual, size_t residual_len,
+                             size_t residual_row_stride, void* sum, size_t sum_len,
+                             size_t sum_row_stride, const float* weight, size_t weight_len, float eps,
+                             size_t rows, size_t dim, void* stream);
+
+/* Turns pairs of every q and k head's first rot_dim dimensions by position times
+ * freqs[i] (f64, radians a position, rot_dim / 2 of them, on the device) and
+ * multiplies them by `scale`; the dimensions behind them are copied. Pair i is
+ * (2 i, 2 i + 1), as the model's (rope.rs:452-473), or with half_pairs != 0 (i,
+ * i + rot_dim / 2). The position of a row is positions[row] (any i32; a negative
+ * one turns back), or, with positions NULL, its position in the batch of starts
+ * and lens that mivi_hip_kv_q4_append takes next (rows outside it are left
+ * alone). Either of q and k may have no heads. Angles are taken in 64 bits at any
+ * position, the rest is f32. head_dim up to 1024. */
+int32_t mivi_hip_rope(int32_t type, void* q_out, size_t q_out_len, size_t q_out_row_stride,
+                      size_t q_out_head_stride, const void* q, size_t q_len, size_t q_row_stride,
+                      size_t q_head_stride, size_t n_heads, void* k_out, size_t k_out_len,
+                      size_t k_out_row_stride, size_t k_out_head_stride, const void* k, size_t k_len,
+                      size_t k_row_stride, size_t k_head_stride, size_t n_kv_heads, size_t rows,
+                      size_t head_dim, size_t rot_dim, int32_t half_pairs, const void* freqs,
+                      size_t freqs_len, float scale, const int32_t* positions, size_t positions_len,
+                      const int32_t* starts, const int32_t* lens, size_t n_seq, void* stream);
+
+/* Frequencies for mivi_hip_rope into host memory: base^(-2 i / rot_dim), and for
+ * a context `factor` times the trained one (factor <= 1: unchanged)
+ *   MIVI_ROPE_LINEAR  all divided by factor
+ *   MIVI_ROPE_BASE    of the base base factor^(rot_dim / (rot_dim - 2))
+ *   MIVI_ROPE_YARN    divided by factor where a pair turns less than once over
+ *                     `context` trained tokens, unchanged where 32 times or more,
+ *                     in between by a ramp over the pair's index; multiply with
+ *                     scale 0.1 ln(factor) + 1
+ *   MIVI_ROPE_MODEL   as the model handles past 4096 tokens (model.rs:194-206,
+ *                     rope.rs:50-122): a ramp over the wavelength between
+ *                     context / 32 and context, no scale */
+#define MIVI_ROPE_PLAIN 0
+#define MIVI_ROPE_LINEAR 1
+#define MIVI_ROPE_BASE 2
+#define MIVI_ROPE_YARN 3
+#define MIVI_ROPE_MODEL 4
+int32_t mivi_hip_rope_frequencies(int32_t kind, float base, float factor, size_t context,
+                                  size_t rot_dim, void* freqs, size_t freqs_len);
+
+/* 4-bit weights with group scales: weight (n, k) is (c - z) s, c a code 0..15, s
+ * (f16 or bf16: scale_type) and z (0..15, or 8 without zeros) of its group of
+ * `group` columns. group: 32, 64, a multiple of 128, or cols; cols a multiple of
+ * 32 and of group. */
+
+/* Bytes of the packed weights (0: no such shape). */
+size_t mivi_hip_w4_packed_size(size_t rows, size_t cols, size_t group, int32_t has_zeros);
+
+/* Lays weights out for the products, once at load: codes [rows][cols / 2], the
+ * even column in the low nibble; scales and zeros (bytes; may be NULL)
+ * [rows][cols / group]. packed: 16-byte aligned. */
+int32_t mivi_hip_w4_pack(const uint8_t* codes, size_t codes_len, int32_t scale_type, const void* scales,
+                         size_t scales_len, const uint8_t* zeros, size_t zeros_len, uint8_t* packed,
+                         size_t packed_len, size_t rows, size_t cols, size_t group, void* stream);
+
+/* out[batch][rows] = x[batch][cols] W^T, both in `type`. The products are exact
+ * in f16 and bf16, of 24 bits of x in f32; sums and scales are f32. The order of
+ * a row's sums, and so its last bits, depends on the batch it is in. */
+int32_t mivi_hip_w4_matmul_rows(int32_t type, void* out, size_t out_len, size_t out_row_stride,
+                                const uint8_t* packed, size_t packed_len, int32_t scale_type,
+                                int32_t has_zeros, const void* x, size_t x_len, size_t x_row_stride,
+                                size_t batch, size_t rows, size_t cols, size_t group, void* stream);
+
+/* The same for x in 8 bits as mivi_hip_rms_norm_q8 leaves it (codes
+ * [batch][cols], scales [batch][cols / x_group], or [batch] with x_group 0); out
+ * in `type`. Sums over 128 columns (or the smaller group) are exact. */
+int32_t mivi_hip_w4_matmul_rows_q8(int32_t type, void* out, size_t out_len, size_t out_row_stride,
+                                   const uint8_t* packed, size_t packed_len, int32_t scale_type,
+                                   int32_t has_zeros, const uint8_t* codes, size_t codes_len,
+                                   const float* scales, size_t scales_len, size_t x_group, size_t batch,
+                                   size_t rows, size_t cols, size_t group, void* stream);
+
+/* Verification of drafted tokens, sequence s on rows starts[s] .. starts[s + 1]
+ * - 1 (as mivi_hip_kv_q4_attention computed them): row r but the last holds in
+ * target[r] the target's probabilities and in draft[r] the draft's of the place
+ * where drafted[r] was drafted (draft NULL: each was certain), and is accepted if
+ * accept[r] draft[r][t] < target[r][t], t = drafted[r], in it and in all before
+ * it. The next token is drawn from the first row that is not: from max(target -
+ * draft, 0), or, in the last row and where that is all zero, from target: the
+ * first index whose cumulative sum passes pick[s] times the whole. With accept
+ * and pick uniform in [0, 1) the tokens have the target's distribution.
+ * tokens[rows]: the accepted ones, the drawn one (-1 where the row has no
+ * probability above 0) and -1 behind it; counts[n_seq]: accepted ones. Rows need
+ * not sum to 1; what is negative, infinite or NaN counts as 0; a drafted id
+ * outside 0 .. n - 1 is not accepted. Comparisons are exact, sums of 64 bits in a
+ * fixed order. A sequence without rows has count 0; rows outside the sequences
+ * are left alone. n_seq at most 65535. workspace: 16-byte aligned, of
+ * mivi_hip_verify_rows_workspace bytes, as mivi_hip_kv_q4_attention's. */
+size_t mivi_hip_verify_rows_workspace(size_t n, size_t n_seq);
+int32_t mivi_hip_verify_rows(int32_t* tokens, size_t tokens_len, int32_t* counts, size_t counts_len,
+                             const float* target, size_t target_len, size_t target_row_stride,
+                             const float* draft, size_t draft_len, size_t draft_row_stride,
+                             const int32_t* drafted, size_t drafted_len, const float* accept,
+                             size_t accept_len, const float* pick, size_t pick_len,
+                             const int32_t* starts, size_t n_seq, size_t rows, size_t n,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------
  * mivi-model: one hybrid (ShortConv + GQA) model resident on the GPU
  * ------------------------------------------------------------------- */
 

@@ -33,15 +33,18 @@ DEVICE_FLAGS = [
 ]
 HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall"]
 
-SOURCES = ["errors.cpp", "synth.cpp", "quant.hip", "gemm.hip", "model.hip", "sampler.hip", "kv_q4.hip"]
+SOURCES = ["errors.cpp", "synth.cpp", "quant.hip", "gemm.hip", "model.hip", "sampler.hip", "kv_q4.hip",
+           "norm.hip", "rope.hip", "verify.hip", "w4.hip"]
 
 # Per-source device flags. quant.hip, gemm.hip: MFMA results straight into
 # VGPRs (the GEMV kernels consume each result at once, the row products fold
-# theirs into f32 sums, the 4-bit cache's attention works on its scores; in
-# AGPRs every one of them costs a v_accvgpr_read).
+# theirs into f32 sums, the 4-bit cache's attention works on its scores, the
+# 4-bit weights' products scale their sums group by group; in AGPRs every one
+# of them costs a v_accvgpr_read).
 EXTRA_FLAGS = {"quant.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                "gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-               "kv_q4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+               "kv_q4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+               "w4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _deps(src: str) -> list[str]:

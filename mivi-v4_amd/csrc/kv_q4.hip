@@ -38,6 +38,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "rows.h"
 
 using namespace mivi;
 
@@ -1513,43 +1514,10 @@ constexpr size_t kMaxPageTokens = 1024;
 
 bool head_dim_ok(size_t hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 192 || hd == 256; }
 
-size_t type_bytes(int32_t t) { return t == MIVI_GGML_F32 ? 4 : t == MIVI_GGML_F16 || t == MIVI_GGML_BF16 ? 2 : 0; }
-
-// Elements from the first to the last of rows x heads x hd, or SIZE_MAX.
-size_t span(size_t rows, size_t row_stride, size_t heads, size_t head_stride, size_t hd) {
-    size_t a, b, c;
-    if (__builtin_mul_overflow(rows - 1, row_stride, &a) || __builtin_mul_overflow(heads - 1, head_stride, &b) ||
-        __builtin_add_overflow(a, b, &c) || __builtin_add_overflow(c, hd, &c) || c > (size_t)INT64_MAX / 8)
-        return SIZE_MAX;
-    return c;
-}
-
-int32_t check_tensor(const char* what, const void* p, size_t len, int32_t type, size_t rows, size_t row_stride,
-                     size_t heads, size_t head_stride, size_t hd, bool written) {
-    const size_t need = span(rows, row_stride, heads, head_stride, hd);
-    if (need == SIZE_MAX) return err_overflow();
-    if (len < need) return err_buffer_too_small(need, len);
-    if (!p) return set_error(MIVI_ERR_INVALID_ARGUMENT, "null %s", what);
-    if ((uintptr_t)p % type_bytes(type)) return set_error(MIVI_ERR_INVALID_ARGUMENT, "%s not aligned to its type", what);
-    // rows and heads that are written must not overlap each other
-    if (written && heads > 1 && head_stride < hd)
-        return set_error(MIVI_ERR_INVALID_ARGUMENT, "%s: head stride %zu < head_dim %zu", what, head_stride, hd);
-    if (written && rows > 1) {
-        const bool rows_outer = row_stride >= (heads - 1) * head_stride + hd;
-        const bool heads_outer = heads > 1 && row_stride >= hd && head_stride >= (rows - 1) * row_stride + hd;
-        if (!rows_outer && !heads_outer)
-            return set_error(MIVI_ERR_INVALID_ARGUMENT, "%s: rows of stride %zu overlap", what, row_stride);
-    }
-    return MIVI_OK;
-}
-
 // Vector access: pointer and strides multiples of `bytes`.
 int wide_ok(const void* p, size_t row_stride, size_t head_stride, size_t elem, size_t bytes) {
     return (uintptr_t)p % bytes == 0 && row_stride * elem % bytes == 0 && head_stride * elem % bytes == 0;
 }
-
-// A launch counts the threads of a dimension in 32 bits.
-bool grid_fits(size_t groups, size_t threads) { return groups <= UINT32_MAX / threads; }
 
 int32_t check_geometry(size_t n_kv, size_t hd, size_t page_tokens) {
     if (hd % 32) return err_misaligned(hd, 32);

@@ -166,6 +166,48 @@ pub mod ffi {
             n_seq: usize, starts: *const i32, lens: *const i32,
             workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> i32;
 
+        // the parts of a step around the 4-bit cache
+        pub fn mivi_hip_rms_norm(type_: i32, out: *mut c_void, out_len: usize, out_row_stride: usize,
+            out_head_stride: usize, x: *const c_void, x_len: usize, x_row_stride: usize, x_head_stride:
+            usize, residual: *const c_void, residual_len: usize, residual_row_stride: usize,
+            residual_head_stride: usize, sum: *mut c_void, sum_len: usize, sum_row_stride: usize,
+            sum_head_stride: usize, weight: *const f32, weight_len: usize, eps: f32, rows: usize, heads:
+            usize, dim: usize, stream: *mut c_void) -> i32;
+        pub fn mivi_hip_rms_norm_q8(type_: i32, codes: *mut u8, codes_len: usize, scales: *mut f32,
+            scales_len: usize, group: usize, x: *const c_void, x_len: usize, x_row_stride: usize,
+            residual: *const c_void, residual_len: usize, residual_row_stride: usize, sum: *mut c_void,
+            sum_len: usize, sum_row_stride: usize, weight: *const f32, weight_len: usize, eps: f32,
+            rows: usize, dim: usize, stream: *mut c_void) -> i32;
+        pub fn mivi_hip_rope(type_: i32, q_out: *mut c_void, q_out_len: usize, q_out_row_stride: usize,
+            q_out_head_stride: usize, q: *const c_void, q_len: usize, q_row_stride: usize,
+            q_head_stride: usize, n_heads: usize, k_out: *mut c_void, k_out_len: usize,
+            k_out_row_stride: usize, k_out_head_stride: usize, k: *const c_void, k_len: usize,
+            k_row_stride: usize, k_head_stride: usize, n_kv_heads: usize, rows: usize, head_dim: usize,
+            rot_dim: usize, half_pairs: i32, freqs: *const c_void, freqs_len: usize, scale: f32,
+            positions: *const i32, positions_len: usize, starts: *const i32, lens: *const i32, n_seq:
+            usize, stream: *mut c_void) -> i32;
+        pub fn mivi_hip_rope_frequencies(kind: i32, base: f32, factor: f32, context: usize, rot_dim:
+            usize, freqs: *mut c_void, freqs_len: usize) -> i32;
+        pub fn mivi_hip_w4_packed_size(rows: usize, cols: usize, group: usize, has_zeros: i32) -> usize;
+        pub fn mivi_hip_w4_pack(codes: *const u8, codes_len: usize, scale_type: i32, scales: *const
+            c_void, scales_len: usize, zeros: *const u8, zeros_len: usize, packed: *mut u8, packed_len:
+            usize, rows: usize, cols: usize, group: usize, stream: *mut c_void) -> i32;
+        pub fn mivi_hip_w4_matmul_rows(type_: i32, out: *mut c_void, out_len: usize, out_row_stride:
+            usize, packed: *const u8, packed_len: usize, scale_type: i32, has_zeros: i32, x: *const
+            c_void, x_len: usize, x_row_stride: usize, batch: usize, rows: usize, cols: usize, group:
+            usize, stream: *mut c_void) -> i32;
+        pub fn mivi_hip_w4_matmul_rows_q8(type_: i32, out: *mut c_void, out_len: usize, out_row_stride:
+            usize, packed: *const u8, packed_len: usize, scale_type: i32, has_zeros: i32, codes: *const
+            u8, codes_len: usize, scales: *const f32, scales_len: usize, x_group: usize, batch: usize,
+            rows: usize, cols: usize, group: usize, stream: *mut c_void) -> i32;
+        pub fn mivi_hip_verify_rows_workspace(n: usize, n_seq: usize) -> usize;
+        pub fn mivi_hip_verify_rows(tokens: *mut i32, tokens_len: usize, counts: *mut i32, counts_len:
+            usize, target: *const f32, target_len: usize, target_row_stride: usize, draft: *const f32,
+            draft_len: usize, draft_row_stride: usize, drafted: *const i32, drafted_len: usize, accept:
+            *const f32, accept_len: usize, pick: *const f32, pick_len: usize, starts: *const i32, n_seq:
+            usize, rows: usize, n: usize, workspace: *mut c_void, workspace_bytes: usize, stream: *mut
+            c_void) -> i32;
+
         // crates/mivi-model/src/model.rs:105-606
         pub fn mivi_hip_model_create(gguf: *const u8, gguf_len: usize, max_ctx: usize, kv_precision: i32,
             max_batch: usize, out: *mut *mut MiviModel) -> i32;

@@ -130,6 +130,18 @@ _sig = {
     "mivi_hip_kv_q4_attention_workspace": ([_S] * 8, _S),
     "mivi_hip_kv_q4_attention": ([_I, _P, _S, _S, _S, _P, _S, _S, _S, _S, _S, _S, C.c_float, _S] + _kv_q4
                                  + [_P, _S, _P], _I),
+    "mivi_hip_rms_norm": ([_I] + [_P, _S, _S, _S] * 4 + [_P, _S, C.c_float, _S, _S, _S, _P], _I),
+    "mivi_hip_rms_norm_q8": ([_I, _P, _S, _P, _S, _S] + [_P, _S, _S] * 3 + [_P, _S, C.c_float, _S, _S, _P], _I),
+    "mivi_hip_rope": ([_I] + [_P, _S, _S, _S, _P, _S, _S, _S, _S] * 2 + [_S, _S, _S, _I, _P, _S, C.c_float, _P, _S, _P,
+                                                                        _P, _S, _P], _I),
+    "mivi_hip_rope_frequencies": ([_I, C.c_float, C.c_float, _S, _S, _P, _S], _I),
+    "mivi_hip_w4_packed_size": ([_S, _S, _S, _I], _S),
+    "mivi_hip_w4_pack": ([_P, _S, _I, _P, _S, _P, _S, _P, _S, _S, _S, _S, _P], _I),
+    "mivi_hip_w4_matmul_rows": ([_I, _P, _S, _S, _P, _S, _I, _I, _P, _S, _S, _S, _S, _S, _S, _P], _I),
+    "mivi_hip_w4_matmul_rows_q8": ([_I, _P, _S, _S, _P, _S, _I, _I, _P, _S, _P, _S, _S, _S, _S, _S, _S, _P], _I),
+    "mivi_hip_verify_rows_workspace": ([_S, _S], _S),
+    "mivi_hip_verify_rows": ([_P, _S, _P, _S, _P, _S, _S, _P, _S, _S, _P, _S, _P, _S, _P, _S, _P, _S, _S, _S, _P, _S,
+                              _P], _I),
     "mivi_hip_model_create": ([_P, _S, _S, _I, _S, C.POINTER(_P)], _I),
     "mivi_hip_model_destroy": ([_P], None),
     "mivi_hip_model_info": ([_P, C.POINTER(MiviModelInfo)], _I),
@@ -393,3 +405,5 @@ def synth_random_weights(ggml_type, seed: int, rows: int, cols: int, std: float 
 
 from .kv_q4 import KvCacheQ4, kv_q4_append, kv_q4_attention, kv_q4_page_bytes, kv_q4_read  # noqa: E402,F401
 from .model import Model, PrefixCache, chunk_hash  # noqa: E402,F401
+from .step import (W4Weights, rms_norm, rms_norm_q8, rope, rope_frequencies, verify_rows,  # noqa: E402,F401
+                   w4_matmul_rows)

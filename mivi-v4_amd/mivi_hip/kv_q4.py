@@ -19,6 +19,16 @@ _attention = _lib.mivi_hip_kv_q4_attention
 _workspace = _lib.mivi_hip_kv_q4_attention_workspace
 
 
+def _load():
+    """torch, and its types' ids."""
+    global torch
+    if torch is None:
+        import torch as t
+        _TYPES.update({t.float32: 0, t.float16: 1, t.bfloat16: 30})
+        torch = t
+    return torch
+
+
 def kv_q4_page_bytes(n_kv_heads: int, head_dim: int, page_tokens: int) -> int:
     """Bytes of a page (0: no such geometry)."""
     return int(_lib.mivi_hip_kv_q4_page_bytes(n_kv_heads, head_dim, page_tokens))
@@ -31,11 +41,7 @@ class KvCacheQ4:
     `set_pages`). Both stay the caller's."""
 
     def __init__(self, data, pages, n_kv_heads: int, head_dim: int, page_tokens: int):
-        global torch
-        if torch is None:
-            import torch as t
-            _TYPES.update({t.float32: 0, t.float16: 1, t.bfloat16: 30})
-            torch = t
+        _load()
         if data.dtype != torch.uint8 or not data.is_contiguous() or not data.is_cuda:
             raise ValueError("data is a contiguous u8 GPU tensor")
         self.data, self.n_kv_heads, self.head_dim, self.page_tokens = data, n_kv_heads, head_dim, page_tokens
@@ -89,7 +95,7 @@ def _call(fn, args, device, stream):
         raw = stream
     else:
         if stream.device != device:
-            raise ValueError("the stream is on another device than the cache")
+            raise ValueError("the stream is on another device than the tensors")
         raw = stream.cuda_stream
     if torch._C._cuda_getDevice() == device.index:
         rc = fn(*args, raw)

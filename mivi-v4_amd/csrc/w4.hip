@@ -38,14 +38,15 @@ typedef uint32_t u32_a1 __attribute__((aligned(1)));
 
 constexpr int kWaves = 8;
 constexpr int kStep = 128;   // columns of a step
-constexpr int kRing = 4;     // steps of a wave in flight
-constexpr size_t kLds = 64 * 1024;
+constexpr int kRing = 3;     // steps of a wave in flight (w4_rows_kernel)
+constexpr int kItems = 8;    // pieces of x a thread stages, half of them of f32
+constexpr size_t kLds = 128 * 1024, kLdsFew = 156 * 1024;
 
 enum XKind { X_F16, X_BF16, X_F32, X_I8 };
 constexpr int parts_of(int x) { return x == X_F32 ? 3 : 1; }
 
 struct W4Args {
-    const uint8_t *codes, *scales, *zeros;  // planes of the packed weights; zeros: or null
+    const uint8_t *codes, *scales, *zeros;  // planes of the packed weights (zeros: the codes where there are none)
     const void* x;
     const float* x_scales;
     void* out;
@@ -53,10 +54,9 @@ struct W4Args {
     int rows, cols, batch, tiles, steps;
     int block;      // inputs of a workgroup
     int wk;         // waves of a tile
-    int phase;      // steps of x in LDS: all, or a multiple of wk times kRing
     int w_units;    // units of a step that have a scale of their own
     int x_shift, x_groups;  // 8-bit x: log2 of a scale's columns, scales of a row; -1, 1: a row has one
-    int bf16_scales, out_type;
+    int bf16_scales, has_zeros, out_type;
 };
 
 __device__ __forceinline__ float scale_f32(uint32_t bits, bool bf16) {
@@ -77,16 +77,28 @@ __device__ __forceinline__ half8 weights_f16(uint32_t w, uint32_t z) {
     r.h[3] = __builtin_elementwise_fma(__builtin_bit_cast(half2v, (w8 & 0x00F000F0u) | 0x64006400u), sixteenth, hi);
     return r.v;
 }
+// Byte K of w as a float; the compiler takes a nibble out first, two instructions.
+template <int K>
+__device__ __forceinline__ float byte_f32(uint32_t w) {
+    float f;
+    if constexpr (K == 0) asm("v_cvt_f32_ubyte0 %0, %1" : "=v"(f) : "v"(w));
+    else if constexpr (K == 1) asm("v_cvt_f32_ubyte1 %0, %1" : "=v"(f) : "v"(w));
+    else if constexpr (K == 2) asm("v_cvt_f32_ubyte2 %0, %1" : "=v"(f) : "v"(w));
+    else asm("v_cvt_f32_ubyte3 %0, %1" : "=v"(f) : "v"(w));
+    return f;
+}
 __device__ __forceinline__ bf16x8 weights_bf16(uint32_t w, float z) {
     const uint32_t even = w & 0x0F0F0F0Fu, odd = w >> 4 & 0x0F0F0F0Fu;
     union { bf16x8 v; uint32_t u[4]; } r;
-#pragma unroll
-    for (int p = 0; p < 4; p++) {  // integers up to 15: the upper halves of the floats are exact
-        const uint32_t pairs = p % 2 ? odd : even;  // columns 2 p and 2 p + 1: bytes p / 2 and 2 + p / 2
-        const uint32_t a = __float_as_uint(ubyte_f32(pairs, p / 2) - z);
-        const uint32_t b = __float_as_uint(ubyte_f32(pairs, 2 + p / 2) - z);
-        r.u[p] = __builtin_amdgcn_perm(b, a, 0x07060302);
-    }
+    // columns 2 p and 2 p + 1 are bytes p / 2 and 2 + p / 2 of even or odd;
+    // integers up to 15: the upper halves of the floats are exact
+    const auto pair = [&](float a, float b) {
+        return __builtin_amdgcn_perm(__float_as_uint(b - z), __float_as_uint(a - z), 0x07060302);
+    };
+    r.u[0] = pair(byte_f32<0>(even), byte_f32<2>(even));
+    r.u[1] = pair(byte_f32<0>(odd), byte_f32<2>(odd));
+    r.u[2] = pair(byte_f32<1>(even), byte_f32<3>(even));
+    r.u[3] = pair(byte_f32<1>(odd), byte_f32<3>(odd));
     return r.v;
 }
 // In the order 0 4 1 5 2 6 3 7 of the columns, in which x is laid out too.
@@ -97,160 +109,155 @@ __device__ __forceinline__ long weights_i8(uint32_t w, uint32_t zzzz) {
     return (long)((uint64_t)b << 32 | a);
 }
 
-// x of `count` inputs and the phase's columns to LDS.
-template <int X, int U>
-__device__ __forceinline__ void stage(const W4Args& a, uint8_t* lds, int b0, int count, int cols_x, int k0, int kn) {
-    const int n8 = kn / 8;
-    if constexpr (X == X_I8) {  // and the scales of a step's sums, behind the codes
-        if (a.x_shift >= 0) {
-            float* xs = (float*)(lds + a.phase * 16 * cols_x * 8);
-            const int n = kn / kStep * U;
-            for (int i = threadIdx.x; i < count * n; i += kWaves * 64) {
-                const int b = i / n, u = i % n, k = min(k0 + u * (kStep / U), a.cols - 1);
-                xs[u * cols_x + b] = a.x_scales[(int64_t)(b0 + b) * a.x_groups + (k >> a.x_shift)];
-            }
+// A scale's four rows of a unit, as the f32 factors of a lane's four results.
+__device__ __forceinline__ void scales_f32(u32x2 s, bool bf16, float (&f)[4]) {
+    f[0] = scale_f32(s.x & 0xFFFF, bf16), f[1] = scale_f32(s.x >> 16, bf16);
+    f[2] = scale_f32(s.y & 0xFFFF, bf16), f[3] = scale_f32(s.y >> 16, bf16);
+}
+
+// What a lane holds of a step: a row's codes, the scales of its results' rows,
+// and zeros: where ROW of its own row (a byte a unit), else of those of its
+// results (bytes [row 4 q + i][unit]).
+template <int W, bool ROW>
+struct Step {
+    u32x4 codes;
+    u32x2 scales[W];
+    uint32_t zeros[ROW ? 1 : W];
+};
+
+// Loads without a branch: of weights without zeros the codes stand in for them.
+template <int W, bool ROW>
+__device__ __forceinline__ void fetch(const W4Args& a, int64_t st, int lane, Step<W, ROW>* o) {
+    o->codes = *(const u32x4*)(a.codes + st * 1024 + lane * 16);
+    const int q = lane >> 4;
+    const uint8_t* s = a.scales + st * (32 * W) + q * (8 * W);
+    if constexpr (W == 1) {
+        o->scales[0] = *(const u32x2*)s;
+    } else {
+#pragma unroll
+        for (int u = 0; u < W; u += 2) {
+            const u32x4 v = *(const u32x4*)(s + u * 8);
+            o->scales[u] = u32x2{v.x, v.y}, o->scales[u + 1] = u32x2{v.z, v.w};
         }
     }
-    for (int i = threadIdx.x; i < count * n8; i += kWaves * 64) {
-        const int b = i / n8, c = i % n8, k = k0 + c * 8;
-        const int64_t at = (int64_t)(b0 + b) * a.x_row + k;
-        const bool in = k < a.cols;
-        if constexpr (X == X_I8) {
-            u32x2 v = {0, 0};
-            if (in) v = *(const u32x2_a1*)((const int8_t*)a.x + at);
-            *(u32x2*)(lds + ((int64_t)c * cols_x + b) * 8) =
-                u32x2{__builtin_amdgcn_perm(v.y, v.x, 0x05010400), __builtin_amdgcn_perm(v.y, v.x, 0x07030602)};
-        } else if constexpr (X == X_F32) {
-            float v[8];
-            load_row8<MIVI_GGML_F32>(a.x, at, in ? 8 : 0, v);
-            bf16x8 p[3];
+    const uint8_t* z = a.zeros + st * (16 * W);
+    if constexpr (ROW) {
+        const int r = lane & 15;
+        uint32_t v;
+        if constexpr (W == 4) v = ((const uint32_t*)z)[r];
+        else if constexpr (W == 2) v = ((const uint16_t*)z)[r];
+        else v = z[r];
+        o->zeros[0] = a.has_zeros ? v : 0x08080808u;
+    } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                __bf16 p0, p1, p2;
-                split_bf16(v[e], p0, p1, p2);
-                p[0][e] = p0, p[1][e] = p1, p[2][e] = p2;
-            }
-#pragma unroll
-            for (int j = 0; j < 3; j++) *(bf16x8*)(lds + ((int64_t)c * cols_x + 3 * b + j) * 16) = p[j];
-        } else {
-            u32x4 v = {0, 0, 0, 0};
-            if (in) v = *(const u32x4_a1*)((const uint16_t*)a.x + at);
-            *(u32x4*)(lds + ((int64_t)c * cols_x + b) * 16) = v;
+        for (int u = 0; u < W; u++) {
+            const uint32_t v = ((const uint32_t*)(z + q * (4 * W)))[u];
+            o->zeros[u] = a.has_zeros ? v : 0x08080808u;
         }
     }
 }
 
-// U: sums of a step that are scaled by themselves; NT: tiles of 16 columns.
-template <int X, int U, int NT>
-__global__ __launch_bounds__(kWaves * 64) void w4_kernel(W4Args a) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    constexpr int XB = X == X_I8 ? 8 : 16, PARTS = parts_of(X), PER = 4 / U;
-    typedef typename std::conditional<X == X_I8, i32x4, f32x4>::type D;
-    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave % a.wk, wm = wave / a.wk;
-    const int wms = kWaves / a.wk, tile = blockIdx.x * wms + wm;
-    const bool live = tile < a.tiles;
-    const int b0 = blockIdx.y * a.block, count = min(a.block, a.batch - b0), cols_x = count * PARTS;
-    int col[NT];  // columns behind the last repeat it: their results are not used
-#pragma unroll
-    for (int n = 0; n < NT; n++) col[n] = min(16 * n + r, cols_x - 1);
-    const float* xs = (const float*)(lds + a.phase * 16 * cols_x * 8);
-    const int64_t first = (int64_t)(live ? tile : 0) * a.steps;
-    const int mine = live ? max(0, (a.steps - wk + a.wk - 1) / a.wk) : 0;  // steps of this wave
+// An operand of x: 8 columns of one input, 16 bytes or 8.
+template <int X>
+struct Operand { u32x4 v; };
+template <>
+struct Operand<X_I8> { u32x2 v; };
 
-    u32x4 codes[kRing];
-    u32x2 sc[kRing][U];
-    uint32_t zc[kRing][U];
-    const auto fetch = [&](int slot, int i) {
-        const int64_t st = first + wk + i * a.wk;
-        codes[slot] = *(const u32x4*)(a.codes + st * 1024 + lane * 16);
-        const uint8_t* s = a.scales + (st * 4 + q) * a.w_units * 8;
-#pragma unroll
-        for (int u = 0; u < U; u++) sc[slot][u] = *(const u32x2*)(s + u * a.w_units / U * 8);
-        const uint8_t* z = a.zeros + (st * 16 + r) * a.w_units;
-#pragma unroll
-        for (int u = 0; u < U; u++) zc[slot][u] = a.zeros ? z[u * a.w_units / U] & 15 : 8;
-    };
-    f32x4 acc[NT];
-#pragma unroll
-    for (int n = 0; n < NT; n++) acc[n] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int p = 0; p < kRing; p++)
-        if (p < mine) fetch(p, p);
-
-    const auto compute = [&](int slot, int local) {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            D d[NT];
-#pragma unroll
-            for (int n = 0; n < NT; n++) d[n] = D{0, 0, 0, 0};
-#pragma unroll
-            for (int p = 0; p < PER; p++) {
-                const int j = u * PER + p;
-                const uint8_t* xl = lds + (local * 16 + j * 4 + q) * cols_x * XB;
-                const uint32_t w = codes[slot][j], z = zc[slot][u];
-                if constexpr (X == X_F16) {
-                    const half8 wv = weights_f16(w, z);
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-                        d[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv, *(const half8*)(xl + col[n] * XB), d[n], 0, 0, 0);
-                } else if constexpr (X == X_I8) {
-                    const long wv = weights_i8(w, z * 0x01010101u);
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-                        d[n] = __builtin_amdgcn_mfma_i32_16x16x32_i8(wv, *(const long*)(xl + col[n] * XB), d[n], 0, 0, 0);
-                } else {
-                    const bf16x8 wv = weights_bf16(w, (float)z);
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-                        d[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, *(const bf16x8*)(xl + col[n] * XB), d[n], 0, 0, 0);
-                }
-            }
-            const u32x2 s = sc[slot][u];
-            const float f[4] = {scale_f32(s.x & 0xFFFF, a.bf16_scales), scale_f32(s.x >> 16, a.bf16_scales),
-                                scale_f32(s.y & 0xFFFF, a.bf16_scales), scale_f32(s.y >> 16, a.bf16_scales)};
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                float m = 1.f;
-                if constexpr (X == X_I8) {
-                    if (a.x_shift >= 0) m = xs[(local * U + u) * cols_x + col[n]];
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) acc[n][i] = fmaf((float)d[n][i], X == X_I8 ? f[i] * m : f[i], acc[n][i]);
-            }
-        }
-    };
-
-    const int per_phase = a.phase / a.wk;
-    for (int ph = 0; ph * a.phase < a.steps; ph++) {
-        if (ph) __syncthreads();
-        stage<X, U>(a, lds, b0, count, cols_x, ph * a.phase * kStep, min(a.phase, a.steps - ph * a.phase) * kStep);
-        __syncthreads();
-        const int end = min(mine, (ph + 1) * per_phase);
-        for (int i = ph * per_phase; i < end; i += kRing) {
-#pragma unroll
-            for (int p = 0; p < kRing; p++) {
-                if (i + p < end) {
-                    compute(p, wk + (i + p) * a.wk - ph * a.phase);
-                    if (i + p + kRing < mine) fetch(p, i + p + kRing);
-                }
-            }
-        }
+// A dword's weights as an operand, and a product of 16 rows and 16 columns, 32
+// deep.
+template <int X>
+struct Weights8 {
+    u32x4 v;
+    __device__ __forceinline__ Weights8(uint32_t w, uint32_t z) {
+        if constexpr (X == X_F16) v = __builtin_bit_cast(u32x4, weights_f16(w, z));
+        else v = __builtin_bit_cast(u32x4, weights_bf16(w, (float)z));
     }
+    __device__ __forceinline__ f32x4 times(const Operand<X>& x, f32x4 d) const {
+        if constexpr (X == X_F16)
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, v), __builtin_bit_cast(half8, x.v), d, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, x.v), d, 0, 0, 0);
+    }
+};
+template <>
+struct Weights8<X_I8> {
+    long v;
+    __device__ __forceinline__ Weights8(uint32_t w, uint32_t z) { v = weights_i8(w, z * 0x01010101u); }
+    __device__ __forceinline__ i32x4 times(const Operand<X_I8>& x, i32x4 d) const {
+        return __builtin_amdgcn_mfma_i32_16x16x32_i8(v, __builtin_bit_cast(long, x.v), d, 0, 0, 0);
+    }
+};
 
-    // join the waves of a tile and the parts of an input
-    __syncthreads();
-    float* red = (float*)lds;
+// x as it lies in memory: 8 columns from k on of input b, or the last 8 where
+// there are none (then `blank` makes zeros of them).
+template <int X>
+struct Raw { u32x4 v[X == X_F32 ? 2 : 1]; };
+template <>
+struct Raw<X_I8> { u32x2 v[1]; };
+
+template <int X>
+__device__ __forceinline__ Raw<X> load_x(const W4Args& a, int b, int k) {
+    Raw<X> r;
+    const int64_t at = (int64_t)b * a.x_row + min(k, a.cols - 8);
+    if constexpr (X == X_I8) {
+        r.v[0] = *(const u32x2_a1*)((const int8_t*)a.x + at);
+    } else if constexpr (X == X_F32) {
+        r.v[0] = *(const u32x4_a1*)((const float*)a.x + at);
+        r.v[1] = *(const u32x4_a1*)((const float*)a.x + at + 4);
+    } else {
+        r.v[0] = *(const u32x4_a1*)((const uint16_t*)a.x + at);
+    }
+    return r;
+}
+template <int X>
+__device__ __forceinline__ void blank(Raw<X>* r, bool in) {
 #pragma unroll
-    for (int n = 0; n < NT; n++) *(f32x4*)(red + ((wave * NT + n) * 16 + r) * 16 + q * 4) = acc[n];
-    __syncthreads();
-    for (int i = tid; i < wms * count * 16; i += kWaves * 64) {
-        const int m = i & 15, b = (i >> 4) % count, w = (i >> 4) / count;
-        const int row = (blockIdx.x * wms + w) * 16 + m;
+    for (int i = 0; i < (X == X_F32 ? 2 : 1); i++)
+#pragma unroll
+        for (int j = 0; j < (X == X_I8 ? 2 : 4); j++) r->v[i][j] = in ? r->v[i][j] : 0u;
+}
+
+// Its operands, one a part.
+template <int X>
+__device__ __forceinline__ void operands(const Raw<X>& r, Operand<X> (&o)[parts_of(X)]) {
+    if constexpr (X == X_I8) {
+        o[0].v = u32x2{__builtin_amdgcn_perm(r.v[0].y, r.v[0].x, 0x05010400),
+                       __builtin_amdgcn_perm(r.v[0].y, r.v[0].x, 0x07030602)};
+    } else if constexpr (X == X_F32) {
+        bf16x8 p[3];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            __bf16 p0, p1, p2;
+            split_bf16(__uint_as_float(r.v[e / 4][e % 4]), p0, p1, p2);
+            p[0][e] = p0, p[1][e] = p1, p[2][e] = p2;
+        }
+#pragma unroll
+        for (int j = 0; j < 3; j++) o[j].v = __builtin_bit_cast(u32x4, p[j]);
+    } else {
+        o[0].v = r.v[0];
+    }
+}
+
+// The scale of 8-bit input b's unit u of a step.
+template <int U>
+__device__ __forceinline__ float x_scale(const W4Args& a, int b, int step, int u) {
+    const int k = min(step * kStep + u * (kStep / U), a.cols - 1);
+    return a.x_scales[(int64_t)b * a.x_groups + (k >> a.x_shift)];
+}
+
+// Joins the waves of a tile and the parts of an input, and stores: red holds
+// [wave][column][16 rows].
+template <int X, int PARTS>
+__device__ __forceinline__ void store_tiles(const W4Args& a, const float* red, int first_tile, int tiles, int b0,
+                                            int count, int columns) {
+    for (int i = threadIdx.x; i < tiles * count * 16; i += blockDim.x) {
+        const int m = i & 15, t = (i >> 4) / count, b = (i >> 4) - t * count;
+        const int row = (first_tile + t) * 16 + m;
         if (row >= a.rows) continue;
         float v = 0;
+#pragma unroll
         for (int p = PARTS - 1; p >= 0; p--)
-            for (int k = 0; k < a.wk; k++) v += red[((w * a.wk + k) * NT * 16 + b * PARTS + p) * 16 + m];
+            for (int k = 0; k < a.wk; k++) v += red[((t * a.wk + k) * columns + b * PARTS + p) * 16 + m];
         if constexpr (X == X_I8) {
             if (a.x_shift < 0) v *= a.x_scales[b0 + b];
         }
@@ -259,6 +266,341 @@ __global__ __launch_bounds__(kWaves * 64) void w4_kernel(W4Args a) {
         else if (a.out_type == MIVI_GGML_F16) store_elem<MIVI_GGML_F16>(a.out, o, v);
         else store_elem<MIVI_GGML_BF16>(a.out, o, v);
     }
+}
+
+// --------------------------------------------------------------- few inputs
+// Up to 16 columns of the product. The weights enter as fp16 numbers c 2^-24
+// and, from the nibbles above, 16 c 2^-24: masks alone, where 1 + c / 16 or c - z
+// would take two to four times the instructions; x against the latter is held
+// as a sixteenth. x is held in fp16, each step's 128 columns multiplied by the
+// power of two that takes their largest to 2^14 .. 2^15 (f32 in two parts, 22
+// bits; nothing to less than 2^-36 of that largest). The zeros come out of the
+// results, d - z sum x, where both are at most four times what the weights'
+// values would give.
+constexpr int few_parts(int x) { return x == X_F32 ? 2 : 1; }
+constexpr int kFewRing = 4;  // steps of a wave in flight
+
+struct FewArgs {
+    W4Args w;
+    int n;                         // steps of a wave
+    int pitch, sums, red;          // bytes of LDS: of 8 columns; before the sums of x; before the results
+};
+
+// Largest magnitude's bits over 16 lanes; sums over 16, 8 or 4.
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+    const auto f = [](uint32_t x) { return __uint_as_float(x); };
+    const auto u = [](float x) { return __float_as_uint(x); };
+    v = max(v, u(dpp_mov<0xB1>(f(v))));
+    v = max(v, u(dpp_mov<0x4E>(f(v))));
+    v = max(v, u(xor4_mov(f(v))));
+    return max(v, u(dpp_mov<0x128>(f(v))));
+}
+template <int U>
+__device__ __forceinline__ float unit_sum(float v) {
+    v += dpp_mov<0xB1>(v);
+    v += dpp_mov<0x4E>(v);
+    if (U <= 2) v += xor4_mov(v);
+    if (U <= 1) v += dpp_mov<0x128>(v);
+    return v;
+}
+
+// 8 columns of an input as operands, the sums of their units times 2^-24, and
+// what the step's results are to be multiplied by (2^24 aside).
+template <int X, int U>
+__device__ __forceinline__ void few_operands(const Raw<X>& r, Operand<X_F16> (&o)[few_parts(X)], float (&sum)[few_parts(X)],
+                                             float* factor) {
+    float v[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        if constexpr (X == X_F32) v[e] = __uint_as_float(r.v[e / 4][e % 4]);
+        else if constexpr (X == X_F16) v[e] = half_bits_to_f32(r.v[0][e / 2] >> (e % 2 * 16));
+        else v[e] = bf16_bits_to_f32(r.v[0][e / 2] >> (e % 2 * 16));
+        top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    }
+    // biased exponents: 2^(14 - e) for a largest value of 2^e, 2^126 at most
+    const int ex = min(127 + 14 - ((int)(max16(top) >> 23) - 127), 253);
+    const float up = __uint_as_float((uint32_t)ex << 23), up16 = __uint_as_float((uint32_t)(ex - 4) << 23);
+    *factor = __uint_as_float((uint32_t)(254 - ex) << 23);
+    half8 h[few_parts(X)];
+#pragma unroll
+    for (int p = 0; p < few_parts(X); p++) sum[p] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const bool sixteenth = e / 2 % 2;
+        float y = v[e] * (sixteenth ? up16 : up);
+#pragma unroll
+        for (int p = 0; p < few_parts(X); p++) {
+            const _Float16 part = (_Float16)y;
+            h[p][e] = part;
+            sum[p] = fmaf((float)part, sixteenth ? 0x1p-20f : 0x1p-24f, sum[p]);
+            // what an infinity leaves is nothing
+            y = p == 0 && __builtin_fabsf(y) == __builtin_inff() ? 0.f : y - (float)part;
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < few_parts(X); p++) {
+        o[p].v = __builtin_bit_cast(u32x4, h[p]);
+        sum[p] = unit_sum<U>(sum[p]);
+    }
+}
+
+template <int X, int U, int W, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    constexpr bool I8 = X == X_I8;
+    constexpr int PARTS = few_parts(X), PER = 4 / U, XB = I8 ? 8 : 16;
+    typedef typename std::conditional<I8, i32x4, f32x4>::type D;
+    const W4Args& a = g.w;
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave % a.wk, wm = wave / a.wk;
+    const int wms = WAVES / a.wk, stride = gridDim.x * wms, cols_x = a.batch * PARTS, col = min(r, cols_x - 1);
+    float* sums = (float*)(lds + g.sums);                    // [step][unit][column]: z times which comes off
+    float* factors = sums + a.steps * U * cols_x;            // [step][column], of 8-bit x [step][unit][column]
+
+    Step<W, false> w[kFewRing];
+    int tile = blockIdx.x * wms + wm, next_tile = tile, next = 0;  // of the next fetch
+    const auto refill = [&](int slot) {
+        // behind the last step and tile those are loaded again
+        fetch<W, false>(a, (int64_t)min(next_tile, a.tiles - 1) * a.steps + min(wk + next * a.wk, a.steps - 1), lane, &w[slot]);
+        if (++next == g.n) next = 0, next_tile += stride;
+    };
+#pragma unroll
+    for (int p = 0; p < kFewRing; p++) refill(p);
+
+    // x to LDS, four pieces of 8 columns of a thread's on their way at once
+    const int n8 = a.steps * 16, items = a.batch * n8;
+    for (int base = 0; base < items; base += 4 * WAVES * 64) {
+        Raw<X> raw[4];
+        int at[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int i = min(base + e * WAVES * 64 + tid, items - 1), b = i / n8, c = i - b * n8;
+            at[e] = base + e * WAVES * 64 + tid < items ? c << 4 | b : -1;
+            raw[e] = load_x<X>(a, b, c * 8);
+            blank<X>(&raw[e], c * 8 < a.cols);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (base + e * WAVES * 64 >= items) break;
+            const int c = at[e] >> 4, b = at[e] & 15;
+            uint8_t* to = lds + c * g.pitch + b * PARTS * XB;
+            const int unit = (c >> 4) * U + (c & 15) / (16 / U);
+            const bool head = at[e] >= 0 && (c & (16 / U - 1)) == 0;
+            if constexpr (I8) {
+                Operand<X> o[1];
+                operands<X>(raw[e], o);
+                int s = __builtin_amdgcn_sdot4((int)o[0].v.x, 0x01010101, 0, false);
+                s = __builtin_amdgcn_sdot4((int)o[0].v.y, 0x01010101, s, false);
+                const float sum = unit_sum<U>((float)s);  // whole numbers far below 2^24
+                if (at[e] >= 0) *(Operand<X>*)to = o[0];
+                if (head) {
+                    ((int*)sums)[unit * cols_x + b] = (int)sum;
+                    factors[unit * cols_x + b] = a.x_shift < 0 ? 1.f : x_scale<U>(a, b, c >> 4, unit & (U - 1));
+                }
+            } else {
+                Operand<X_F16> o[PARTS];
+                float sum[PARTS], factor;
+                few_operands<X, U>(raw[e], o, sum, &factor);
+#pragma unroll
+                for (int p = 0; p < PARTS; p++) {
+                    if (at[e] >= 0) *(Operand<X_F16>*)(to + p * XB) = o[p];
+                    if (head) sums[unit * cols_x + b * PARTS + p] = sum[p];
+                    if (at[e] >= 0 && (c & 15) == 0) factors[(c >> 4) * cols_x + b * PARTS + p] = factor;
+                }
+            }
+        }
+    }
+    __syncthreads();
+
+    f32x4 acc = {0, 0, 0, 0};
+    int s = 0, it = 0, t0 = blockIdx.x * wms;
+    const auto compute = [&](const Step<W, false>& c, int step) {
+        const uint8_t* xl = lds + (step * 16 + q) * g.pitch + col * XB;
+        f32x4 part = {0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            constexpr int per_w = U / W;
+            D d = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < PER; k++) {
+                const int j = u * PER + k;
+                const uint32_t wd = c.codes[j];
+                if constexpr (I8) {
+                    const uint32_t even = wd & 0x0F0F0F0Fu, odd = wd >> 4 & 0x0F0F0F0Fu;
+                    const long wv = (long)((uint64_t)odd << 32 | even);
+                    d = __builtin_amdgcn_mfma_i32_16x16x32_i8(wv, *(const long*)(xl + j * 4 * g.pitch), d, 0, 0, 0);
+                } else {
+                    const uint32_t w8 = wd >> 8;
+                    const u32x4 wv = {wd & 0x000F000Fu, wd & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u};
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, wv),
+                                                               *(const half8*)(xl + j * 4 * g.pitch), d, 0, 0, 0);
+                }
+            }
+            float f[4];
+            scales_f32(c.scales[u / per_w], a.bf16_scales, f);
+            const int at = (step * U + u) * cols_x + col;
+            const float m = I8 ? factors[at] : 1.f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int byte = i * W + u / per_w;
+                const uint32_t z = c.zeros[byte / 4] >> (byte % 4 * 8) & 0xFF;
+                if constexpr (I8) acc[i] = fmaf((float)(d[i] - (int)z * ((const int*)sums)[at]), f[i] * m, acc[i]);
+                else part[i] = fmaf(fmaf(-(float)z, sums[at], d[i]), f[i], part[i]);
+            }
+        }
+        if constexpr (!I8) {
+            const float m = factors[step * cols_x + col] * 0x1p24f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] = fmaf(part[i], m, acc[i]);
+        }
+    };
+    while (t0 < a.tiles) {
+#pragma unroll
+        for (int p = 0; p < kFewRing; p++) {
+            if (t0 >= a.tiles) break;
+            const int step = wk + s * a.wk;
+            if (tile < a.tiles && step < a.steps) compute(w[p], step);
+            refill(p);
+            if (++s == g.n) {
+                float* red = (float*)(lds + g.red) + it * (WAVES * 256);
+                *(f32x4*)(red + (wave * 16 + r) * 16 + q * 4) = acc;
+                __syncthreads();
+                store_tiles<X, PARTS>(a, red, t0, min(wms, a.tiles - t0), 0, a.batch, 16);
+                acc = f32x4{0, 0, 0, 0};
+                s = 0, it ^= 1, t0 += stride, tile += stride;
+            }
+        }
+    }
+}
+
+// More inputs, or deeper rows: NT tiles of 16 columns; x goes through LDS, wk
+// steps of it at a time in two buffers, [32 columns][q][column of the product],
+// loaded a phase ahead into registers.
+template <int X, int U, int W, int NT>
+__global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    constexpr int XB = X == X_I8 ? 8 : 16, PARTS = parts_of(X), PER = 4 / U;
+    constexpr int ITEMS = X == X_F32 ? kItems / 2 : kItems;
+    typedef typename std::conditional<X == X_I8, i32x4, f32x4>::type D;
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave % a.wk, wm = wave / a.wk;
+    const int wms = kWaves / a.wk, tile = blockIdx.x * wms + wm;
+    const bool live = tile < a.tiles;
+    const int b0 = blockIdx.y * a.block, count = min(a.block, a.batch - b0), cols_x = count * PARTS;
+    int col[NT];  // columns behind the last repeat it: their results are not used
+#pragma unroll
+    for (int n = 0; n < NT; n++) col[n] = min(16 * n + r, cols_x - 1) * XB;
+    const int pitch = cols_x * XB + 16;  // 16 bytes over: a wave's stores of x take every bank in turn
+    const int xs_at = a.wk * 16 * pitch;  // 8-bit x: its scales behind the codes
+    const int buffer = (xs_at + (X == X_I8 ? a.wk * cols_x * 4 * U : 0) + 15) / 16 * 16;
+    // a thread stages 8 columns of every (threads / pieces of an input)-th input
+    const int n8 = a.wk * 16, c8 = tid & (n8 - 1), bx = tid / n8, b_step = kWaves * 64 / n8;
+    const int phases = (a.steps + a.wk - 1) / a.wk;
+    const int64_t first = (int64_t)(live ? tile : 0) * a.steps;
+
+    Raw<X> raw[ITEMS];
+    float xs_raw[2];  // 8-bit x: scales of (inputs x units); count wk <= 16 kItems kWaves / 4, so two a thread do
+    const int nu = a.wk * U;
+    const auto load = [&](int ph) {
+        if constexpr (X == X_I8) {
+            if (a.x_shift >= 0) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int i = tid + e * kWaves * 64, u = i & (nu - 1);
+                    xs_raw[e] = x_scale<U>(a, b0 + min(i / nu, count - 1), ph * a.wk + u / U, u % U);
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < ITEMS; e++) {
+            const int b = bx + e * b_step;
+            if (e * b_step < count) raw[e] = load_x<X>(a, b0 + min(b, count - 1), ph * a.wk * kStep + c8 * 8);
+        }
+    };
+    const auto store = [&](int ph) {
+        uint8_t* to = lds + (ph & 1) * buffer;
+#pragma unroll
+        for (int e = 0; e < ITEMS; e++) {
+            const int b = bx + e * b_step;
+            if (b < count) {
+                blank<X>(&raw[e], (ph * a.wk * 16 + c8) * 8 < a.cols);
+                Operand<X> o[PARTS];
+                operands<X>(raw[e], o);
+#pragma unroll
+                for (int p = 0; p < PARTS; p++) *(Operand<X>*)(to + c8 * pitch + (b * PARTS + p) * XB) = o[p];
+            }
+        }
+        if constexpr (X == X_I8) {
+            if (a.x_shift >= 0) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int i = tid + e * kWaves * 64, b = i / nu;
+                    if (b < count) ((float*)(to + xs_at))[(i & (nu - 1)) * cols_x + b] = xs_raw[e];
+                }
+            }
+        }
+    };
+
+    f32x4 acc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) acc[n] = f32x4{0, 0, 0, 0};
+    Step<W, true> w[kRing];
+    load(0);
+    const auto refill = [&](int slot, int ph) {  // behind the last step it is loaded again
+        fetch<W, true>(a, first + min(wk + ph * a.wk, a.steps - 1), lane, &w[slot]);
+    };
+#pragma unroll
+    for (int p = 0; p < kRing; p++) refill(p, p);
+    store(0);
+
+    for (int base = 0; base < phases; base += kRing) {
+#pragma unroll
+        for (int p = 0; p < kRing; p++) {
+            const int ph = base + p;
+            if (ph >= phases) break;
+            __syncthreads();  // this phase's x is there, the phase before is read
+            if (ph + 1 < phases) load(ph + 1);
+            if (live && wk + ph * a.wk < a.steps) {
+                const Step<W, true>& c = w[p];
+                const uint8_t* xl = lds + (ph & 1) * buffer + (wk * 16 + q) * pitch;
+                const float* xs = (const float*)(lds + (ph & 1) * buffer + xs_at) + wk * U * cols_x;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    D d[NT];
+#pragma unroll
+                    for (int n = 0; n < NT; n++) d[n] = D{0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < PER; k++) {
+                        const int j = u * PER + k;
+                        const Weights8<X> wv(c.codes[j], c.zeros[0] >> (8 * (u / (U / W))) & 15);
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+                            d[n] = wv.times(*(const Operand<X>*)(xl + j * 4 * pitch + col[n]), d[n]);
+                    }
+                    float f[4];
+                    scales_f32(c.scales[u / (U / W)], a.bf16_scales, f);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        float m = 1.f;
+                        if constexpr (X == X_I8) {
+                            if (a.x_shift >= 0) m = xs[u * cols_x + col[n] / XB];
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[n][i] = fmaf((float)d[n][i], X == X_I8 ? f[i] * m : f[i], acc[n][i]);
+                    }
+                }
+            }
+            refill(p, ph + kRing);
+            if (ph + 1 < phases) store(ph + 1);
+        }
+    }
+    __syncthreads();
+    float* red = (float*)lds;
+#pragma unroll
+    for (int n = 0; n < NT; n++) *(f32x4*)(red + ((wave * NT + n) * 16 + r) * 16 + q * 4) = acc[n];
+    __syncthreads();
+    store_tiles<X, PARTS>(a, red, blockIdx.x * wms, min(wms, a.tiles - (int)blockIdx.x * wms), b0, count, 16 * NT);
 }
 
 // ------------------------------------------------------------------ packing
@@ -321,21 +663,94 @@ int32_t packed_of(size_t rows, size_t cols, size_t group, bool zeros, Packed* p)
     return MIVI_OK;
 }
 
-template <int X, int U, int NT>
-void launch_w4(const W4Args& a, dim3 grid, size_t lds, hipStream_t s) {
-    w4_kernel<X, U, NT><<<grid, kWaves * 64, lds, s>>>(a);
+// How a product is laid out: w4_few_kernel, or w4_rows_kernel with nt tiles of
+// columns.
+struct W4Plan {
+    bool few;
+    int nt, waves;
+    dim3 grid;
+    size_t lds;
+    FewArgs g;
+};
+
+template <int X, int U, int W>
+void launch_rows(const W4Args& a, const W4Plan& p, hipStream_t s) {
+#define ROWS(N) w4_rows_kernel<X, U, W, N><<<p.grid, kWaves * 64, p.lds, s>>>(a)
+    switch (p.nt) {
+        case 1: ROWS(1); break;
+        case 2: ROWS(2); break;
+        case 3: ROWS(3); break;
+        case 4: ROWS(4); break;
+        case 5: ROWS(5); break;
+        default: ROWS(8); break;
+    }
+#undef ROWS
 }
-template <int X, int U>
-void launch_w4(const W4Args& a, int nt, dim3 grid, size_t lds, hipStream_t s) {
-    if (nt == 1) launch_w4<X, U, 1>(a, grid, lds, s);
-    else if (nt == 2) launch_w4<X, U, 2>(a, grid, lds, s);
-    else launch_w4<X, U, 4>(a, grid, lds, s);
+template <int X, int U, int W>
+void launch_w4(const W4Args& a, W4Plan& p, hipStream_t s) {
+    if (!p.few) return launch_rows<X, U, W>(a, p, s);
+    p.g.w = a;
+    if (p.waves == 8) w4_few_kernel<X, U, W, 8><<<p.grid, 512, p.lds, s>>>(p.g);
+    else w4_few_kernel<X, U, W, 16><<<p.grid, 1024, p.lds, s>>>(p.g);
 }
+// u: sums of a step that are scaled by themselves, w: those that the weights'
+// groups ask for (fewer where 8-bit inputs have the finer scales)
 template <int X>
-void launch_w4(const W4Args& a, int units, int nt, dim3 grid, size_t lds, hipStream_t s) {
-    if (units == 1) launch_w4<X, 1>(a, nt, grid, lds, s);
-    else if (units == 2) launch_w4<X, 2>(a, nt, grid, lds, s);
-    else launch_w4<X, 4>(a, nt, grid, lds, s);
+void launch_w4(const W4Args& a, int u, int w, W4Plan& p, hipStream_t s) {
+    if (u == w) {
+        if (u == 1) launch_w4<X, 1, 1>(a, p, s);
+        else if (u == 2) launch_w4<X, 2, 2>(a, p, s);
+        else launch_w4<X, 4, 4>(a, p, s);
+    } else if constexpr (X == X_I8) {
+        if (u == 2) launch_w4<X, 2, 1>(a, p, s);
+        else if (w == 1) launch_w4<X, 4, 1>(a, p, s);
+        else launch_w4<X, 4, 2>(a, p, s);
+    }
+}
+
+W4Plan w4_plan(W4Args* a, int x, int units, size_t batch, size_t tiles, size_t steps) {
+    W4Plan p = {};
+    const size_t cus = (size_t)num_cus();
+    {
+        const size_t columns = batch * few_parts(x), xb = x == X_I8 ? 8 : 16;
+        // columns of a multiple of 64 bytes would store to the same banks
+        const size_t pitch = columns * xb + (columns * xb % 64 ? 0 : 16);
+        const size_t x_bytes = steps * 16 * pitch, sums = steps * columns * 4 * (units + (x == X_I8 ? units : 1));
+        const size_t red = (x_bytes + sums + 15) / 16 * 16;
+        // 16 waves a CU: two workgroups of 8, or one of 16 where x fills LDS
+        p.waves = red + 2 * 8 * 1024 <= kLdsFew / 2 ? 8 : 16;
+        p.lds = red + 2 * p.waves * 1024;
+        if (columns <= 16 && steps <= 65536 && p.lds <= kLdsFew) {
+            p.few = true;
+            a->wk = 1;
+            while (a->wk < kWaves && (size_t)a->wk < steps && tiles * a->wk < 16 * cus) a->wk *= 2;
+            p.g.n = (int)((steps + a->wk - 1) / a->wk);
+            p.g.pitch = (int)pitch, p.g.sums = (int)x_bytes, p.g.red = (int)red;
+            // workgroups as many as fit the card, with as many tiles each
+            const size_t groups = (tiles * a->wk + p.waves - 1) / p.waves, fit = cus * (16 / p.waves);
+            const size_t rounds = (groups + fit - 1) / fit;
+            p.grid = dim3((unsigned)((groups + rounds - 1) / rounds));
+            a->block = (int)batch;
+            return p;
+        }
+    }
+    const size_t parts = parts_of(x);
+    // even blocks of at most 128 columns
+    const size_t most = 128 / parts, blocks = (batch + most - 1) / most;
+    const size_t block = (batch + blocks - 1) / blocks;
+    p.nt = (int)((block * parts + 15) / 16);
+    if (p.nt > 5) p.nt = 8;
+    const size_t step_bytes = 16 * (block * parts * (x == X_I8 ? 8 : 16) + 16) + (x == X_I8 ? 4 * units * block : 0);
+    const size_t most_items = (x == X_F32 ? kItems / 2 : kItems) * kWaves * 64;
+    a->wk = kWaves;
+    while (a->wk > 1 && (tiles * a->wk * blocks > 16 * cus || 2 * a->wk * step_bytes > kLds ||
+                         block * a->wk * 16 > most_items))
+        a->wk /= 2;
+    a->block = (int)block;
+    const size_t wms = kWaves / a->wk;
+    p.grid = dim3((unsigned)((tiles + wms - 1) / wms), (unsigned)std::min<size_t>(blocks, 65536));
+    p.lds = std::max<size_t>(2 * ((a->wk * step_bytes + 15) / 16 * 16), (size_t)kWaves * p.nt * 1024);
+    return p;
 }
 
 // The part that both products share: x is laid out in `a` already.
@@ -352,36 +767,21 @@ int32_t run_w4(W4Args a, int x, int32_t type, void* out, size_t out_len, size_t 
         return rc;
     if ((uintptr_t)packed % 16) return set_error(MIVI_ERR_INVALID_ARGUMENT, "packed not 16-byte aligned");
     if (batch == 0) return clear_error();
-    const int parts = parts_of(x), xb = x == X_I8 ? 8 : 16;
-    const size_t all = batch * parts;
-    const int nt = all <= 16 ? 1 : all <= 32 ? 2 : 4;
-    const size_t block = std::min<size_t>(batch, 16 * nt / parts), blocks = (batch + block - 1) / block;
     const int units = std::max((int)p.units, x_units);
-    const size_t step_bytes = block * parts * (16 * xb + (x == X_I8 ? 4 * units : 0));
-    // waves of a tile: as many as keep 16 a CU busy, and as x's columns allow
-    a.wk = 8;
-    while (a.wk > 1 && p.tiles * a.wk > 16 * (size_t)num_cus()) a.wk /= 2;
-    size_t phase = (p.steps + a.wk - 1) / a.wk * a.wk;
-    if (phase * step_bytes > kLds) {
-        while (a.wk > 1 && a.wk * kRing * step_bytes > kLds) a.wk /= 2;
-        phase = kLds / (a.wk * kRing * step_bytes) * a.wk * kRing;
-    }
-    a.phase = (int)phase;
-    const size_t wms = kWaves / a.wk, grid_x = (p.tiles + wms - 1) / wms;
-    const size_t lds = std::max<size_t>(a.phase * step_bytes, (size_t)kWaves * nt * 1024);
-    if (!grid_fits(grid_x, kWaves * 64) || blocks > 65535) return err_overflow();
+    W4Plan plan = w4_plan(&a, x, units, batch, p.tiles, p.steps);
+    if (!grid_fits(plan.grid.x, kWaves * 64) || plan.grid.y > 65535) return err_overflow();
     clear_error();
-    a.codes = packed, a.scales = packed + p.codes, a.zeros = zeros ? packed + p.codes + p.scales : nullptr;
+    a.codes = packed, a.scales = packed + p.codes, a.zeros = zeros ? packed + p.codes + p.scales : packed;
+    a.has_zeros = zeros;
     a.out = out, a.out_row = (int64_t)out_row_stride, a.out_type = type;
     a.rows = (int)rows, a.cols = (int)cols, a.batch = (int)batch;
-    a.tiles = (int)p.tiles, a.steps = (int)p.steps, a.block = (int)block;
+    a.tiles = (int)p.tiles, a.steps = (int)p.steps;
     a.w_units = (int)p.units, a.bf16_scales = scale_type == MIVI_GGML_BF16;
-    const dim3 grid((unsigned)grid_x, (unsigned)blocks);
     switch (x) {
-        case X_F16: launch_w4<X_F16>(a, units, nt, grid, lds, s); break;
-        case X_BF16: launch_w4<X_BF16>(a, units, nt, grid, lds, s); break;
-        case X_F32: launch_w4<X_F32>(a, units, nt, grid, lds, s); break;
-        default: launch_w4<X_I8>(a, units, nt, grid, lds, s); break;
+        case X_F16: launch_w4<X_F16>(a, units, (int)p.units, plan, s); break;
+        case X_BF16: launch_w4<X_BF16>(a, units, (int)p.units, plan, s); break;
+        case X_F32: launch_w4<X_F32>(a, units, (int)p.units, plan, s); break;
+        default: launch_w4<X_I8>(a, units, (int)p.units, plan, s); break;
     }
     MIVI_HIP_CHECK(hipGetLastError());
     return MIVI_OK;

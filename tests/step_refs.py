@@ -79,15 +79,28 @@ def w4_dense(codes, scales, zeros):
     return torch.from_numpy(w.reshape(n, -1))
 
 
-def w4_close(out, x, dense):
-    """x in 64 bits. Of cols products (the parts of an f32 input are 24 bits of it)
-    at most 32 are summed by an instruction, four such in a row, then a wave's
-    steps of 128 and eight waves; each sum may be off by a whole step of f32, the
-    scales' products by half of one."""
-    want = x @ dense.T
-    size = x.abs() @ dense.abs().T
+def w4_reach(codes, scales, zeros):
+    """(c + z) |s|: what the two sums that a value's product may be taken from,
+    s (sum c x - z sum x), add up to."""
+    c, s = codes.cpu().numpy(), f64(scales).abs().numpy()
+    n, groups = s.shape
+    w = np.empty((n, 2 * c.shape[1]))
+    w[:, 0::2], w[:, 1::2] = c & 15, c >> 4
+    z = np.full_like(s, 8.0) if zeros is None else (zeros.cpu().numpy() & 15).astype(np.float64)
+    w = (w.reshape(n, groups, -1) + z[..., None]) * s[..., None]
+    return torch.from_numpy(w.reshape(n, -1))
+
+
+def w4_close(out, x, w):
+    """x in 64 bits; w: codes, scales and zeros. An f32 input may enter with 22
+    bits, which are off by 2^-22 of it at most. Of cols products at most 32 are
+    summed by an instruction, four such in a row, then a wave's steps of 128 and
+    eight waves; each sum may be off by a whole step of f32, the factors' products
+    by half of one each."""
+    want = x @ w4_dense(*w).T
+    size = x.abs() @ w4_reach(*w).T
     depth = 32 + 4 + x.shape[1] // 128 + 1 + 8 + 3
-    room = size * (depth * 2 * U + 2 * U)
+    room = size * (depth * 2 * U + 2 * U + 4 * U)
     room = room + (0 if out.dtype == torch.float32 else HALF_STEP[out.dtype]) * (want.abs() + room) + LEAST[out.dtype]
     return bool(((f64(out) - want).abs() <= room).all())
 

@@ -59,8 +59,14 @@ struct W4Args {
     int bf16_scales, has_zeros, out_type;
 };
 
-__device__ __forceinline__ float scale_f32(uint32_t bits, bool bf16) {
-    return bf16 ? bf16_bits_to_f32(bits) : half_bits_to_f32(bits);
+// A scale's four rows of a unit, as the factors of a lane's four results.
+__device__ __forceinline__ void scales_f32(u32x2 s, bool bf16, float (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t bits = s[i / 2] >> (i % 2 * 16);
+        const float a = half_bits_to_f32(bits), b = bf16_bits_to_f32(bits);
+        f[i] = bf16 ? b : a;
+    }
 }
 
 // Eight weights c - z of a dword, in the order of the columns.
@@ -107,12 +113,6 @@ __device__ __forceinline__ long weights_i8(uint32_t w, uint32_t zzzz) {
     // bytes 128 + c - z borrow nothing from each other
     const uint32_t a = ((even | 0x80808080u) - zzzz) ^ 0x80808080u, b = ((odd | 0x80808080u) - zzzz) ^ 0x80808080u;
     return (long)((uint64_t)b << 32 | a);
-}
-
-// A scale's four rows of a unit, as the f32 factors of a lane's four results.
-__device__ __forceinline__ void scales_f32(u32x2 s, bool bf16, float (&f)[4]) {
-    f[0] = scale_f32(s.x & 0xFFFF, bf16), f[1] = scale_f32(s.x >> 16, bf16);
-    f[2] = scale_f32(s.y & 0xFFFF, bf16), f[3] = scale_f32(s.y >> 16, bf16);
 }
 
 // What a lane holds of a step: a row's codes, the scales of its results' rows,
@@ -245,13 +245,14 @@ __device__ __forceinline__ float x_scale(const W4Args& a, int b, int step, int u
     return a.x_scales[(int64_t)b * a.x_groups + (k >> a.x_shift)];
 }
 
-// Joins the waves of a tile and the parts of an input, and stores: red holds
-// [wave][column][16 rows].
-template <int X, int PARTS>
-__device__ __forceinline__ void store_tiles(const W4Args& a, const float* red, int first_tile, int tiles, int b0,
-                                            int count, int columns) {
-    for (int i = threadIdx.x; i < tiles * count * 16; i += blockDim.x) {
-        const int m = i & 15, t = (i >> 4) / count, b = (i >> 4) - t * count;
+// Joins the waves of a tile and the parts of an input, and stores the tiles of a
+// workgroup from first_tile on: red holds [wave][column][16 rows].
+template <int X, int PARTS, int WAVES>
+__device__ __forceinline__ void store_tiles(const W4Args& a, const float* red, int first_tile, int b0, int count,
+                                            int columns) {
+    const int wms = WAVES / a.wk, sh = 31 - __clz(wms);  // tiles, a power of two
+    for (int i = threadIdx.x; i < count * wms * 16; i += WAVES * 64) {
+        const int m = i & 15, t = i >> 4 & (wms - 1), b = i >> 4 >> sh;
         const int row = (first_tile + t) * 16 + m;
         if (row >= a.rows) continue;
         float v = 0;
@@ -345,7 +346,7 @@ __device__ __forceinline__ void few_operands(const Raw<X>& r, Operand<X_F16> (&o
     }
 }
 
-template <int X, int U, int W, int WAVES>
+template <int X, int U, int W, bool SB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr bool I8 = X == X_I8;
@@ -417,42 +418,51 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
     int s = 0, it = 0, t0 = blockIdx.x * wms;
     const auto compute = [&](const Step<W, false>& c, int step) {
         const uint8_t* xl = lds + (step * 16 + q) * g.pitch + col * XB;
+        const int at = step * U * cols_x + col;
+        Operand<I8 ? X_I8 : X_F16> x[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = *(const Operand<I8 ? X_I8 : X_F16>*)(xl + j * 4 * g.pitch);
+        float sum[U], m[I8 ? U : 1];
+#pragma unroll
+        for (int u = 0; u < U; u++) sum[u] = sums[at + u * cols_x];
+#pragma unroll
+        for (int u = 0; u < (I8 ? U : 1); u++) m[u] = factors[I8 ? at + u * cols_x : step * cols_x + col];
+        D d[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            d[u] = D{0, 0, 0, 0};
+#pragma unroll
+            for (int j = u * PER; j < (u + 1) * PER; j++) {
+                const uint32_t wd = c.codes[j];
+                if constexpr (I8) {
+                    const uint32_t even = wd & 0x0F0F0F0Fu, odd = wd >> 4 & 0x0F0F0F0Fu;
+                    d[u] = __builtin_amdgcn_mfma_i32_16x16x32_i8((long)((uint64_t)odd << 32 | even),
+                                                                 __builtin_bit_cast(long, x[j].v), d[u], 0, 0, 0);
+                } else {
+                    const uint32_t w8 = wd >> 8;
+                    const u32x4 wv = {wd & 0x000F000Fu, wd & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u};
+                    d[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, wv),
+                                                                  __builtin_bit_cast(half8, x[j].v), d[u], 0, 0, 0);
+                }
+            }
+        }
         f32x4 part = {0, 0, 0, 0};
 #pragma unroll
         for (int u = 0; u < U; u++) {
             constexpr int per_w = U / W;
-            D d = {0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < PER; k++) {
-                const int j = u * PER + k;
-                const uint32_t wd = c.codes[j];
-                if constexpr (I8) {
-                    const uint32_t even = wd & 0x0F0F0F0Fu, odd = wd >> 4 & 0x0F0F0F0Fu;
-                    const long wv = (long)((uint64_t)odd << 32 | even);
-                    d = __builtin_amdgcn_mfma_i32_16x16x32_i8(wv, *(const long*)(xl + j * 4 * g.pitch), d, 0, 0, 0);
-                } else {
-                    const uint32_t w8 = wd >> 8;
-                    const u32x4 wv = {wd & 0x000F000Fu, wd & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u};
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, wv),
-                                                               *(const half8*)(xl + j * 4 * g.pitch), d, 0, 0, 0);
-                }
-            }
             float f[4];
-            scales_f32(c.scales[u / per_w], a.bf16_scales, f);
-            const int at = (step * U + u) * cols_x + col;
-            const float m = I8 ? factors[at] : 1.f;
+            scales_f32(c.scales[u / per_w], SB, f);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int byte = i * W + u / per_w;
                 const uint32_t z = c.zeros[byte / 4] >> (byte % 4 * 8) & 0xFF;
-                if constexpr (I8) acc[i] = fmaf((float)(d[i] - (int)z * ((const int*)sums)[at]), f[i] * m, acc[i]);
-                else part[i] = fmaf(fmaf(-(float)z, sums[at], d[i]), f[i], part[i]);
+                if constexpr (I8) acc[i] = fmaf((float)(d[u][i] - (int)z * (int)__float_as_uint(sum[u])), f[i] * m[u], acc[i]);
+                else part[i] = fmaf(fmaf(-(float)z, sum[u], d[u][i]), f[i], part[i]);
             }
         }
         if constexpr (!I8) {
-            const float m = factors[step * cols_x + col] * 0x1p24f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[i] = fmaf(part[i], m, acc[i]);
+            for (int i = 0; i < 4; i++) acc[i] = fmaf(part[i], m[0] * 0x1p24f, acc[i]);
         }
     };
     while (t0 < a.tiles) {
@@ -466,7 +476,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
                 float* red = (float*)(lds + g.red) + it * (WAVES * 256);
                 *(f32x4*)(red + (wave * 16 + r) * 16 + q * 4) = acc;
                 __syncthreads();
-                store_tiles<X, PARTS>(a, red, t0, min(wms, a.tiles - t0), 0, a.batch, 16);
+                store_tiles<X, PARTS, WAVES>(a, red, t0, 0, a.batch, 16);
                 acc = f32x4{0, 0, 0, 0};
                 s = 0, it ^= 1, t0 += stride, tile += stride;
             }
@@ -476,7 +486,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
 
 // More inputs, or deeper rows: NT tiles of 16 columns; x goes through LDS, wk
 // steps of it at a time in two buffers, [32 columns][q][column of the product],
-// loaded a phase ahead into registers.
+// loaded into registers a phase ahead.
 template <int X, int U, int W, int NT>
 __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -600,7 +610,7 @@ __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
 #pragma unroll
     for (int n = 0; n < NT; n++) *(f32x4*)(red + ((wave * NT + n) * 16 + r) * 16 + q * 4) = acc[n];
     __syncthreads();
-    store_tiles<X, PARTS>(a, red, blockIdx.x * wms, min(wms, a.tiles - (int)blockIdx.x * wms), b0, count, 16 * NT);
+    store_tiles<X, PARTS, kWaves>(a, red, blockIdx.x * wms, b0, count, 16 * NT);
 }
 
 // ------------------------------------------------------------------ packing
@@ -690,8 +700,12 @@ template <int X, int U, int W>
 void launch_w4(const W4Args& a, W4Plan& p, hipStream_t s) {
     if (!p.few) return launch_rows<X, U, W>(a, p, s);
     p.g.w = a;
-    if (p.waves == 8) w4_few_kernel<X, U, W, 8><<<p.grid, 512, p.lds, s>>>(p.g);
-    else w4_few_kernel<X, U, W, 16><<<p.grid, 1024, p.lds, s>>>(p.g);
+#define FEW(SB)                                                                                 \
+    if (p.waves == 8) w4_few_kernel<X, U, W, SB, 8><<<p.grid, 512, p.lds, s>>>(p.g);            \
+    else w4_few_kernel<X, U, W, SB, 16><<<p.grid, 1024, p.lds, s>>>(p.g)
+    if (a.bf16_scales) { FEW(true); }
+    else { FEW(false); }
+#undef FEW
 }
 // u: sums of a step that are scaled by themselves, w: those that the weights'
 // groups ask for (fewer where 8-bit inputs have the finer scales)
@@ -723,7 +737,11 @@ W4Plan w4_plan(W4Args* a, int x, int units, size_t batch, size_t tiles, size_t s
         if (columns <= 16 && steps <= 65536 && p.lds <= kLdsFew) {
             p.few = true;
             a->wk = 1;
-            while (a->wk < kWaves && (size_t)a->wk < steps && tiles * a->wk < 16 * cus) a->wk *= 2;
+            // waves of a tile, as many as keep 16 a CU busy: at least a ring's steps
+            // each, half of one where that leaves CUs without work
+            while (a->wk < kWaves && tiles * a->wk < 16 * cus &&
+                   steps >= (size_t)a->wk * (tiles * a->wk < 8 * cus ? kFewRing : 2 * kFewRing))
+                a->wk *= 2;
             p.g.n = (int)((steps + a->wk - 1) / a->wk);
             p.g.pitch = (int)pitch, p.g.sums = (int)x_bytes, p.g.red = (int)red;
             // workgroups as many as fit the card, with as many tiles each
@@ -735,21 +753,32 @@ W4Plan w4_plan(W4Args* a, int x, int units, size_t batch, size_t tiles, size_t s
         }
     }
     const size_t parts = parts_of(x);
-    // even blocks of at most 128 columns
-    const size_t most = 128 / parts, blocks = (batch + most - 1) / most;
-    const size_t block = (batch + blocks - 1) / blocks;
-    p.nt = (int)((block * parts + 15) / 16);
-    if (p.nt > 5) p.nt = 8;
-    const size_t step_bytes = 16 * (block * parts * (x == X_I8 ? 8 : 16) + 16) + (x == X_I8 ? 4 * units * block : 0);
-    const size_t most_items = (x == X_F32 ? kItems / 2 : kItems) * kWaves * 64;
-    a->wk = kWaves;
-    while (a->wk > 1 && (tiles * a->wk * blocks > 16 * cus || 2 * a->wk * step_bytes > kLds ||
-                         block * a->wk * 16 > most_items))
-        a->wk /= 2;
-    a->block = (int)block;
-    const size_t wms = kWaves / a->wk;
-    p.grid = dim3((unsigned)((tiles + wms - 1) / wms), (unsigned)std::min<size_t>(blocks, 65536));
-    p.lds = std::max<size_t>(2 * ((a->wk * step_bytes + 15) / 16 * 16), (size_t)kWaves * p.nt * 1024);
+    // Blocks of inputs and waves of a tile by an estimate: a phase takes 1.2 us and
+    // 0.06 a tile of columns where a CU has one workgroup (staging, products and
+    // the barrier in turn), 0.35 and 0.2 where workgroups share it.
+    double best = 0;
+    for (const int nt : {1, 2, 3, 4, 5, 8}) {
+        const size_t most = 16 * nt / parts, blocks = (batch + most - 1) / most, block = (batch + blocks - 1) / blocks;
+        if (best > 0 && (block * parts + 15) / 16 * 2 <= (size_t)nt) break;  // the batch has no more columns
+        const size_t step_bytes = 16 * (block * parts * (x == X_I8 ? 8 : 16) + 16) + (x == X_I8 ? 4 * units * block : 0);
+        for (int wk = 1; wk <= kWaves; wk *= 2) {
+            const size_t items = (block * wk * 16 + kWaves * 64 - 1) / (kWaves * 64);
+            const size_t buffers = 2 * ((wk * step_bytes + 15) / 16 * 16);
+            if (wk > 1 && (buffers > kLds || items > (size_t)(x == X_F32 ? kItems / 2 : kItems))) break;
+            const size_t lds = std::max<size_t>(buffers, (size_t)kWaves * nt * 1024), phases = (steps + wk - 1) / wk;
+            const size_t fit = nt <= 3 && lds <= 80 * 1024 ? 2 : 1, grid_x = (tiles * wk + kWaves - 1) / kWaves;
+            const size_t of_cu = (grid_x * blocks + cus - 1) / cus;
+            const double staging = x == X_F32 ? 0.1 * (double)items : 0;
+            const double alone = 1.2 + 0.06 * nt + staging, shared = 0.35 + 0.2 * nt + staging;
+            const double us = (double)phases * ((double)(of_cu / fit) * std::max(alone, (double)fit * shared) +
+                                                (of_cu % fit ? alone : 0.0));
+            if (best == 0 || us < best) {
+                best = us;
+                p.nt = nt, p.lds = lds, a->wk = wk, a->block = (int)block;
+                p.grid = dim3((unsigned)std::min<size_t>(grid_x, UINT32_MAX), (unsigned)std::min<size_t>(blocks, 65536));
+            }
+        }
+    }
     return p;
 }
 

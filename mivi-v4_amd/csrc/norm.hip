@@ -31,10 +31,10 @@ struct NormArgs {
     int8_t* codes;
     float* scales;
     int64_t x_row, x_head, r_row, r_head, ro_row, ro_head, o_row, o_head;
-    double eps;
+    double eps, inv_dim;
     uint32_t n_rows, heads;  // n_rows: rows times heads
     int dim, group;          // group: a row's dimensions where it has one scale
-    int lanes, waves;        // a row has `lanes` (a power of two) of a wave, or `waves` whole ones
+    int lanes, waves;        // of a row: waves, or (waves 0) lanes of one, a power of two
 };
 
 // ------------------------------------------------- 64-bit reductions of lanes
@@ -73,11 +73,10 @@ __device__ __forceinline__ double fold_lanes(double v, int lanes) {
     return v;
 }
 
-// Over the row: its lanes, then its waves through `part`.
+// Over the workgroup: its waves' sums through `part`.
 template <bool MAX>
 __device__ __forceinline__ double fold_row(double v, const NormArgs& a, double* part) {
-    v = fold_lanes<MAX>(v, a.lanes);
-    if (a.waves == 1) return v;
+    v = fold_lanes<MAX>(v, 64);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
     v = part[0];
@@ -85,7 +84,18 @@ __device__ __forceinline__ double fold_row(double v, const NormArgs& a, double* 
     return v;
 }
 
-// --------------------------------------------------------------- the kernel
+// The instructions' 1 / sqrt x and 1 / x (2^-24) with a Newton step: 2^-46, in six
+// instructions where the library's take forty to eighty.
+__device__ __forceinline__ double inv_sqrt(double m) {
+    const double y = __builtin_amdgcn_rsq(m);
+    return m > 1.7976931348623157e308 ? 0.0 : y * fma(-0.5 * m, y * y, 1.5);
+}
+__device__ __forceinline__ double inverse(double x) {
+    const double y = __builtin_amdgcn_rcp(x);
+    return fma(fma(-x, y, 1.0), y, y);
+}
+
+// --------------------------------------------------------------- the kernels
 // s of n elements (up to 8) from i on; where `keep`, written to ro too.
 template <int T, class F>
 __device__ __forceinline__ void load_sum(const NormArgs& a, int64_t xo, int64_t ro, int64_t i, int n, F (&s)[8]) {
@@ -120,7 +130,7 @@ __device__ __forceinline__ double largest(double m, const double (&v)[8]) {
 // Codes of 8 values of a group whose largest magnitude is top; nothing that
 // stands for a value where top or the row's sum is not finite.
 __device__ __forceinline__ void store_codes(int8_t* at, int n, const double (&v)[8], double top, bool ok) {
-    const double inv = top > 0 ? 127 / top : 0.0;
+    const double inv = top > 0 ? 127 * inverse(top) : 0.0;
     int c[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -151,19 +161,11 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
     constexpr bool HOLD = E > 0;
     __shared__ double part[2][16];
     const int tid = threadIdx.x;
-    int t = tid;
-    uint32_t row = blockIdx.x;
-    if (a.waves == 1) {
-        const int per = 64 / a.lanes;
-        t = tid & (a.lanes - 1);
-        row = (blockIdx.x * (blockDim.x >> 6) + (tid >> 6)) * per + (tid & 63) / a.lanes;
-    }
-    const bool live = row < a.n_rows;  // lanes behind the last row take part with no elements
-    const int dim = live ? a.dim : 0;
-    const uint32_t r0 = live ? row / a.heads : 0, h0 = live ? row % a.heads : 0;
+    const int t = tid, dim = a.dim;
+    const uint32_t row = blockIdx.x, r0 = row / a.heads, h0 = row - r0 * a.heads;
     const int64_t xo = r0 * a.x_row + h0 * a.x_head, rr = r0 * a.r_row + h0 * a.r_head;
     const int64_t ko = r0 * a.ro_row + h0 * a.ro_head, oo = r0 * a.o_row + h0 * a.o_head;
-    const int tpr = a.lanes * a.waves;
+    const int tpr = 64 * a.waves;
     const int steps = HOLD ? E : (a.dim + 8 * tpr - 1) / (8 * tpr);
 
     F s[HOLD ? E : 1][8];
@@ -201,7 +203,7 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
         }
     }
     sum = fold_row<false>(sum, a, part[0]);
-    const double f = 1.0 / sqrt(sum / a.dim + a.eps);
+    const double f = inv_sqrt(fma(sum, a.inv_dim, a.eps));
     const bool ok = sum <= 1.7976931348623157e308;
     if constexpr (Q8) {
         if (a.group == a.dim) top = fold_row<true>(top, a, part[1]);
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
             if (n > 0) {
                 store_codes(a.codes + (int64_t)row * a.dim + i, n, v, top, fine);
                 if (i % a.group == 0)
-                    a.scales[(int64_t)row * ng + i / a.group] = fine ? (float)(top * f / 127) : __builtin_nanf("");
+                    a.scales[(int64_t)row * ng + i / a.group] = fine ? (float)(top * f * (1.0 / 127)) : __builtin_nanf("");
             }
         } else if (n > 0) {
             float y[8];
@@ -242,8 +244,64 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
     }
 }
 
+// Rows of up to 512 elements, 8 a lane: R rows for every group of lanes, all
+// their loads first.
+template <int T, int R, bool Q8>
+__global__ __launch_bounds__(256) void norm_short_kernel(NormArgs a) {
+    typedef typename std::conditional<Q8, double, float>::type F;
+    const int t = threadIdx.x & (a.lanes - 1), i = t * 8;
+    const uint32_t groups = gridDim.x * 256 / a.lanes, first = (blockIdx.x * 256 + threadIdx.x) / a.lanes;
+    F s[R][8];
+    int n[R];
+    int64_t ko[R], oo[R];
+#pragma unroll
+    for (int e = 0; e < R; e++) {
+        const uint32_t row = first + e * groups;
+        const bool live = row < a.n_rows;  // lanes behind the last row take part with no elements
+        const uint32_t r = live ? row / a.heads : 0, h = live ? row - r * a.heads : 0;
+        n[e] = live ? a.dim - i : 0;
+        ko[e] = r * a.ro_row + h * a.ro_head + i, oo[e] = r * a.o_row + h * a.o_head + i;
+        load_sum<T>(a, r * a.x_row + h * a.x_head, r * a.r_row + h * a.r_head, i, n[e], s[e]);
+    }
+    float w[8];
+    load_row8<MIVI_GGML_F32>(a.w, i, a.dim - i, w);
+#pragma unroll
+    for (int e = 0; e < R; e++) {
+        if (n[e] > 0) keep_sum<T>(a, ko[e], n[e], s[e]);
+        double sum = 0, top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) sum = fma((double)s[e][j], (double)s[e][j], sum);
+        sum = fold_lanes<false>(sum, a.lanes);
+        const double f = inv_sqrt(fma(sum, a.inv_dim, a.eps));
+        if constexpr (Q8) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) s[e][j] *= w[j];
+            top = fold_lanes<true>(largest(0, s[e]), a.group == a.dim ? a.lanes : a.group / 8);
+            const bool fine = sum <= 1.7976931348623157e308 && top <= 1.7976931348623157e308;
+            if (n[e] > 0) {
+                const int64_t row = first + e * groups;
+                store_codes(a.codes + row * a.dim + i, n[e], s[e], top, fine);
+                if (i % a.group == 0)
+                    a.scales[row * (a.dim / a.group) + i / a.group] =
+                        fine ? (float)(top * f * (1.0 / 127)) : __builtin_nanf("");
+            }
+        } else if (n[e] > 0) {
+            const float f32 = (float)f;
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = s[e][j] * f32 * w[j];
+            store_row8<T>(a.out, oo[e], n[e], y);
+        }
+    }
+}
+
 template <int T, bool Q8>
 void launch_norm(const NormArgs& a, int e, unsigned grid, unsigned threads, hipStream_t s) {
+    if (a.waves == 0) {
+        if (e == 1) norm_short_kernel<T, 1, Q8><<<grid, threads, 0, s>>>(a);
+        else norm_short_kernel<T, 4, Q8><<<grid, threads, 0, s>>>(a);
+        return;
+    }
     switch (e) {
         case 1: norm_kernel<T, 1, Q8><<<grid, threads, 0, s>>>(a); break;
         case 2: norm_kernel<T, 2, Q8><<<grid, threads, 0, s>>>(a); break;
@@ -257,24 +315,27 @@ void launch_norm(const NormArgs& a, int e, unsigned grid, unsigned threads, hipS
 }
 
 // Lays the rows out and launches: rows of up to 512 elements on the fewest
-// lanes that take 8 each; longer ones on as many waves as take E chunks a
-// thread.
+// lanes that take 8 each, four rows a group where that leaves 8 waves a CU;
+// longer ones on as many waves as take E chunks a thread.
 int32_t run_norm(NormArgs a, int32_t type, bool q8, size_t rows, size_t heads, size_t dim, hipStream_t s) {
     const size_t n_rows = rows * heads, chunks = (dim + 7) / 8;
+    size_t grid, threads = 256;
     int e = 1;
-    a.lanes = 64, a.waves = 1;
+    a.n_rows = (uint32_t)n_rows, a.heads = (uint32_t)heads, a.dim = (int)dim;
+    a.inv_dim = 1.0 / (double)dim;
+    a.lanes = 64, a.waves = 0;
     if (chunks <= 64) {
         a.lanes = 1;
         while ((size_t)a.lanes < chunks) a.lanes *= 2;
+        if (n_rows * a.lanes >= 4 * 8 * 64 * (size_t)num_cus()) e = 4;
+        grid = (n_rows * a.lanes + 256 * e - 1) / (256 * e);
     } else {
         e = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : chunks <= 4096 && !q8 ? 4 : 0;
         a.waves = (int)std::min<size_t>(16, e ? ((chunks + e - 1) / e + 63) / 64 : 16);
+        grid = n_rows, threads = 64 * a.waves;
     }
-    const size_t per = a.waves > 1 ? 1 : 4 * (64 / a.lanes), threads = a.waves > 1 ? 64 * a.waves : 256;
-    const size_t grid = (n_rows + per - 1) / per;
     if (!grid_fits(grid, threads)) return err_overflow();
     clear_error();
-    a.n_rows = (uint32_t)n_rows, a.heads = (uint32_t)heads, a.dim = (int)dim;
 #define NORM(T) (q8 ? launch_norm<T, true>(a, e, (unsigned)grid, (unsigned)threads, s) \
                     : launch_norm<T, false>(a, e, (unsigned)grid, (unsigned)threads, s))
     if (type == MIVI_GGML_F32) NORM(MIVI_GGML_F32);

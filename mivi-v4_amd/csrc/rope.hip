@@ -97,37 +97,51 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
             c[e] *= a.scale, s[e] *= a.scale;
         }
     }
-    const int all = a.heads + a.kv;
-    for (int h = part * a.per + slot; h < all; h += a.parts * a.per) {
+    // two runs of 8 elements a head: its firsts and seconds, or 16 neighbours with
+    // the pairs side by side; of the dimensions behind rot 16 neighbours too
+    const int i0 = turns ? HALF ? u * 8 : u * 16 : a.rot + (u - a.units) * 16;
+    const int i1 = turns && HALF ? half + u * 8 : i0 + 8;
+    const int n0 = turns ? HALF ? n : 2 * n : a.hd - i0, n1 = turns && HALF ? n : n0 - 8;
+    const int all = a.heads + a.kv, step = a.parts * a.per;
+    const auto at = [&](int h, const void** x, int64_t* xi, void** o, int64_t* oi) {
         const bool is_q = h < a.heads;
         const int hh = is_q ? h : h - a.heads;
-        const void* x = is_q ? a.q : a.k;
-        void* o = is_q ? a.q_out : a.k_out;
-        const int64_t xi = (int64_t)row * (is_q ? a.q_row : a.k_row) + hh * (is_q ? a.q_head : a.k_head);
-        const int64_t oi = (int64_t)row * (is_q ? a.qo_row : a.ko_row) + hh * (is_q ? a.qo_head : a.ko_head);
-        float v[2][8];
-        if (turns) {
-            // HALF: 8 firsts and 8 seconds; else 16 neighbours, pairs side by side
-            const int i0 = HALF ? u * 8 : u * 16, i1 = HALF ? half + u * 8 : u * 16 + 8;
-            const int n0 = HALF ? n : 2 * n, n1 = HALF ? n : 2 * n - 8;
-            load_row8<T>(x, xi + i0, n0, v[0]);
-            load_row8<T>(x, xi + i1, n1, v[1]);
+        *x = is_q ? a.q : a.k, *o = is_q ? a.q_out : a.k_out;
+        *xi = (int64_t)row * (is_q ? a.q_row : a.k_row) + hh * (is_q ? a.q_head : a.k_head);
+        *oi = (int64_t)row * (is_q ? a.qo_row : a.ko_row) + hh * (is_q ? a.qo_head : a.ko_head);
+        return h < all && (turns || (is_q ? a.copy_q : a.copy_k));
+    };
+    // two heads' loads before their stores
+    for (int h = part * a.per + slot; h < all; h += 2 * step) {
+        float v[2][2][8];
+        void* o[2];
+        int64_t oi[2];
+        bool live[2];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float& p = HALF ? v[0][e] : v[e / 4][e % 4 * 2];
-                float& q = HALF ? v[1][e] : v[e / 4][e % 4 * 2 + 1];
-                const float y = fmaf(p, c[e], -(q * s[e]));
-                q = fmaf(q, c[e], p * s[e]);
-                p = y;
+        for (int j = 0; j < 2; j++) {
+            const void* x;
+            int64_t xi;
+            live[j] = at(h + j * step, &x, &xi, &o[j], &oi[j]);
+            if (live[j]) {
+                load_row8<T>(x, xi + i0, n0, v[j][0]);
+                load_row8<T>(x, xi + i1, n1, v[j][1]);
             }
-            store_row8<T>(o, oi + i0, n0, v[0]);
-            store_row8<T>(o, oi + i1, n1, v[1]);
-        } else if (is_q ? a.copy_q : a.copy_k) {
-            const int i = a.rot + (u - a.units) * 16, m = a.hd - i;
-            load_row8<T>(x, xi + i, m, v[0]);
-            load_row8<T>(x, xi + i + 8, m - 8, v[1]);
-            store_row8<T>(o, oi + i, m, v[0]);
-            store_row8<T>(o, oi + i + 8, m - 8, v[1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            if (!live[j]) continue;
+            if (turns) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float& p = HALF ? v[j][0][e] : v[j][e / 4][e % 4 * 2];
+                    float& q = HALF ? v[j][1][e] : v[j][e / 4][e % 4 * 2 + 1];
+                    const float y = fmaf(p, c[e], -(q * s[e]));
+                    q = fmaf(q, c[e], p * s[e]);
+                    p = y;
+                }
+            }
+            store_row8<T>(o[j], oi[j] + i0, n0, v[j][0]);
+            store_row8<T>(o[j], oi[j] + i1, n1, v[j][1]);
         }
     }
 }
@@ -186,8 +200,10 @@ extern "C" int32_t mivi_hip_rope(int32_t type, void* q_out, size_t q_out_len, si
     a.units = (int)((rot_dim / 2 + 7) / 8);
     a.tail = a.copy_q || a.copy_k ? (int)((head_dim - rot_dim + 15) / 16) : 0;
     a.per = 64 / (a.units + a.tail);
+    // waves of a row: one for each time that its heads fill one, fewer where rows
+    // alone are 16 a CU, so that angles serve several heads
     const size_t passes = (n_heads + n_kv_heads + a.per - 1) / a.per;
-    a.parts = (int)passes;
+    a.parts = (int)std::min(passes, std::max<size_t>(1, 16 * (size_t)num_cus() / rows));
     size_t waves;
     if (__builtin_mul_overflow(rows, (size_t)a.parts, &waves) || !grid_fits((waves + 3) / 4, 256)) return err_overflow();
     clear_error();

@@ -101,6 +101,17 @@ __device__ __forceinline__ double wave_sum64(double v) {
     return v;
 }
 
+// The first thread (from `base` on) that passes into at, the last with any mass
+// into behind.
+__device__ __forceinline__ void mark(bool passes, bool some, int base, int* at, int* behind) {
+    const uint64_t a = __ballot(passes), b = __ballot(some);
+    const int wave = base + (threadIdx.x & ~63);
+    if ((threadIdx.x & 63) == 0) {
+        if (a) atomicMin(at, wave + (int)__ffsll((unsigned long long)a) - 1);
+        if (b) atomicMax(behind, wave + 63 - (int)__clzll((long long)b));
+    }
+}
+
 __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
     __shared__ int first;
     __shared__ double sh[2][kThreads / 64];
@@ -141,7 +152,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
 // it is the last with any mass.
 __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
     __shared__ double sh[kThreads / 64];
-    __shared__ int at, behind;
+    __shared__ int at, behind, found;
     __shared__ double before;
     const int s = blockIdx.x, tid = threadIdx.x;
     int lo, hi;
@@ -153,12 +164,18 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
     const int count = a.found[s], row = lo + count;
     const bool last = row == hi - 1;
     const double2* parts = a.parts + (int64_t)s * a.chunks;
-    double l = 0, m = 0, whole, all_p;
-    for (int c = tid; c < a.chunks; c += kThreads) l += parts[c].x, m += parts[c].y;
-    scan(l, sh, &whole);
-    scan(m, sh, &all_p);
+    // the whole, with the first chunks' sums in hand
+    const double2 mine = tid < a.chunks ? parts[tid] : double2{0, 0};
+    double l = mine.x, whole;
+    for (int64_t c = tid + kThreads; c < a.chunks; c += kThreads) l += parts[c].x;
+    const double first = scan(l, sh, &whole);
+    const bool one = a.chunks <= kThreads;
     const bool from_p = whole == 0;  // nothing is left of the row
-    if (from_p) whole = all_p;
+    if (from_p) {
+        double m = mine.y;
+        for (int64_t c = tid + kThreads; c < a.chunks; c += kThreads) m += parts[c].y;
+        scan(m, sh, &whole);
+    }
     int token = -1;
     if (whole > 0) {
         const double goal = (double)a.pick[s] * whole;
@@ -167,11 +184,11 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
         double base = 0;
         for (int64_t b = 0; b < a.chunks; b += kThreads) {
             const int64_t c = b + tid;
-            const double v = c < a.chunks ? (from_p ? parts[c].y : parts[c].x) : 0.0;
-            double all;
-            const double ex = base + scan(v, sh, &all);
-            if (v > 0 && ex + v > goal) atomicMin(&at, (int)c);
-            if (v > 0) atomicMax(&behind, (int)c);
+            double v = b == 0 ? (from_p ? mine.y : mine.x) : 0.0;
+            if (b && c < a.chunks) v = from_p ? parts[c].y : parts[c].x;
+            double all = 0;
+            const double ex = one && !from_p ? first : base + scan(v, sh, &all);
+            mark(v > 0 && ex + v > goal, v > 0, (int)b, &at, &behind);
             __syncthreads();
             if (at == (int)c) before = ex;
             base += all;
@@ -195,9 +212,11 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
         }
         double all;
         const double ex = scan(v, sh, &all);
-        if (v > 0) {
+        mark(v > 0 && ex + v > rest, v > 0, 0, &at, &behind);
+        __syncthreads();
+        if (tid == (at != INT32_MAX ? at : behind)) {  // its sum passes: the same sums pass in it
             double sum = 0;
-            int hit = -1, some = -1;
+            int hit = -1, some = 0;
 #pragma unroll
             for (int e = 0; e < kPer; e++) {
                 sum += left[e];
@@ -206,11 +225,10 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
                     if (hit < 0 && ex + sum > rest) hit = e;
                 }
             }
-            if (hit >= 0) atomicMin(&at, (int)i + hit);
-            atomicMax(&behind, (int)i + some);
+            found = (int)i + (hit >= 0 ? hit : some);
         }
         __syncthreads();
-        token = at != INT32_MAX ? at : behind;
+        token = found;
     }
     if (tid == 0) a.counts[s] = count;
     for (int64_t r = (int64_t)lo + tid; r < hi; r += kThreads)

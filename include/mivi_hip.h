@@ -375,9 +375,12 @@ int32_t mivi_hip_w4_pack(const uint8_t* codes, size_t codes_len, int32_t scale_t
                          size_t scales_len, const uint8_t* zeros, size_t zeros_len, uint8_t* packed,
                          size_t packed_len, size_t rows, size_t cols, size_t group, void* stream);
 
-/* out[batch][rows] = x[batch][cols] W^T, both in `type`. The products are exact
- * in f16 and bf16, of 24 bits of x in f32; sums and scales are f32. The order of
- * a row's sums, and so its last bits, depends on the batch it is in. */
+/* out[batch][rows] = x[batch][cols] W^T, both in `type`. f16 and bf16 inputs
+ * enter the products with all their bits, f32 ones with 22 or, in larger
+ * batches, 24, any of them to no less than 2^-40 of the largest magnitude of 128
+ * columns; c - z enters exactly, sums and scales are f32 (a group's sum of (c -
+ * z) x has to be an f32 number). The order of a row's sums, and so its last bits,
+ * depends on the batch it is in. An infinity or NaN stays in its input's row. */
 int32_t mivi_hip_w4_matmul_rows(int32_t type, void* out, size_t out_len, size_t out_row_stride,
                                 const uint8_t* packed, size_t packed_len, int32_t scale_type,
                                 int32_t has_zeros, const void* x, size_t x_len, size_t x_row_stride,

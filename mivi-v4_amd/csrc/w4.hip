@@ -270,21 +270,22 @@ __device__ __forceinline__ void store_tiles(const W4Args& a, const float* red, i
 }
 
 // --------------------------------------------------------------- few inputs
-// Up to 16 columns of the product. The weights enter as fp16 numbers c 2^-24
-// and, from the nibbles above, 16 c 2^-24: masks alone, where 1 + c / 16 or c - z
-// would take two to four times the instructions; x against the latter is held
-// as a sixteenth. x is held in fp16, each step's 128 columns multiplied by the
-// power of two that takes their largest to 2^14 .. 2^15 (f32 in two parts, 22
-// bits; nothing to less than 2^-36 of that largest). The zeros come out of the
-// results, d - z sum x, where both are at most four times what the weights'
-// values would give.
+// Up to 16 columns of the product. x lies whole in LDS, in operand order, and
+// tiles stream past it. f16 inputs stay as they are; bf16 and f32 ones are held
+// in fp16, each step's 128 columns multiplied by the power of two that takes
+// their largest to 2^14 .. 2^15 (f32 in two parts, 22 bits; nothing to less than
+// 2^-40 of that largest). Against 8-bit x the weights enter as codes and z sum x
+// comes off their sums, all whole numbers. (With codes as the fp16 numbers c
+// 2^-24, masks alone, one input takes 4 to 10 % less, but sums have 17 bits: the
+// matrix cores align products by their operands' exponents as if all were normal
+// numbers.)
 constexpr int few_parts(int x) { return x == X_F32 ? 2 : 1; }
 constexpr int kFewRing = 4;  // steps of a wave in flight
 
 struct FewArgs {
     W4Args w;
     int n;                         // steps of a wave
-    int pitch, sums, red;          // bytes of LDS: of 8 columns; before the sums of x; before the results
+    int pitch, sums, red;          // bytes of LDS: of 8 columns; before x's sums and factors; before the results
 };
 
 // Largest magnitude's bits over 16 lanes; sums over 16, 8 or 4.
@@ -305,45 +306,32 @@ __device__ __forceinline__ float unit_sum(float v) {
     return v;
 }
 
-// 8 columns of an input as operands, the sums of their units times 2^-24, and
-// what the step's results are to be multiplied by (2^24 aside).
-template <int X, int U>
-__device__ __forceinline__ void few_operands(const Raw<X>& r, Operand<X_F16> (&o)[few_parts(X)], float (&sum)[few_parts(X)],
-                                             float* factor) {
+// 8 columns of an input as operands, and what the step's results are to be
+// multiplied by. 16 lanes have a step.
+template <int X>
+__device__ __forceinline__ void few_operands(const Raw<X>& r, Operand<X_F16> (&o)[few_parts(X)], float* factor) {
     float v[8];
     uint32_t top = 0;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         if constexpr (X == X_F32) v[e] = __uint_as_float(r.v[e / 4][e % 4]);
-        else if constexpr (X == X_F16) v[e] = half_bits_to_f32(r.v[0][e / 2] >> (e % 2 * 16));
         else v[e] = bf16_bits_to_f32(r.v[0][e / 2] >> (e % 2 * 16));
         top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
     }
     // biased exponents: 2^(14 - e) for a largest value of 2^e, 2^126 at most
     const int ex = min(127 + 14 - ((int)(max16(top) >> 23) - 127), 253);
-    const float up = __uint_as_float((uint32_t)ex << 23), up16 = __uint_as_float((uint32_t)(ex - 4) << 23);
+    const float up = __uint_as_float((uint32_t)ex << 23);
     *factor = __uint_as_float((uint32_t)(254 - ex) << 23);
     half8 h[few_parts(X)];
 #pragma unroll
-    for (int p = 0; p < few_parts(X); p++) sum[p] = 0;
-#pragma unroll
     for (int e = 0; e < 8; e++) {
-        const bool sixteenth = e / 2 % 2;
-        float y = v[e] * (sixteenth ? up16 : up);
-#pragma unroll
-        for (int p = 0; p < few_parts(X); p++) {
-            const _Float16 part = (_Float16)y;
-            h[p][e] = part;
-            sum[p] = fmaf((float)part, sixteenth ? 0x1p-20f : 0x1p-24f, sum[p]);
-            // what an infinity leaves is nothing
-            y = p == 0 && __builtin_fabsf(y) == __builtin_inff() ? 0.f : y - (float)part;
-        }
+        const float y = v[e] * up;
+        h[0][e] = (_Float16)y;
+        // what an infinity leaves is nothing
+        if constexpr (X == X_F32) h[1][e] = (_Float16)(__builtin_fabsf(y) == __builtin_inff() ? 0.f : y - (float)h[0][e]);
     }
 #pragma unroll
-    for (int p = 0; p < few_parts(X); p++) {
-        o[p].v = __builtin_bit_cast(u32x4, h[p]);
-        sum[p] = unit_sum<U>(sum[p]);
-    }
+    for (int p = 0; p < few_parts(X); p++) o[p].v = __builtin_bit_cast(u32x4, h[p]);
 }
 
 template <int X, int U, int W, bool SB, int WAVES>
@@ -356,14 +344,14 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave % a.wk, wm = wave / a.wk;
     const int wms = WAVES / a.wk, stride = gridDim.x * wms, cols_x = a.batch * PARTS, col = min(r, cols_x - 1);
-    float* sums = (float*)(lds + g.sums);                    // [step][unit][column]: z times which comes off
-    float* factors = sums + a.steps * U * cols_x;            // [step][column], of 8-bit x [step][unit][column]
+    int* sums = (int*)(lds + g.sums);                               // of 8-bit x: [step][unit][column]
+    float* factors = (float*)sums + (I8 ? a.steps * U * cols_x : 0);  // the same, of others [step][column]
 
-    Step<W, false> w[kFewRing];
+    Step<W, !I8> w[kFewRing];
     int tile = blockIdx.x * wms + wm, next_tile = tile, next = 0;  // of the next fetch
     const auto refill = [&](int slot) {
         // behind the last step and tile those are loaded again
-        fetch<W, false>(a, (int64_t)min(next_tile, a.tiles - 1) * a.steps + min(wk + next * a.wk, a.steps - 1), lane, &w[slot]);
+        fetch<W, !I8>(a, (int64_t)min(next_tile, a.tiles - 1) * a.steps + min(wk + next * a.wk, a.steps - 1), lane, &w[slot]);
         if (++next == g.n) next = 0, next_tile += stride;
     };
 #pragma unroll
@@ -386,9 +374,9 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
             if (base + e * WAVES * 64 >= items) break;
             const int c = at[e] >> 4, b = at[e] & 15;
             uint8_t* to = lds + c * g.pitch + b * PARTS * XB;
-            const int unit = (c >> 4) * U + (c & 15) / (16 / U);
-            const bool head = at[e] >= 0 && (c & (16 / U - 1)) == 0;
             if constexpr (I8) {
+                const int unit = (c >> 4) * U + (c & 15) / (16 / U);
+                const bool head = at[e] >= 0 && (c & (16 / U - 1)) == 0;
                 Operand<X> o[1];
                 operands<X>(raw[e], o);
                 int s = __builtin_amdgcn_sdot4((int)o[0].v.x, 0x01010101, 0, false);
@@ -396,18 +384,18 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
                 const float sum = unit_sum<U>((float)s);  // whole numbers far below 2^24
                 if (at[e] >= 0) *(Operand<X>*)to = o[0];
                 if (head) {
-                    ((int*)sums)[unit * cols_x + b] = (int)sum;
+                    sums[unit * cols_x + b] = (int)sum;
                     factors[unit * cols_x + b] = a.x_shift < 0 ? 1.f : x_scale<U>(a, b, c >> 4, unit & (U - 1));
                 }
             } else {
                 Operand<X_F16> o[PARTS];
-                float sum[PARTS], factor;
-                few_operands<X, U>(raw[e], o, sum, &factor);
+                float factor = 1.f;
+                if constexpr (X == X_F16) o[0].v = raw[e].v[0];
+                else few_operands<X>(raw[e], o, &factor);
 #pragma unroll
                 for (int p = 0; p < PARTS; p++) {
                     if (at[e] >= 0) *(Operand<X_F16>*)(to + p * XB) = o[p];
-                    if (head) sums[unit * cols_x + b * PARTS + p] = sum[p];
-                    if (at[e] >= 0 && (c & 15) == 0) factors[(c >> 4) * cols_x + b * PARTS + p] = factor;
+                    if (X != X_F16 && at[e] >= 0 && (c & 15) == 0) factors[(c >> 4) * cols_x + b * PARTS + p] = factor;
                 }
             }
         }
@@ -416,53 +404,56 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
 
     f32x4 acc = {0, 0, 0, 0};
     int s = 0, it = 0, t0 = blockIdx.x * wms;
-    const auto compute = [&](const Step<W, false>& c, int step) {
+    const auto compute = [&](const Step<W, !I8>& c, int step) {
         const uint8_t* xl = lds + (step * 16 + q) * g.pitch + col * XB;
         const int at = step * U * cols_x + col;
         Operand<I8 ? X_I8 : X_F16> x[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) x[j] = *(const Operand<I8 ? X_I8 : X_F16>*)(xl + j * 4 * g.pitch);
-        float sum[U], m[I8 ? U : 1];
+        int sum[U];
+        float m[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) sum[u] = sums[at + u * cols_x];
-#pragma unroll
-        for (int u = 0; u < (I8 ? U : 1); u++) m[u] = factors[I8 ? at + u * cols_x : step * cols_x + col];
+        for (int u = 0; u < U; u++) {
+            if constexpr (I8) sum[u] = sums[at + u * cols_x], m[u] = factors[at + u * cols_x];
+            else if (u == 0) m[u] = X == X_F16 ? 1.f : factors[step * cols_x + col];
+        }
+        constexpr int per_w = U / W;
         D d[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             d[u] = D{0, 0, 0, 0};
 #pragma unroll
             for (int j = u * PER; j < (u + 1) * PER; j++) {
-                const uint32_t wd = c.codes[j];
                 if constexpr (I8) {
-                    const uint32_t even = wd & 0x0F0F0F0Fu, odd = wd >> 4 & 0x0F0F0F0Fu;
+                    const uint32_t even = c.codes[j] & 0x0F0F0F0Fu, odd = c.codes[j] >> 4 & 0x0F0F0F0Fu;
                     d[u] = __builtin_amdgcn_mfma_i32_16x16x32_i8((long)((uint64_t)odd << 32 | even),
                                                                  __builtin_bit_cast(long, x[j].v), d[u], 0, 0, 0);
                 } else {
-                    const uint32_t w8 = wd >> 8;
-                    const u32x4 wv = {wd & 0x000F000Fu, wd & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u};
-                    d[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, wv),
-                                                                  __builtin_bit_cast(half8, x[j].v), d[u], 0, 0, 0);
+                    const Weights8<X_F16> wv(c.codes[j], c.zeros[0] >> (8 * (u / per_w)) & 15);
+                    d[u] = wv.times(x[j], d[u]);
                 }
             }
         }
         f32x4 part = {0, 0, 0, 0};
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            constexpr int per_w = U / W;
             float f[4];
             scales_f32(c.scales[u / per_w], SB, f);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int byte = i * W + u / per_w;
-                const uint32_t z = c.zeros[byte / 4] >> (byte % 4 * 8) & 0xFF;
-                if constexpr (I8) acc[i] = fmaf((float)(d[u][i] - (int)z * (int)__float_as_uint(sum[u])), f[i] * m[u], acc[i]);
-                else part[i] = fmaf(fmaf(-(float)z, sum[u], d[u][i]), f[i], part[i]);
+                if constexpr (I8) {
+                    const int byte = i * W + u / per_w, z = (int)(c.zeros[byte / 4] >> (byte % 4 * 8) & 0xFF);
+                    acc[i] = fmaf((float)(d[u][i] - z * sum[u]), f[i] * m[u], acc[i]);
+                } else if constexpr (X == X_F16) {
+                    acc[i] = fmaf(d[u][i], f[i], acc[i]);
+                } else {
+                    part[i] = fmaf(d[u][i], f[i], part[i]);
+                }
             }
         }
-        if constexpr (!I8) {
+        if constexpr (!I8 && X != X_F16) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[i] = fmaf(part[i], m[0] * 0x1p24f, acc[i]);
+            for (int i = 0; i < 4; i++) acc[i] = fmaf(part[i], m[0], acc[i]);
         }
     };
     while (t0 < a.tiles) {
@@ -729,7 +720,7 @@ W4Plan w4_plan(W4Args* a, int x, int units, size_t batch, size_t tiles, size_t s
         const size_t columns = batch * few_parts(x), xb = x == X_I8 ? 8 : 16;
         // columns of a multiple of 64 bytes would store to the same banks
         const size_t pitch = columns * xb + (columns * xb % 64 ? 0 : 16);
-        const size_t x_bytes = steps * 16 * pitch, sums = steps * columns * 4 * (units + (x == X_I8 ? units : 1));
+        const size_t x_bytes = steps * 16 * pitch, sums = steps * columns * 4 * (x == X_I8 ? 2 * units : 1);
         const size_t red = (x_bytes + sums + 15) / 16 * 16;
         // 16 waves a CU: two workgroups of 8, or one of 16 where x fills LDS
         p.waves = red + 2 * 8 * 1024 <= kLdsFew / 2 ? 8 : 16;

@@ -175,3 +175,24 @@ def test_more_blocks_than_one(hip):
     for dt in TYPES.values():
         x = inputs(1000, 384, dt)
         assert ref.w4_close(run(hip, w, on_gpu(hip, w), x), ref.f64(x), w)
+
+
+@pytest.mark.parametrize("batch", [1, 8, 9, 40])
+@pytest.mark.parametrize("group", [32, 128])
+def test_sums_keep_the_bits_of_f32(hip, batch, group):
+    """The root mean square of the errors, each over the root of its products'
+    squares. Partial sums are about that root; some 60 sums of a value each round
+    to 2^-24 of it (random: 5 2^-24), 22-bit inputs add 2.3 2^-24: 2^-20 in all is
+    twice that. (Sums of 17 bits give 2^-17.)"""
+    d = 4096
+    w = weights(300, d, group, True)
+    packed, dense = on_gpu(hip, w), ref.w4_dense(*w)
+    x = inputs(batch, d, torch.float32)
+    g = torch.Generator().manual_seed(6)
+    c = torch.randint(-127, 128, (batch, d), dtype=torch.int8, generator=g)
+    s = torch.rand((batch, d // 128), generator=g) + 0.1
+    wide = ref.f64(c) * ref.f64(s).repeat_interleave(128, 1)
+    for out, v in ((run(hip, w, packed, x), ref.f64(x)),
+                   (run(hip, w, packed, c.cuda(), torch.float32, s.cuda()), wide)):
+        error = (ref.f64(out) - v @ dense.T) / torch.sqrt((v * v) @ (dense * dense).T)
+        assert float(error.square().mean().sqrt()) < 2.0 ** -20

@@ -1,4 +1,5 @@
-"""Builds libmivi_hip.so (HIP kernels + C ABI) for gfx950, in-tree.
+"""Builds libmivi_hip.so (HIP kernels + C ABI) for gfx950, in-tree, and the
+Python binding of its step calls (_step.so).
 
     python mivi-v4_amd/build.py            # incremental
     python mivi-v4_amd/build.py --force    # rebuild everything
@@ -82,7 +83,29 @@ def build(force: bool = False) -> str:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("link failed")
     shutil.move(tmp, OUT)
+    _binding(force)
     return OUT
+
+
+def _binding(force: bool) -> None:
+    """mivi_hip/_step.so: tensors to calls for the installed torch and Python."""
+    import sysconfig
+
+    import torch
+
+    src, out = os.path.join(CSRC, "step_calls.cpp"), os.path.join(HERE, "mivi_hip", "_step.so")
+    if not force and os.path.exists(out) and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in _deps(src)):
+        return
+    t = os.path.dirname(torch.__file__)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + sysconfig.get_paths()["include"], "-isystem", os.path.join(t, "include"), src, "-o", out + ".tmp",
+           "-L" + os.path.dirname(OUT), "-lmivi_hip", "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(t, "lib"), "-ltorch_python",
+           "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("compile failed: step_calls.cpp")
+    shutil.move(out + ".tmp", out)
 
 
 if __name__ == "__main__":

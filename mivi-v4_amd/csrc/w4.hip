@@ -196,18 +196,25 @@ template <>
 struct Raw<X_I8> { u32x2 v[1]; };
 
 template <int X>
-__device__ __forceinline__ Raw<X> load_x(const W4Args& a, int b, int k) {
+constexpr int kXBytes = X == X_I8 ? 1 : X == X_F32 ? 4 : 2;
+template <int X>
+__device__ __forceinline__ const uint8_t* x_at(const W4Args& a, int b, int k) {
+    return (const uint8_t*)a.x + ((int64_t)b * a.x_row + k) * kXBytes<X>;
+}
+template <int X>
+__device__ __forceinline__ Raw<X> load_x(const uint8_t* p) {
     Raw<X> r;
-    const int64_t at = (int64_t)b * a.x_row + min(k, a.cols - 8);
     if constexpr (X == X_I8) {
-        r.v[0] = *(const u32x2_a1*)((const int8_t*)a.x + at);
-    } else if constexpr (X == X_F32) {
-        r.v[0] = *(const u32x4_a1*)((const float*)a.x + at);
-        r.v[1] = *(const u32x4_a1*)((const float*)a.x + at + 4);
+        r.v[0] = *(const u32x2_a1*)p;
     } else {
-        r.v[0] = *(const u32x4_a1*)((const uint16_t*)a.x + at);
+        r.v[0] = *(const u32x4_a1*)p;
+        if constexpr (X == X_F32) r.v[1] = *(const u32x4_a1*)(p + 16);
     }
     return r;
+}
+template <int X>
+__device__ __forceinline__ Raw<X> load_x(const W4Args& a, int b, int k) {
+    return load_x<X>(x_at<X>(a, b, min(k, a.cols - 8)));
 }
 template <int X>
 __device__ __forceinline__ void blank(Raw<X>* r, bool in) {
@@ -500,6 +507,10 @@ __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
     const int phases = (a.steps + a.wk - 1) / a.wk;
     const int64_t first = (int64_t)(live ? tile : 0) * a.steps;
 
+    const int full = a.cols / (a.wk * kStep);  // phases with no columns behind the last
+    const uint8_t* xp[ITEMS];
+#pragma unroll
+    for (int e = 0; e < ITEMS; e++) xp[e] = x_at<X>(a, b0 + min(bx + e * b_step, count - 1), 0);
     Raw<X> raw[ITEMS];
     float xs_raw[2];  // 8-bit x: scales of (inputs x units); count wk <= 16 kItems kWaves / 4, so two a thread do
     const int nu = a.wk * U;
@@ -513,11 +524,10 @@ __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
                 }
             }
         }
+        const int64_t at = (int64_t)min(ph * a.wk * kStep + c8 * 8, a.cols - 8) * kXBytes<X>;
 #pragma unroll
-        for (int e = 0; e < ITEMS; e++) {
-            const int b = bx + e * b_step;
-            if (e * b_step < count) raw[e] = load_x<X>(a, b0 + min(b, count - 1), ph * a.wk * kStep + c8 * 8);
-        }
+        for (int e = 0; e < ITEMS; e++)
+            if (e * b_step < count) raw[e] = load_x<X>(xp[e] + at);
     };
     const auto store = [&](int ph) {
         uint8_t* to = lds + (ph & 1) * buffer;
@@ -525,7 +535,7 @@ __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
         for (int e = 0; e < ITEMS; e++) {
             const int b = bx + e * b_step;
             if (b < count) {
-                blank<X>(&raw[e], (ph * a.wk * 16 + c8) * 8 < a.cols);
+                if (ph >= full) blank<X>(&raw[e], (ph * a.wk * 16 + c8) * 8 < a.cols);
                 Operand<X> o[PARTS];
                 operands<X>(raw[e], o);
 #pragma unroll

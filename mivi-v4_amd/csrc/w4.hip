@@ -20,8 +20,8 @@
 //           64 columns, or the step where groups have 128 or more;
 //   zeros   [tile][step][row][unit] bytes, where there are zeros.
 //
-// A workgroup has 8 waves: wk of them share a tile's steps, 8 / wk tiles. x goes
-// through LDS in operand order, [32 columns][q][column of the product].
+// A workgroup has 8 or 16 waves: wk of them share a tile's steps. x goes through
+// LDS in operand order, [32 columns][q][column of the product].
 #include <algorithm>
 
 #include "rows.h"
@@ -39,7 +39,8 @@ typedef uint32_t u32_a1 __attribute__((aligned(1)));
 constexpr int kWaves = 8;
 constexpr int kStep = 128;   // columns of a step
 constexpr int kRing = 3;     // steps of a wave in flight (w4_rows_kernel)
-constexpr int kItems = 8;    // pieces of x a thread stages, half of them of f32
+// pieces of x a thread stages at most
+constexpr int items_of(int x, int waves) { return (waves == 8 ? 8 : 5) / (x == 2 ? 2 : 1); }
 constexpr size_t kLds = 128 * 1024, kLdsFew = 156 * 1024;
 
 enum XKind { X_F16, X_BF16, X_F32, X_I8 };
@@ -483,17 +484,20 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
 }
 
 // More inputs, or deeper rows: NT tiles of 16 columns; x goes through LDS, wk
-// steps of it at a time in two buffers, [32 columns][q][column of the product],
-// loaded into registers a phase ahead.
-template <int X, int U, int W, int NT>
-__global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
+// steps of it at a time, [32 columns][q][column of the product], loaded into
+// registers a phase ahead. 8 waves have two buffers and one barrier a phase; 16
+// have one buffer and two barriers, but four waves a SIMD, whose loads from LDS,
+// products and sums overlap better.
+template <int X, int U, int W, int NT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
+    constexpr int BUFFERS = WAVES == 8 ? 2 : 1, RING = WAVES == 8 ? kRing : 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr int XB = X == X_I8 ? 8 : 16, PARTS = parts_of(X), PER = 4 / U;
-    constexpr int ITEMS = X == X_F32 ? kItems / 2 : kItems;
+    constexpr int ITEMS = items_of(X, WAVES);
     typedef typename std::conditional<X == X_I8, i32x4, f32x4>::type D;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave % a.wk, wm = wave / a.wk;
-    const int wms = kWaves / a.wk, tile = blockIdx.x * wms + wm;
+    const int wms = WAVES / a.wk, tile = blockIdx.x * wms + wm;
     const bool live = tile < a.tiles;
     const int b0 = blockIdx.y * a.block, count = min(a.block, a.batch - b0), cols_x = count * PARTS;
     int col[NT];  // columns behind the last repeat it: their results are not used
@@ -503,7 +507,7 @@ __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
     const int xs_at = a.wk * 16 * pitch;  // 8-bit x: its scales behind the codes
     const int buffer = (xs_at + (X == X_I8 ? a.wk * cols_x * 4 * U : 0) + 15) / 16 * 16;
     // a thread stages 8 columns of every (threads / pieces of an input)-th input
-    const int n8 = a.wk * 16, c8 = tid & (n8 - 1), bx = tid / n8, b_step = kWaves * 64 / n8;
+    const int n8 = a.wk * 16, c8 = tid & (n8 - 1), bx = tid / n8, b_step = WAVES * 64 / n8;
     const int phases = (a.steps + a.wk - 1) / a.wk;
     const int64_t first = (int64_t)(live ? tile : 0) * a.steps;
 
@@ -512,14 +516,14 @@ __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
 #pragma unroll
     for (int e = 0; e < ITEMS; e++) xp[e] = x_at<X>(a, b0 + min(bx + e * b_step, count - 1), 0);
     Raw<X> raw[ITEMS];
-    float xs_raw[2];  // 8-bit x: scales of (inputs x units); count wk <= 16 kItems kWaves / 4, so two a thread do
+    float xs_raw[2];  // 8-bit x: scales of (inputs x units); count wk <= 16 kItems WAVES / 4, so two a thread do
     const int nu = a.wk * U;
     const auto load = [&](int ph) {
         if constexpr (X == X_I8) {
             if (a.x_shift >= 0) {
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const int i = tid + e * kWaves * 64, u = i & (nu - 1);
+                    const int i = tid + e * WAVES * 64, u = i & (nu - 1);
                     xs_raw[e] = x_scale<U>(a, b0 + min(i / nu, count - 1), ph * a.wk + u / U, u % U);
                 }
             }
@@ -530,7 +534,7 @@ __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
             if (e * b_step < count) raw[e] = load_x<X>(xp[e] + at);
     };
     const auto store = [&](int ph) {
-        uint8_t* to = lds + (ph & 1) * buffer;
+        uint8_t* to = lds + (BUFFERS == 2 ? (ph & 1) * buffer : 0);
 #pragma unroll
         for (int e = 0; e < ITEMS; e++) {
             const int b = bx + e * b_step;
@@ -546,7 +550,7 @@ __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
             if (a.x_shift >= 0) {
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const int i = tid + e * kWaves * 64, b = i / nu;
+                    const int i = tid + e * WAVES * 64, b = i / nu;
                     if (b < count) ((float*)(to + xs_at))[(i & (nu - 1)) * cols_x + b] = xs_raw[e];
                 }
             }
@@ -556,26 +560,26 @@ __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
     f32x4 acc[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) acc[n] = f32x4{0, 0, 0, 0};
-    Step<W, true> w[kRing];
+    Step<W, true> w[RING];
     load(0);
     const auto refill = [&](int slot, int ph) {  // behind the last step it is loaded again
         fetch<W, true>(a, first + min(wk + ph * a.wk, a.steps - 1), lane, &w[slot]);
     };
 #pragma unroll
-    for (int p = 0; p < kRing; p++) refill(p, p);
+    for (int p = 0; p < RING; p++) refill(p, p);
     store(0);
 
-    for (int base = 0; base < phases; base += kRing) {
+    for (int base = 0; base < phases; base += RING) {
 #pragma unroll
-        for (int p = 0; p < kRing; p++) {
+        for (int p = 0; p < RING; p++) {
             const int ph = base + p;
             if (ph >= phases) break;
             __syncthreads();  // this phase's x is there, the phase before is read
             if (ph + 1 < phases) load(ph + 1);
             if (live && wk + ph * a.wk < a.steps) {
                 const Step<W, true>& c = w[p];
-                const uint8_t* xl = lds + (ph & 1) * buffer + (wk * 16 + q) * pitch;
-                const float* xs = (const float*)(lds + (ph & 1) * buffer + xs_at) + wk * U * cols_x;
+                const uint8_t* xl = lds + (BUFFERS == 2 ? (ph & 1) * buffer : 0) + (wk * 16 + q) * pitch;
+                const float* xs = (const float*)(lds + (BUFFERS == 2 ? (ph & 1) * buffer : 0) + xs_at) + wk * U * cols_x;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     D d[NT];
@@ -602,7 +606,8 @@ __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
                     }
                 }
             }
-            refill(p, ph + kRing);
+            refill(p, ph + RING);
+            if (BUFFERS == 1) __syncthreads();  // this phase's x is read
             if (ph + 1 < phases) store(ph + 1);
         }
     }
@@ -611,7 +616,7 @@ __global__ __launch_bounds__(kWaves * 64) void w4_rows_kernel(W4Args a) {
 #pragma unroll
     for (int n = 0; n < NT; n++) *(f32x4*)(red + ((wave * NT + n) * 16 + r) * 16 + q * 4) = acc[n];
     __syncthreads();
-    store_tiles<X, PARTS, kWaves>(a, red, blockIdx.x * wms, b0, count, 16 * NT);
+    store_tiles<X, PARTS, WAVES>(a, red, blockIdx.x * wms, b0, count, 16 * NT);
 }
 
 // ------------------------------------------------------------------ packing
@@ -674,6 +679,12 @@ int32_t packed_of(size_t rows, size_t cols, size_t group, bool zeros, Packed* p)
     return MIVI_OK;
 }
 
+// Whether w4_rows_kernel has a form of 16 waves for nt tiles of columns: where 128
+// registers hold it.
+constexpr bool rows_of_16(int x, int units, int nt) {
+    return nt >= 2 && nt <= 5 && (x != X_I8 || units * nt <= 6);
+}
+
 // How a product is laid out: w4_few_kernel, or w4_rows_kernel with nt tiles of
 // columns.
 struct W4Plan {
@@ -686,7 +697,13 @@ struct W4Plan {
 
 template <int X, int U, int W>
 void launch_rows(const W4Args& a, const W4Plan& p, hipStream_t s) {
-#define ROWS(N) w4_rows_kernel<X, U, W, N><<<p.grid, kWaves * 64, p.lds, s>>>(a)
+#define ROWS(N)                                                                                     \
+    if constexpr (rows_of_16(X, U, N))                                                              \
+        if (p.waves == 16) {                                                                        \
+            w4_rows_kernel<X, U, W, N, 16><<<p.grid, 1024, p.lds, s>>>(a);                          \
+            break;                                                                                  \
+        }                                                                                           \
+    w4_rows_kernel<X, U, W, N, 8><<<p.grid, 512, p.lds, s>>>(a)
     switch (p.nt) {
         case 1: ROWS(1); break;
         case 2: ROWS(2); break;
@@ -754,28 +771,34 @@ W4Plan w4_plan(W4Args* a, int x, int units, size_t batch, size_t tiles, size_t s
         }
     }
     const size_t parts = parts_of(x);
-    // Blocks of inputs and waves of a tile by an estimate: a phase takes 1.2 us and
-    // 0.06 a tile of columns where a CU has one workgroup (staging, products and
-    // the barrier in turn), 0.35 and 0.2 where workgroups share it.
+    // Blocks of inputs, waves of a workgroup and of a tile by an estimate. A phase
+    // of 8 waves takes 1.2 us and 0.06 a tile of columns where a CU has one workgroup
+    // (staging, products and the barrier in turn), 0.35 and 0.2 where two share it;
+    // of 16 waves, which have twice the steps, 1.35 and 0.28. (80 bf16 inputs, 14336 x
+    // 4096, groups of 32: one block and 16 waves 29.8 us, 8 waves 34.5, two blocks of
+    // 8 waves 52; 4096 x 14336, groups of 128: two blocks and 16 waves 30.6, one 34.0,
+    // of 8 waves 38 and 85. 512 inputs: blocks of 128 and 8 waves 124, of 74 138.)
     double best = 0;
     for (const int nt : {1, 2, 3, 4, 5, 8}) {
         const size_t most = 16 * nt / parts, blocks = (batch + most - 1) / most, block = (batch + blocks - 1) / blocks;
         if (best > 0 && (block * parts + 15) / 16 * 2 <= (size_t)nt) break;  // the batch has no more columns
         const size_t step_bytes = 16 * (block * parts * (x == X_I8 ? 8 : 16) + 16) + (x == X_I8 ? 4 * units * block : 0);
-        for (int wk = 1; wk <= kWaves; wk *= 2) {
-            const size_t items = (block * wk * 16 + kWaves * 64 - 1) / (kWaves * 64);
-            const size_t buffers = 2 * ((wk * step_bytes + 15) / 16 * 16);
-            if (wk > 1 && (buffers > kLds || items > (size_t)(x == X_F32 ? kItems / 2 : kItems))) break;
-            const size_t lds = std::max<size_t>(buffers, (size_t)kWaves * nt * 1024), phases = (steps + wk - 1) / wk;
-            const size_t fit = nt <= 3 && lds <= 80 * 1024 ? 2 : 1, grid_x = (tiles * wk + kWaves - 1) / kWaves;
+        for (int form = 0; form < 9; form++) {
+            const int waves = form < 4 ? 8 : 16, wk = form < 4 ? 1 << form : 1 << (form - 4);
+            if (waves == 16 && !rows_of_16(x, units, nt)) break;
+            const size_t items = (block * wk * 16 + waves * 64 - 1) / (waves * 64);
+            const size_t buffers = (waves == 8 ? 2 : 1) * ((wk * step_bytes + 15) / 16 * 16);
+            if ((wk > 1 || waves == 16) && (buffers > kLds || items > (size_t)items_of(x, waves))) continue;
+            const size_t lds = std::max<size_t>(buffers, (size_t)waves * nt * 1024), phases = (steps + wk - 1) / wk;
+            const size_t fit = waves == 8 && nt <= 3 && lds <= 80 * 1024 ? 2 : 1, grid_x = (tiles * wk + waves - 1) / waves;
             const size_t of_cu = (grid_x * blocks + cus - 1) / cus;
             const double staging = x == X_F32 ? 0.1 * (double)items : 0;
-            const double alone = 1.2 + 0.06 * nt + staging, shared = 0.35 + 0.2 * nt + staging;
+            const double alone = (waves == 8 ? 1.2 + 0.06 * nt : 1.35 + 0.28 * nt) + staging, shared = 0.35 + 0.2 * nt + staging;
             const double us = (double)phases * ((double)(of_cu / fit) * std::max(alone, (double)fit * shared) +
                                                 (of_cu % fit ? alone : 0.0));
             if (best == 0 || us < best) {
                 best = us;
-                p.nt = nt, p.lds = lds, a->wk = wk, a->block = (int)block;
+                p.nt = nt, p.lds = lds, p.waves = waves, a->wk = wk, a->block = (int)block;
                 p.grid = dim3((unsigned)std::min<size_t>(grid_x, UINT32_MAX), (unsigned)std::min<size_t>(blocks, 65536));
             }
         }
@@ -799,7 +822,7 @@ int32_t run_w4(W4Args a, int x, int32_t type, void* out, size_t out_len, size_t 
     if (batch == 0) return clear_error();
     const int units = std::max((int)p.units, x_units);
     W4Plan plan = w4_plan(&a, x, units, batch, p.tiles, p.steps);
-    if (!grid_fits(plan.grid.x, kWaves * 64) || plan.grid.y > 65535) return err_overflow();
+    if (!grid_fits(plan.grid.x, 1024) || plan.grid.y > 65535) return err_overflow();
     clear_error();
     a.codes = packed, a.scales = packed + p.codes, a.zeros = zeros ? packed + p.codes + p.scales : packed;
     a.has_zeros = zeros;

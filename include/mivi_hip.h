@@ -331,7 +331,7 @@ int32_t mivi_hip_rms_norm_q8(int32_t type, uint8_t* codes, size_t codes_len, flo
  * one turns back), or, with positions NULL, its position in the batch of starts
  * and lens that mivi_hip_kv_q4_append takes next (rows outside it are left
  * alone). Either of q and k may have no heads. Angles are taken in 64 bits at any
- * position, the rest is f32. head_dim up to 1024. */
+ * position, the rest is f32. head_dim up to 512. */
 int32_t mivi_hip_rope(int32_t type, void* q_out, size_t q_out_len, size_t q_out_row_stride,
                       size_t q_out_head_stride, const void* q, size_t q_len, size_t q_row_stride,
                       size_t q_head_stride, size_t n_heads, void* k_out, size_t k_out_len,
@@ -380,7 +380,8 @@ int32_t mivi_hip_w4_pack(const uint8_t* codes, size_t codes_len, int32_t scale_t
  * batches, 24, any of them to no less than 2^-40 of the largest magnitude of 128
  * columns; c - z enters exactly, sums and scales are f32 (a group's sum of (c -
  * z) x has to be an f32 number). The order of a row's sums, and so its last bits,
- * depends on the batch it is in. An infinity or NaN stays in its input's row. */
+ * depends on the batch it is in. An infinity or NaN stays in its input's row. out
+ * must not overlap x. */
 int32_t mivi_hip_w4_matmul_rows(int32_t type, void* out, size_t out_len, size_t out_row_stride,
                                 const uint8_t* packed, size_t packed_len, int32_t scale_type,
                                 int32_t has_zeros, const void* x, size_t x_len, size_t x_row_stride,
@@ -405,12 +406,13 @@ int32_t mivi_hip_w4_matmul_rows_q8(int32_t type, void* out, size_t out_len, size
  * first index whose cumulative sum passes pick[s] times the whole. With accept
  * and pick uniform in [0, 1) the tokens have the target's distribution.
  * tokens[rows]: the accepted ones, the drawn one (-1 where the row has no
- * probability above 0) and -1 behind it; counts[n_seq]: accepted ones. Rows need
- * not sum to 1; what is negative, infinite or NaN counts as 0; a drafted id
- * outside 0 .. n - 1 is not accepted. Comparisons are exact, sums of 64 bits in a
- * fixed order. A sequence without rows has count 0; rows outside the sequences
- * are left alone. n_seq at most 65535. workspace: 16-byte aligned, of
- * mivi_hip_verify_rows_workspace bytes, as mivi_hip_kv_q4_attention's. */
+ * probability above 0) and -1 behind it (tokens may be drafted itself);
+ * counts[n_seq]: accepted ones. Rows need not sum to 1; what is negative,
+ * infinite or NaN counts as 0; a drafted id outside 0 .. n - 1 is not accepted.
+ * Comparisons are exact, sums of 64 bits in a fixed order. A sequence without
+ * rows has count 0; rows outside the sequences are left alone. n_seq at most
+ * 65535. workspace: 16-byte aligned, of mivi_hip_verify_rows_workspace bytes, as
+ * mivi_hip_kv_q4_attention's. */
 size_t mivi_hip_verify_rows_workspace(size_t n, size_t n_seq);
 int32_t mivi_hip_verify_rows(int32_t* tokens, size_t tokens_len, int32_t* counts, size_t counts_len,
                              const float* target, size_t target_len, size_t target_row_stride,

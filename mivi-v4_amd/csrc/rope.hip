@@ -159,8 +159,8 @@ extern "C" int32_t mivi_hip_rope(int32_t type, void* q_out, size_t q_out_len, si
     if (!type_bytes(type)) return err_unsupported(type);
     if (n_heads + n_kv_heads == 0 || n_heads > 65535 || n_kv_heads > 65535)
         return set_error(MIVI_ERR_INVALID_ARGUMENT, "%zu heads and %zu kv heads", n_heads, n_kv_heads);
-    if (head_dim == 0 || head_dim > 1024)
-        return set_error(MIVI_ERR_INVALID_ARGUMENT, "heads of %zu dimensions (1 to 1024)", head_dim);
+    if (head_dim == 0 || head_dim > 512)  // a head's units are lanes of one wave
+        return set_error(MIVI_ERR_INVALID_ARGUMENT, "heads of %zu dimensions (1 to 512)", head_dim);
     if (rot_dim % 2) return err_misaligned(rot_dim, 2);
     if (rot_dim == 0 || rot_dim > head_dim)
         return set_error(MIVI_ERR_INVALID_ARGUMENT, "%zu of %zu dimensions turned", rot_dim, head_dim);
@@ -187,6 +187,8 @@ extern "C" int32_t mivi_hip_rope(int32_t type, void* q_out, size_t q_out_len, si
         (rc = check_in_place("k", k_out, k_out_row_stride, k_out_head_stride, k, k_row_stride, k_head_stride, rows,
                              n_kv_heads)))
         return rc;
+    if (n_heads && n_kv_heads && q_out == k_out)
+        return set_error(MIVI_ERR_INVALID_ARGUMENT, "q_out and k_out are one tensor");
     RopeArgs a = {};
     a.q = q, a.k = k, a.q_out = q_out, a.k_out = k_out;
     a.q_row = (int64_t)q_row_stride, a.q_head = (int64_t)q_head_stride;

@@ -183,6 +183,7 @@ int32_t rope(PyObject* const* a) {
     if (half < 0) throw Raised();
     const float scale = number(a[8]);
     void* stream = handle(a[0]);
+    if (n == 0) return MIVI_OK;  // no address stands for no positions
     const Unlocked u;
     return mivi_hip_rope(type_of(*one), out[0].p, out[0].span, out[0].row, out[0].head, in[0].p, in[0].span, in[0].row,
                          in[0].head, heads[0], out[1].p, out[1].span, out[1].row, out[1].head, in[1].p, in[1].span,

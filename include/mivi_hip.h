@@ -310,12 +310,12 @@ int32_t mivi_hip_rms_norm(int32_t type, void* out, size_t out_len, size_t out_ro
                           size_t dim, void* stream);
 
 /* The same in 8 bits, for mivi_hip_w4_matmul_rows_q8: codes [rows][dim] (signed
- * bytes) and scales [rows][dim / group]; group 32, 64, 128, 256 or 512 dimensions, or 0 for
- * one scale a row. With A the group's largest |s w|: code = 127 s w / A rounded
- * to nearest (ties to even), scale = A / sqrt(mean s^2 + eps) / 127, so codes
- * are those of exact arithmetic in s w. A group of zeros has scale 0; a row with
- * an infinity or NaN in s, and a group with one in s w, has codes 0 and scale
- * NaN. */
+ * bytes) and scales [rows][dim / group]; group 32, 64, 128, 256 or 512
+ * dimensions, or 0 for one scale a row. With A the group's largest |s w|: code =
+ * 127 s w / A rounded to nearest (ties to even) in 64 bits, scale = A / sqrt(mean
+ * s^2 + eps) / 127: codes depend on s w alone, in no order of sums. A group of
+ * zeros has scale 0; a row with an infinity or NaN in s, and a group with one in
+ * s w, has codes 0 and scale NaN. */
 int32_t mivi_hip_rms_norm_q8(int32_t type, uint8_t* codes, size_t codes_len, float* scales,
                              size_t scales_len, size_t group, const void* x, size_t x_len,
                              size_t x_row_stride, const void* residual, size_t residual_len,

@@ -3,11 +3,10 @@
 // zeros; x in f32, f16 or bf16, or as 8-bit codes with scales.
 //
 // On the matrix cores, whatever the batch: c - z is a small integer and enters
-// them exactly, as fp16 (x in fp16), bf16 (x in bf16; x in f32 as three bf16
-// parts, 24 bits, that take three columns of the product) or int8 (8-bit x),
-// 32 columns a product; a group's sum is multiplied by its scale in f32 (8-bit
-// x: an exact integer by the product of both scales). Scaling the weights first
-// would round every one of them.
+// them exactly, as fp16 (x in fp16, and in f32 as two fp16 parts, which take two
+// columns of the product), bf16 or int8 (8-bit x), 32 columns a product; a group's
+// sum is multiplied by its scale in f32 (8-bit x: an exact integer by the product
+// of both scales). Scaling the weights first would round every one of them.
 //
 // Packed layout (mivi_hip_w4_pack), tiles of 16 rows, steps of 128 columns,
 // padded with codes and scales of 0:
@@ -44,7 +43,7 @@ constexpr int items_of(int x, int waves) { return (waves == 8 ? 8 : 5) / (x == 2
 constexpr size_t kLds = 128 * 1024, kLdsFew = 156 * 1024;
 
 enum XKind { X_F16, X_BF16, X_F32, X_I8 };
-constexpr int parts_of(int x) { return x == X_F32 ? 3 : 1; }
+constexpr int parts_of(int x) { return x == X_F32 ? 2 : 1; }  // columns of the product that an input takes
 
 struct W4Args {
     const uint8_t *codes, *scales, *zeros;  // planes of the packed weights (zeros: the codes where there are none)
@@ -225,24 +224,14 @@ __device__ __forceinline__ void blank(Raw<X>* r, bool in) {
         for (int j = 0; j < (X == X_I8 ? 2 : 4); j++) r->v[i][j] = in ? r->v[i][j] : 0u;
 }
 
-// Its operands, one a part.
+// It as an operand (f16, bf16 and 8-bit x).
 template <int X>
-__device__ __forceinline__ void operands(const Raw<X>& r, Operand<X> (&o)[parts_of(X)]) {
+__device__ __forceinline__ void operand(const Raw<X>& r, Operand<X>* o) {
     if constexpr (X == X_I8) {
-        o[0].v = u32x2{__builtin_amdgcn_perm(r.v[0].y, r.v[0].x, 0x05010400),
+        o->v = u32x2{__builtin_amdgcn_perm(r.v[0].y, r.v[0].x, 0x05010400),
                        __builtin_amdgcn_perm(r.v[0].y, r.v[0].x, 0x07030602)};
-    } else if constexpr (X == X_F32) {
-        bf16x8 p[3];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            __bf16 p0, p1, p2;
-            split_bf16(__uint_as_float(r.v[e / 4][e % 4]), p0, p1, p2);
-            p[0][e] = p0, p[1][e] = p1, p[2][e] = p2;
-        }
-#pragma unroll
-        for (int j = 0; j < 3; j++) o[j].v = __builtin_bit_cast(u32x4, p[j]);
     } else {
-        o[0].v = r.v[0];
+        o->v = r.v[0];
     }
 }
 
@@ -292,7 +281,6 @@ __device__ __forceinline__ void store_tiles(const W4Args& a, const float* red, i
 // of 64 with zeros 17.2 us, 4.2 TB/s, the vector pipe 65 % of the cycles; eight 8-bit
 // ones over 28672 x 8192 26.5 us, 4.6 TB/s, 43 %; one f32 input over 8192 x 2048 5.9, a
 // chain of x's load, its conversion, four steps and the join.
-constexpr int few_parts(int x) { return x == X_F32 ? 2 : 1; }
 constexpr int kFewRing = 4;  // steps of a wave in flight
 
 struct FewArgs {
@@ -319,10 +307,10 @@ __device__ __forceinline__ float unit_sum(float v) {
     return v;
 }
 
-// 8 columns of an input as operands, and what the step's results are to be
-// multiplied by. 16 lanes have a step.
+// 8 columns of a bf16 or f32 input as fp16 operands, and what the step's results
+// are to be multiplied by. 16 lanes have a step.
 template <int X>
-__device__ __forceinline__ void few_operands(const Raw<X>& r, Operand<X_F16> (&o)[few_parts(X)], float* factor) {
+__device__ __forceinline__ void scaled_operands(const Raw<X>& r, Operand<X_F16> (&o)[parts_of(X)], float* factor) {
     float v[8];
     uint32_t top = 0;
 #pragma unroll
@@ -335,7 +323,7 @@ __device__ __forceinline__ void few_operands(const Raw<X>& r, Operand<X_F16> (&o
     const int ex = min(127 + 14 - ((int)(max16(top) >> 23) - 127), 253);
     const float up = __uint_as_float((uint32_t)ex << 23);
     *factor = __uint_as_float((uint32_t)(254 - ex) << 23);
-    half8 h[few_parts(X)];
+    half8 h[parts_of(X)];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         const float y = v[e] * up;
@@ -344,14 +332,14 @@ __device__ __forceinline__ void few_operands(const Raw<X>& r, Operand<X_F16> (&o
         if constexpr (X == X_F32) h[1][e] = (_Float16)(__builtin_fabsf(y) == __builtin_inff() ? 0.f : y - (float)h[0][e]);
     }
 #pragma unroll
-    for (int p = 0; p < few_parts(X); p++) o[p].v = __builtin_bit_cast(u32x4, h[p]);
+    for (int p = 0; p < parts_of(X); p++) o[p].v = __builtin_bit_cast(u32x4, h[p]);
 }
 
 template <int X, int U, int W, bool SB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr bool I8 = X == X_I8;
-    constexpr int PARTS = few_parts(X), PER = 4 / U, XB = I8 ? 8 : 16;
+    constexpr int PARTS = parts_of(X), PER = 4 / U, XB = I8 ? 8 : 16;
     typedef typename std::conditional<I8, i32x4, f32x4>::type D;
     const W4Args& a = g.w;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
@@ -390,12 +378,12 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
             if constexpr (I8) {
                 const int unit = (c >> 4) * U + (c & 15) / (16 / U);
                 const bool head = at[e] >= 0 && (c & (16 / U - 1)) == 0;
-                Operand<X> o[1];
-                operands<X>(raw[e], o);
-                int s = __builtin_amdgcn_sdot4((int)o[0].v.x, 0x01010101, 0, false);
-                s = __builtin_amdgcn_sdot4((int)o[0].v.y, 0x01010101, s, false);
+                Operand<X> o;
+                operand<X>(raw[e], &o);
+                int s = __builtin_amdgcn_sdot4((int)o.v.x, 0x01010101, 0, false);
+                s = __builtin_amdgcn_sdot4((int)o.v.y, 0x01010101, s, false);
                 const float sum = unit_sum<U>((float)s);  // whole numbers far below 2^24
-                if (at[e] >= 0) *(Operand<X>*)to = o[0];
+                if (at[e] >= 0) *(Operand<X>*)to = o;
                 if (head) {
                     sums[unit * cols_x + b] = (int)sum;
                     factors[unit * cols_x + b] = a.x_shift < 0 ? 1.f : x_scale<U>(a, b, c >> 4, unit & (U - 1));
@@ -404,7 +392,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
                 Operand<X_F16> o[PARTS];
                 float factor = 1.f;
                 if constexpr (X == X_F16) o[0].v = raw[e].v[0];
-                else few_operands<X>(raw[e], o, &factor);
+                else scaled_operands<X>(raw[e], o, &factor);
 #pragma unroll
                 for (int p = 0; p < PARTS; p++) {
                     if (at[e] >= 0) *(Operand<X_F16>*)(to + p * XB) = o[p];
@@ -503,7 +491,7 @@ template <int X, int U, int W, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
     constexpr int BUFFERS = WAVES == 8 ? 2 : 1, RING = WAVES == 8 ? kRing : 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    constexpr bool I8 = X == X_I8;
+    constexpr bool I8 = X == X_I8, SCALED = X == X_F32;
     constexpr int XB = I8 ? 8 : 16, PARTS = parts_of(X), PER = 4 / U;
     constexpr int ITEMS = items_of(X, WAVES);
     typedef typename std::conditional<X == X_I8, i32x4, f32x4>::type D;
@@ -521,8 +509,8 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
     int slot[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) slot[j] = (r ^ q ^ 4 * j) * XB + j * 4 * pitch;
-    const int xs_at = a.wk * 16 * pitch;  // 8-bit x: its scales behind the codes
-    const int buffer = (xs_at + (X == X_I8 ? a.wk * cols_x * 4 * U : 0) + 15) / 16 * 16;
+    const int xs_at = a.wk * 16 * pitch;  // behind x its scales (8-bit x) or factors (f32)
+    const int buffer = (xs_at + a.wk * cols_x * 4 * (I8 ? U : SCALED ? 1 : 0) + 15) / 16 * 16;
     // a thread stages 8 columns of every (threads / pieces of an input)-th input
     const int n8 = a.wk * 16, c8 = tid & (n8 - 1), bx = tid / n8, b_step = WAVES * 64 / n8;
     const int phases = (a.steps + a.wk - 1) / a.wk;
@@ -557,10 +545,20 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
             const int b = bx + e * b_step;
             if (b < count) {
                 if (ph >= full) blank<X>(&raw[e], (ph * a.wk * 16 + c8) * 8 < a.cols);
-                Operand<X> o[PARTS];
-                operands<X>(raw[e], o);
+                if constexpr (SCALED) {
+                    Operand<X_F16> o[PARTS];
+                    float factor;
+                    scaled_operands<X>(raw[e], o, &factor);
 #pragma unroll
-                for (int p = 0; p < PARTS; p++) *(Operand<X>*)(to + c8 * pitch + ((b * PARTS + p) ^ (c8 & 15)) * XB) = o[p];
+                    for (int p = 0; p < PARTS; p++) {
+                        *(Operand<X_F16>*)(to + c8 * pitch + ((b * PARTS + p) ^ (c8 & 15)) * XB) = o[p];
+                        if ((c8 & 15) == 0) ((float*)(to + xs_at))[(c8 >> 4) * cols_x + b * PARTS + p] = factor;
+                    }
+                } else {
+                    Operand<X> o;
+                    operand<X>(raw[e], &o);
+                    *(Operand<X>*)(to + c8 * pitch + (b ^ (c8 & 15)) * XB) = o;
+                }
             }
         }
         if constexpr (X == X_I8) {
@@ -596,7 +594,10 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
             if (live && wk + ph * a.wk < a.steps) {
                 const Step<W, true>& c = w[p];
                 const uint8_t* xl = lds + (BUFFERS == 2 ? (ph & 1) * buffer : 0) + (wk * 16 + q) * pitch;
-                const float* xs = (const float*)(lds + (BUFFERS == 2 ? (ph & 1) * buffer : 0) + xs_at) + wk * U * cols_x;
+                const float* xs = (const float*)(lds + (BUFFERS == 2 ? (ph & 1) * buffer : 0) + xs_at) + wk * (I8 ? U : 1) * cols_x;
+                f32x4 part[SCALED ? NT : 1];
+#pragma unroll
+                for (int n = 0; n < (SCALED ? NT : 1); n++) part[n] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     D d[NT];
@@ -605,10 +606,10 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
 #pragma unroll
                     for (int k = 0; k < PER; k++) {
                         const int j = u * PER + k;
-                        const Weights8<X> wv(c.codes[j], c.zeros[0] >> (8 * (u / (U / W))) & 15);
+                        const Weights8<SCALED ? X_F16 : X> wv(c.codes[j], c.zeros[0] >> (8 * (u / (U / W))) & 15);
 #pragma unroll
                         for (int n = 0; n < NT; n++)
-                            d[n] = wv.times(*(const Operand<X>*)(xl + slot[j] + 16 * n * XB), d[n]);
+                            d[n] = wv.times(*(const Operand<SCALED ? X_F16 : X>*)(xl + slot[j] + 16 * n * XB), d[n]);
                     }
                     float f[4];
                     scales_f32(c.scales[u / (U / W)], a.bf16_scales, f);
@@ -619,7 +620,18 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
                             if (a.x_shift >= 0) m = xs[u * cols_x + min(16 * n + r, cols_x - 1)];
                         }
 #pragma unroll
-                        for (int i = 0; i < 4; i++) acc[n][i] = fmaf((float)d[n][i], X == X_I8 ? f[i] * m : f[i], acc[n][i]);
+                        for (int i = 0; i < 4; i++) {
+                            if constexpr (SCALED) part[n][i] = fmaf(d[n][i], f[i], part[n][i]);
+                            else acc[n][i] = fmaf((float)d[n][i], I8 ? f[i] * m : f[i], acc[n][i]);
+                        }
+                    }
+                }
+                if constexpr (SCALED) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const float m = xs[min(16 * n + r, cols_x - 1)];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[n][i] = fmaf(part[n][i], m, acc[n][i]);
                     }
                 }
             }
@@ -699,7 +711,7 @@ int32_t packed_of(size_t rows, size_t cols, size_t group, bool zeros, Packed* p)
 // Whether w4_rows_kernel has a form of 16 waves for nt tiles of columns: where 128
 // registers hold it.
 constexpr bool rows_of_16(int x, int units, int nt) {
-    return nt >= 2 && nt <= 5 && (x != X_I8 || units * nt <= 6);
+    return nt >= 2 && nt <= 5 && (x != X_I8 || units * nt <= 6) && (x != X_F32 || units == 1 || nt < 5);
 }
 
 // And one of 8 tiles of columns, by 256 registers.
@@ -766,7 +778,7 @@ W4Plan w4_plan(W4Args* a, int x, int units, size_t batch, size_t tiles, size_t s
     W4Plan p = {};
     const size_t cus = (size_t)num_cus();
     {
-        const size_t columns = batch * few_parts(x), xb = x == X_I8 ? 8 : 16;
+        const size_t columns = batch * parts_of(x), xb = x == X_I8 ? 8 : 16;
         // columns of a multiple of 64 bytes would store to the same banks
         const size_t pitch = columns * xb + (columns * xb % 64 ? 0 : 16);
         const size_t x_bytes = steps * 16 * pitch, sums = steps * columns * 4 * (x == X_I8 ? 2 * units : 1);
@@ -805,7 +817,8 @@ W4Plan w4_plan(W4Args* a, int x, int units, size_t batch, size_t tiles, size_t s
         if (nt == 8 && !rows_of_8(x, units)) break;
         const size_t most = 16 * nt / parts, blocks = (batch + most - 1) / most, block = (batch + blocks - 1) / blocks;
         if (best > 0 && (block * parts + 15) / 16 * 2 <= (size_t)nt) break;  // the batch has no more columns
-        const size_t step_bytes = 16 * rows_pitch(x == X_I8, nt) + (x == X_I8 ? 4 * units * block : 0);
+        const size_t step_bytes =
+            16 * rows_pitch(x == X_I8, nt) + 4 * block * (x == X_I8 ? units : x == X_F32 ? parts : 0);
         for (int form = 0; form < 9; form++) {
             const int waves = form < 4 ? 8 : 16, wk = form < 4 ? 1 << form : 1 << (form - 4);
             if (waves == 16 && !rows_of_16(x, units, nt)) break;
@@ -815,7 +828,7 @@ W4Plan w4_plan(W4Args* a, int x, int units, size_t batch, size_t tiles, size_t s
             const size_t lds = std::max<size_t>(buffers, (size_t)waves * nt * 1024), phases = (steps + wk - 1) / wk;
             const size_t fit = waves == 8 && nt <= 3 && lds <= 80 * 1024 ? 2 : 1, grid_x = (tiles * wk + waves - 1) / waves;
             const size_t of_cu = (grid_x * blocks + cus - 1) / cus;
-            const double staging = x == X_F32 ? 0.1 * (double)items : 0;
+            const double staging = x == X_F32 ? (waves == 8 ? 0.35 : 0.7) * (double)items : 0;  // the conversion
             const double alone = (waves == 8 ? 1.2 + 0.06 * nt : 1.35 + 0.28 * nt) + staging, shared = 0.35 + 0.2 * nt + staging;
             const double us = (double)phases * ((double)(of_cu / fit) * std::max(alone, (double)fit * shared) +
                                                 (of_cu % fit ? alone : 0.0));

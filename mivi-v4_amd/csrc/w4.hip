@@ -69,6 +69,14 @@ __device__ __forceinline__ void scales_f32(u32x2 s, bool bf16, float (&f)[4]) {
     }
 }
 
+// (w & mask) | bits in one instruction, which takes one scalar and no literal: the
+// compiler makes two of it, with literals.
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(bits));
+    return r;
+}
+
 // Eight weights c - z of a dword, in the order of the columns.
 __device__ __forceinline__ half8 weights_f16(uint32_t w, uint32_t z) {
     // a nibble in the low bits of 1024 is 1024 + c, in the next four 1024 + 16 c
@@ -76,11 +84,11 @@ __device__ __forceinline__ half8 weights_f16(uint32_t w, uint32_t z) {
     const half2v hi = __builtin_bit_cast(half2v, 0xD400D400u | z << 20 | z << 4);            // -(64 + z)
     const half2v sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
     union { half8 v; half2v h[4]; } r;
-    const uint32_t w8 = w >> 8;
-    r.h[0] = __builtin_bit_cast(half2v, (w & 0x000F000Fu) | 0x64006400u) - lo;
-    r.h[1] = __builtin_elementwise_fma(__builtin_bit_cast(half2v, (w & 0x00F000F0u) | 0x64006400u), sixteenth, hi);
-    r.h[2] = __builtin_bit_cast(half2v, (w8 & 0x000F000Fu) | 0x64006400u) - lo;
-    r.h[3] = __builtin_elementwise_fma(__builtin_bit_cast(half2v, (w8 & 0x00F000F0u) | 0x64006400u), sixteenth, hi);
+    const uint32_t w8 = w >> 8, k = 0x64006400u;
+    r.h[0] = __builtin_bit_cast(half2v, and_or(w, 0x000F000Fu, k)) - lo;
+    r.h[1] = __builtin_elementwise_fma(__builtin_bit_cast(half2v, and_or(w, 0x00F000F0u, k)), sixteenth, hi);
+    r.h[2] = __builtin_bit_cast(half2v, and_or(w8, 0x000F000Fu, k)) - lo;
+    r.h[3] = __builtin_elementwise_fma(__builtin_bit_cast(half2v, and_or(w8, 0x00F000F0u, k)), sixteenth, hi);
     return r.v;
 }
 // Byte K of w as a float; the compiler takes a nibble out first, two instructions.

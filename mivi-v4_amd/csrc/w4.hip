@@ -353,7 +353,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave % a.wk, wm = wave / a.wk;
     const int wms = WAVES / a.wk, stride = gridDim.x * wms, cols_x = a.batch * PARTS, col = min(r, cols_x - 1);
-    int* sums = (int*)(lds + g.sums);                               // of 8-bit x: [step][unit][column]
+    int* sums = (int*)(lds + g.sums);                               // of -x where it has 8 bits: [step][unit][column]
     float* factors = (float*)sums + (I8 ? a.steps * U * cols_x : 0);  // the same, of others [step][column]
 
     Step<W, !I8> w[kFewRing];
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
                 const float sum = unit_sum<U>((float)s);  // whole numbers far below 2^24
                 if (at[e] >= 0) *(Operand<X>*)to = o;
                 if (head) {
-                    sums[unit * cols_x + b] = (int)sum;
+                    sums[unit * cols_x + b] = -(int)sum;
                     factors[unit * cols_x + b] = a.x_shift < 0 ? 1.f : x_scale<U>(a, b, c >> 4, unit & (U - 1));
                 }
             } else {
@@ -452,7 +452,8 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
             for (int i = 0; i < 4; i++) {
                 if constexpr (I8) {
                     const int byte = i * W + u / per_w, z = (int)(c.zeros[byte / 4] >> (byte % 4 * 8) & 0xFF);
-                    acc[i] = fmaf((float)(d[u][i] - z * sum[u]), f[i] * m[u], acc[i]);
+                    // (a product of 24 bits and the sum in one instruction)
+                    acc[i] = fmaf((float)(d[u][i] + __mul24(z, sum[u])), f[i] * m[u], acc[i]);
                 } else if constexpr (X == X_F16) {
                     acc[i] = fmaf(d[u][i], f[i], acc[i]);
                 } else {

@@ -281,13 +281,13 @@ __device__ __forceinline__ void store_tiles(const W4Args& a, const float* red, i
 // their largest to 2^14 .. 2^15 (f32 in two parts, 22 bits; nothing to less than
 // 2^-40 of that largest). Against 8-bit x the weights enter as codes and z sum x
 // comes off their sums, all whole numbers. (With codes as the fp16 numbers c
-// 2^-24, masks alone, one input takes 4 to 10 % less, but sums have 17 bits: the
+// 2^-24, masks alone, one input takes up to 4 % less, but sums have 17 bits: the
 // matrix cores align products by their operands' exponents as if all were normal
 // numbers.)
 //
 // HBM and vector instructions bound it: one fp16 input over 65535 x 2048 in groups
-// of 64 with zeros 17.2 us, 4.2 TB/s, the vector pipe 65 % of the cycles; eight 8-bit
-// ones over 28672 x 8192 26.5 us, 4.6 TB/s, 43 %; one f32 input over 8192 x 2048 5.9, a
+// of 64 with zeros 17.0 us, 4.3 TB/s, the vector pipe 57 % of the cycles; eight 8-bit
+// ones over 28672 x 8192 26.4 us, 4.6 TB/s, 41 %; one f32 input over 8192 x 2048 5.9, a
 // chain of x's load, its conversion, four steps and the join.
 constexpr int kFewRing = 4;  // steps of a wave in flight
 

@@ -377,8 +377,9 @@ int32_t mivi_hip_w4_pack(const uint8_t* codes, size_t codes_len, int32_t scale_t
 
 /* out[batch][rows] = x[batch][cols] W^T, both in `type`. f16 and bf16 inputs
  * enter the products with all their bits, f32 ones with 22, any of them to no less
- * than 2^-40 of the largest magnitude of 128 columns; c - z enters exactly, sums and scales are f32 (a group's sum of (c -
- * z) x has to be an f32 number). The order of a row's sums, and so its last bits,
+ * than 2^-40 of the largest magnitude of 128 columns; c - z enters exactly, sums
+ * and scales are f32 (a group's sum of (c - z) x has to be an f32 number, a
+ * scale's magnitude below 2^100). The order of a row's sums, and so its last bits,
  * depends on the batch it is in. An infinity or NaN stays in its input's row. out
  * must not overlap x. */
 int32_t mivi_hip_w4_matmul_rows(int32_t type, void* out, size_t out_len, size_t out_row_stride,

@@ -706,7 +706,8 @@ int32_t packed_of(size_t rows, size_t cols, size_t group, bool zeros, Packed* p)
     if (group != 32 && group != 64 && group != cols && (group == 0 || group % kStep))
         return set_error(MIVI_ERR_INVALID_ARGUMENT, "groups of %zu (32, 64, a multiple of 128 or the whole row)", group);
     if (cols % group) return err_misaligned(cols, group);
-    if (rows > (size_t)INT32_MAX - 15 || cols > (size_t)INT32_MAX / 8) return err_overflow();
+    // (rows: the 16 tiles of a workgroup may reach 255 behind the last)
+    if (rows > (size_t)INT32_MAX - 1023 || cols > (size_t)INT32_MAX / 8) return err_overflow();
     p->tiles = (rows + 15) / 16, p->steps = (cols + kStep - 1) / kStep;
     p->units = group == 32 ? 4 : group == 64 ? 2 : 1;
     size_t cells, all;

@@ -175,6 +175,8 @@ def test_w4_sizes():
     for n, d, g in ((0, 256, 64), (16, 0, 64), (16, 250, 50), (16, 256, 0), (16, 256, 96), (16, 256, 192), (16, 320, 128),
                     (1 << 31, 256, 64), (16, 1 << 40, 64)):
         assert size(n, d, g, 0) == 0, (n, d, g)
+    # workgroups have up to 16 tiles: indexes of rows behind the last stay within 32 bits
+    assert size((1 << 31) - 1024, 32, 32, 0) == ((1 << 27) - 64) * (1024 + 128) and size((1 << 31) - 1023, 32, 32, 0) == 0
 
 
 @pytest.mark.parametrize("call", [pack, w4, w4_q8])

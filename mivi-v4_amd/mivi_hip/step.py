@@ -135,6 +135,10 @@ class W4Weights:
                 self.data = torch.empty(n, dtype=torch.uint8, device=d)
         self._args = (self.data, self.scale_type, int(self.has_zeros), self.rows, self.cols, self.group)
         kv_q4._call(_lib.mivi_hip_w4_pack, args + (self.data.data_ptr(), n, self.rows, self.cols, self.group), d, stream)
+        if stream is not None:  # the inputs' memory is another stream's: reused only behind this one's work
+            for t in (codes, scales, zeros):
+                if t is not None:
+                    t.record_stream(_stream_of(stream, d))
 
 
 def w4_matmul_rows(out, weights: W4Weights, x, x_scales=None, stream=None):

@@ -41,6 +41,9 @@ constexpr int kRing = 3;     // steps of a wave in flight (w4_rows_kernel)
 // pieces of x a thread stages at most
 constexpr int items_of(int x, int waves) { return (waves == 8 ? 8 : 5) / (x == 2 ? 2 : 1); }
 constexpr size_t kLds = 128 * 1024, kLdsFew = 156 * 1024;
+// inputs of a launch: in blocks of 8, the smallest, 2^15 of the 65535 that a grid's
+// second dimension may have
+constexpr size_t kMostInputs = (size_t)1 << 18;
 
 enum XKind { X_F16, X_BF16, X_F32, X_I8 };
 constexpr int parts_of(int x) { return x == X_F32 ? 2 : 1; }  // columns of the product that an input takes
@@ -845,7 +848,7 @@ W4Plan w4_plan(W4Args* a, int x, int units, size_t batch, size_t tiles, size_t s
             if (best == 0 || us < best) {
                 best = us;
                 p.nt = nt, p.lds = lds, p.waves = waves, a->wk = wk, a->block = (int)block;
-                p.grid = dim3((unsigned)std::min<size_t>(grid_x, UINT32_MAX), (unsigned)std::min<size_t>(blocks, 65536));
+                p.grid = dim3((unsigned)std::min<size_t>(grid_x, UINT32_MAX), (unsigned)blocks);
             }
         }
     }
@@ -867,23 +870,37 @@ int32_t run_w4(W4Args a, int x, int32_t type, void* out, size_t out_len, size_t 
     if ((uintptr_t)packed % 16) return set_error(MIVI_ERR_INVALID_ARGUMENT, "packed not 16-byte aligned");
     if (batch == 0) return clear_error();
     const int units = std::max((int)p.units, x_units);
-    W4Plan plan = w4_plan(&a, x, units, batch, p.tiles, p.steps);
-    if (!grid_fits(plan.grid.x, 1024) || plan.grid.y > 65535) return err_overflow();
-    clear_error();
     a.codes = packed, a.scales = packed + p.codes, a.zeros = zeros ? packed + p.codes + p.scales : packed;
     a.has_zeros = zeros;
-    a.out = out, a.out_row = (int64_t)out_row_stride, a.out_type = type;
-    a.rows = (int)rows, a.cols = (int)cols, a.batch = (int)batch;
+    a.out_row = (int64_t)out_row_stride, a.out_type = type;
+    a.rows = (int)rows, a.cols = (int)cols;
     a.tiles = (int)p.tiles, a.steps = (int)p.steps;
     a.w_units = (int)p.units, a.bf16_scales = scale_type == MIVI_GGML_BF16;
-    switch (x) {
-        case X_F16: launch_w4<X_F16>(a, units, (int)p.units, plan, s); break;
-        case X_BF16: launch_w4<X_BF16>(a, units, (int)p.units, plan, s); break;
-        case X_F32: launch_w4<X_F32>(a, units, (int)p.units, plan, s); break;
-        default: launch_w4<X_I8>(a, units, (int)p.units, plan, s); break;
+    // launches of `most` inputs, and one of those behind the last of them
+    const size_t most = std::min(batch, kMostInputs), left = batch % most;
+    W4Args args[2] = {a, a};
+    W4Plan plans[2];
+    for (int i = 0; i < (left ? 2 : 1); i++) {
+        args[i].batch = (int)(i ? left : most);
+        plans[i] = w4_plan(&args[i], x, units, args[i].batch, p.tiles, p.steps);
+        if (!grid_fits(plans[i].grid.x, 1024)) return err_overflow();
     }
-    MIVI_HIP_CHECK(hipGetLastError());
-    return MIVI_OK;
+    const size_t x_bytes = x == X_I8 ? 1 : type_bytes(type);
+    for (size_t b = 0; b < batch; b += most) {
+        W4Args& l = args[batch - b < most];
+        W4Plan& plan = plans[batch - b < most];
+        l.x = (const uint8_t*)a.x + b * (size_t)a.x_row * x_bytes;
+        if (x == X_I8) l.x_scales = a.x_scales + b * (size_t)a.x_groups;
+        l.out = (uint8_t*)out + b * out_row_stride * type_bytes(type);
+        switch (x) {
+            case X_F16: launch_w4<X_F16>(l, units, (int)p.units, plan, s); break;
+            case X_BF16: launch_w4<X_BF16>(l, units, (int)p.units, plan, s); break;
+            case X_F32: launch_w4<X_F32>(l, units, (int)p.units, plan, s); break;
+            default: launch_w4<X_I8>(l, units, (int)p.units, plan, s); break;
+        }
+        MIVI_HIP_CHECK(hipGetLastError());
+    }
+    return clear_error();
 }
 
 }  // namespace

@@ -376,9 +376,9 @@ int32_t mivi_hip_w4_pack(const uint8_t* codes, size_t codes_len, int32_t scale_t
                          size_t packed_len, size_t rows, size_t cols, size_t group, void* stream);
 
 /* out[batch][rows] = x[batch][cols] W^T, both in `type`. f16 and bf16 inputs
- * enter the products with all their bits, f32 ones with 22, any of them to no less
- * than 2^-40 of the largest magnitude of 128 columns; c - z enters exactly, sums
- * and scales are f32 (a group's sum of (c - z) x has to be an f32 number, a
+ * enter the products with all their bits (up to 16 bf16 ones to no less than 2^-39
+ * of the largest magnitude of 128 columns), f32 ones to 2^-23 of each, or to 2^-51
+ * of that largest; c - z enters exactly, sums and scales are f32 (a group's sum of (c - z) x has to be an f32 number, a
  * scale's magnitude below 2^100). The order of a row's sums, and so its last bits,
  * depends on the batch it is in. An infinity or NaN stays in its input's row. out
  * must not overlap x. */

@@ -281,12 +281,12 @@ __device__ __forceinline__ void store_tiles(const W4Args& a, const float* red, i
 // Up to 16 columns of the product. x lies whole in LDS, in operand order, and
 // tiles stream past it. f16 inputs stay as they are; bf16 and f32 ones are held
 // in fp16, each step's 128 columns multiplied by the power of two that takes
-// their largest to 2^14 .. 2^15 (f32 in two parts, 22 bits; nothing to less than
-// 2^-40 of that largest). Against 8-bit x the weights enter as codes and z sum x
-// comes off their sums, all whole numbers. (With codes as the fp16 numbers c
-// 2^-24, masks alone, one input takes up to 4 % less, but sums have 17 bits: the
-// matrix cores align products by their operands' exponents as if all were normal
-// numbers.)
+// their largest to 2^14 .. 2^15 (bf16 ones to no less than 2^-39 of that largest;
+// f32 ones in two parts: scaled_operands). Against 8-bit x the weights enter as
+// codes and z sum x comes off their sums, all whole numbers. (With codes as the fp16
+// numbers c 2^-24, masks alone, one input takes up to 4 % less, but sums have 17
+// bits: the matrix cores align products by their operands' exponents as if all were
+// normal numbers.)
 //
 // HBM and vector instructions bound it: one fp16 input over 65535 x 2048 in groups
 // of 64 with zeros 17.0 us, 4.3 TB/s, the vector pipe 57 % of the cycles; eight 8-bit
@@ -319,9 +319,15 @@ __device__ __forceinline__ float unit_sum(float v) {
 }
 
 // 8 columns of a bf16 or f32 input as fp16 operands, and what the step's results
-// are to be multiplied by. 16 lanes have a step.
+// are to be multiplied by. 16 lanes have a step. The first part of an f32 input
+// leaves at most 2^3; 2^12 times that, the second has its own 11 bits whatever the
+// input's size next to the step's largest (with one factor for both, an input 2^-24
+// of the largest kept 15 bits of 24). Both together are off by 2^-23 of the input (a
+// third part would take half as many columns again, and the sums' roundings add
+// more), or by the 2^-37 that a subnormal second part leaves: 2^-51 of the largest.
 template <int X>
-__device__ __forceinline__ void scaled_operands(const Raw<X>& r, Operand<X_F16> (&o)[parts_of(X)], float* factor) {
+__device__ __forceinline__ void scaled_operands(const Raw<X>& r, Operand<X_F16> (&o)[parts_of(X)],
+                                                float (&factor)[parts_of(X)]) {
     float v[8];
     uint32_t top = 0;
 #pragma unroll
@@ -333,14 +339,16 @@ __device__ __forceinline__ void scaled_operands(const Raw<X>& r, Operand<X_F16> 
     // biased exponents: 2^(14 - e) for a largest value of 2^e, 2^126 at most
     const int ex = min(127 + 14 - ((int)(max16(top) >> 23) - 127), 253);
     const float up = __uint_as_float((uint32_t)ex << 23);
-    *factor = __uint_as_float((uint32_t)(254 - ex) << 23);
+    factor[0] = __uint_as_float((uint32_t)(254 - ex) << 23);
+    if constexpr (X == X_F32) factor[1] = factor[0] * 0x1p-12f;
     half8 h[parts_of(X)];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         const float y = v[e] * up;
         h[0][e] = (_Float16)y;
         // what an infinity leaves is nothing
-        if constexpr (X == X_F32) h[1][e] = (_Float16)(__builtin_fabsf(y) == __builtin_inff() ? 0.f : y - (float)h[0][e]);
+        if constexpr (X == X_F32)
+            h[1][e] = (_Float16)(__builtin_fabsf(y) == __builtin_inff() ? 0.f : (y - (float)h[0][e]) * 0x1p12f);
     }
 #pragma unroll
     for (int p = 0; p < parts_of(X); p++) o[p].v = __builtin_bit_cast(u32x4, h[p]);
@@ -401,13 +409,13 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
                 }
             } else {
                 Operand<X_F16> o[PARTS];
-                float factor = 1.f;
+                float factor[PARTS];
                 if constexpr (X == X_F16) o[0].v = raw[e].v[0];
-                else scaled_operands<X>(raw[e], o, &factor);
+                else scaled_operands<X>(raw[e], o, factor);
 #pragma unroll
                 for (int p = 0; p < PARTS; p++) {
                     if (at[e] >= 0) *(Operand<X_F16>*)(to + p * XB) = o[p];
-                    if (X != X_F16 && at[e] >= 0 && (c & 15) == 0) factors[(c >> 4) * cols_x + b * PARTS + p] = factor;
+                    if (X != X_F16 && at[e] >= 0 && (c & 15) == 0) factors[(c >> 4) * cols_x + b * PARTS + p] = factor[p];
                 }
             }
         }
@@ -559,12 +567,12 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
                 if (ph >= full) blank<X>(&raw[e], (ph * a.wk * 16 + c8) * 8 < a.cols);
                 if constexpr (SCALED) {
                     Operand<X_F16> o[PARTS];
-                    float factor;
-                    scaled_operands<X>(raw[e], o, &factor);
+                    float factor[PARTS];
+                    scaled_operands<X>(raw[e], o, factor);
 #pragma unroll
                     for (int p = 0; p < PARTS; p++) {
                         *(Operand<X_F16>*)(to + c8 * pitch + ((b * PARTS + p) ^ (c8 & 15)) * XB) = o[p];
-                        if ((c8 & 15) == 0) ((float*)(to + xs_at))[(c8 >> 4) * cols_x + b * PARTS + p] = factor;
+                        if ((c8 & 15) == 0) ((float*)(to + xs_at))[(c8 >> 4) * cols_x + b * PARTS + p] = factor[p];
                     }
                 } else {
                     Operand<X> o;

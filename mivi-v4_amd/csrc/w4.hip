@@ -5,8 +5,8 @@
 // On the matrix cores, whatever the batch: c - z is a small integer and enters
 // them exactly, as fp16 (x in fp16, and in f32 as two fp16 parts, which take two
 // columns of the product), bf16 or int8 (8-bit x), 32 columns a product; a group's
-// sum is multiplied by its scale in f32 (8-bit x: an exact integer by the product
-// of both scales). Scaling the weights first would round every one of them.
+// sum is multiplied by its scale in f32 (8-bit x: an exact integer by the weights'
+// scale, then by the input's). Scaling the weights first would round every one of them.
 //
 // Packed layout (mivi_hip_w4_pack), tiles of 16 rows, steps of 128 columns,
 // padded with codes and scales of 0:
@@ -464,7 +464,9 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
                 if constexpr (I8) {
                     const int byte = i * W + u / per_w, z = (int)(c.zeros[byte / 4] >> (byte % 4 * 8) & 0xFF);
                     // (a product of 24 bits and the sum in one instruction)
-                    acc[i] = fmaf((float)(d[u][i] + __mul24(z, sum[u])), f[i] * m[u], acc[i]);
+                    // and the input's scale last: the scales' product alone may be no
+                    // normal number, or none at all where the sum is 0
+                    acc[i] = fmaf((float)(d[u][i] + __mul24(z, sum[u])) * f[i], m[u], acc[i]);
                 } else if constexpr (X == X_F16) {
                     acc[i] = fmaf(d[u][i], f[i], acc[i]);
                 } else {
@@ -642,7 +644,8 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             if constexpr (SCALED) part[n][i] = fmaf(d[n][i], f[i], part[n][i]);
-                            else acc[n][i] = fmaf((float)d[n][i], I8 ? f[i] * m : f[i], acc[n][i]);
+                            else if constexpr (I8) acc[n][i] = fmaf((float)d[n][i] * f[i], m, acc[n][i]);
+                            else acc[n][i] = fmaf(d[n][i], f[i], acc[n][i]);
                         }
                     }
                 }

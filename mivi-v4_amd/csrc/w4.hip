@@ -502,6 +502,15 @@ __global__ __launch_bounds__(WAVES * 64, 4) void w4_few_kernel(FewArgs g) {
 // of tiles' worth, so that neighbouring rows are in different banks.
 constexpr int rows_pitch(bool i8, int nt) { return i8 ? (nt | 1) * 128 : nt * 256; }
 
+// Whether w4_rows_kernel has a form of 16 waves for nt tiles of columns: where 128
+// registers hold it.
+constexpr bool rows_of_16(int x, int units, int nt) {
+    return nt >= 2 && nt <= 5 && (x != X_I8 || units * nt <= 6) && (x != X_F32 || units == 1 || nt < 5);
+}
+
+// And one of 8 tiles of columns, by 256 registers.
+constexpr bool rows_of_8(int x, int units) { return x != X_I8 || units < 4; }
+
 // More inputs, or deeper rows: NT tiles of 16 columns; x goes through LDS, wk
 // steps of it at a time, 8 columns of all inputs after another, loaded into
 // registers a phase ahead. 8 waves have two buffers and one barrier a phase; 16
@@ -511,6 +520,7 @@ constexpr int rows_pitch(bool i8, int nt) { return i8 ? (nt | 1) * 128 : nt * 25
 // product's results) 57 % of the cycles, the matrix cores 14 %, LDS 27 %.
 template <int X, int U, int W, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
+    static_assert(WAVES == 8 ? NT < 8 || rows_of_8(X, U) : rows_of_16(X, U, NT), "a form that no plan takes");
     constexpr int BUFFERS = WAVES == 8 ? 2 : 1, RING = WAVES == 8 ? kRing : 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr bool I8 = X == X_I8, SCALED = X == X_F32;
@@ -732,15 +742,6 @@ int32_t packed_of(size_t rows, size_t cols, size_t group, bool zeros, Packed* p)
     return MIVI_OK;
 }
 
-// Whether w4_rows_kernel has a form of 16 waves for nt tiles of columns: where 128
-// registers hold it.
-constexpr bool rows_of_16(int x, int units, int nt) {
-    return nt >= 2 && nt <= 5 && (x != X_I8 || units * nt <= 6) && (x != X_F32 || units == 1 || nt < 5);
-}
-
-// And one of 8 tiles of columns, by 256 registers.
-constexpr bool rows_of_8(int x, int units) { return x != X_I8 || units < 4; }
-
 // How a product is laid out: w4_few_kernel, or w4_rows_kernel with nt tiles of
 // columns.
 struct W4Plan {
@@ -767,7 +768,9 @@ void launch_rows(const W4Args& a, const W4Plan& p, hipStream_t s) {
         case 4: ROWS(4); break;
         case 5: ROWS(5); break;
         default:
-            if constexpr (rows_of_8(X, U)) ROWS(8);
+            if constexpr (rows_of_8(X, U)) {
+                ROWS(8);
+            }
             break;
     }
 #undef ROWS

@@ -38,8 +38,6 @@ typedef uint32_t u32_a1 __attribute__((aligned(1)));
 constexpr int kWaves = 8;
 constexpr int kStep = 128;   // columns of a step
 constexpr int kRing = 3;     // steps of a wave in flight (w4_rows_kernel)
-// pieces of x a thread stages at most
-constexpr int items_of(int x, int waves) { return (waves == 8 ? 8 : 5) / (x == 2 ? 2 : 1); }
 constexpr size_t kLds = 128 * 1024, kLdsFew = 156 * 1024;
 // inputs of a launch: in blocks of 8, the smallest, 2^15 of the 65535 that a grid's
 // second dimension may have
@@ -47,6 +45,8 @@ constexpr size_t kMostInputs = (size_t)1 << 18;
 
 enum XKind { X_F16, X_BF16, X_F32, X_I8 };
 constexpr int parts_of(int x) { return x == X_F32 ? 2 : 1; }  // columns of the product that an input takes
+// pieces of x a thread of w4_rows_kernel stages at most
+constexpr int items_of(int x, int waves) { return (waves == 8 ? 8 : 5) / parts_of(x); }
 
 struct W4Args {
     const uint8_t *codes, *scales, *zeros;  // planes of the packed weights (zeros: the codes where there are none)
@@ -57,7 +57,6 @@ struct W4Args {
     int rows, cols, batch, tiles, steps;
     int block;      // inputs of a workgroup
     int wk;         // waves of a tile
-    int w_units;    // units of a step that have a scale of their own
     int x_shift, x_groups;  // 8-bit x: log2 of a scale's columns, scales of a row; -1, 1: a row has one
     int bf16_scales, has_zeros, out_type;
 };
@@ -553,7 +552,7 @@ __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
 #pragma unroll
     for (int e = 0; e < ITEMS; e++) xp[e] = x_at<X>(a, b0 + min(bx + e * b_step, count - 1), 0);
     Raw<X> raw[ITEMS];
-    float xs_raw[2];  // 8-bit x: scales of (inputs x units); count wk <= 16 kItems WAVES / 4, so two a thread do
+    float xs_raw[2];  // 8-bit x: scales of (inputs x units): count wk <= 4 ITEMS WAVES and U <= 4, so two a thread do
     const int nu = a.wk * U;
     const auto load = [&](int ph) {
         if constexpr (X == X_I8) {
@@ -889,7 +888,7 @@ int32_t run_w4(W4Args a, int x, int32_t type, void* out, size_t out_len, size_t 
     a.out_row = (int64_t)out_row_stride, a.out_type = type;
     a.rows = (int)rows, a.cols = (int)cols;
     a.tiles = (int)p.tiles, a.steps = (int)p.steps;
-    a.w_units = (int)p.units, a.bf16_scales = scale_type == MIVI_GGML_BF16;
+    a.bf16_scales = scale_type == MIVI_GGML_BF16;
     // launches of `most` inputs, and one of those behind the last of them
     const size_t most = std::min(batch, kMostInputs), left = batch % most;
     W4Args args[2] = {a, a};

@@ -144,6 +144,8 @@ class W4Weights:
 def w4_matmul_rows(out, weights: W4Weights, x, x_scales=None, stream=None):
     """out[batch, rows] = x[batch, cols] W^T: x of out's type, or int8 codes with
     x_scales (f32 [batch, cols / group]) as rms_norm_q8 leaves them. Returns out."""
+    if _step is None:  # (weights may come from another process)
+        _load()
     _run(_step.w4_matmul_rows, weights.data, stream, out, *weights._args, x, x_scales)
     return out
 

@@ -20,7 +20,8 @@ def _load():
     global torch, _step, _raw_stream, _device
     torch = kv_q4._load()
     from . import _step as calls  # the checks and calls (csrc/step_calls.cpp)
-    _step, _raw_stream, _device = calls, torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+    _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+    _step = calls  # last: another thread takes it for the sign that all are there
 
 
 def _run(fn, of, stream, *args):

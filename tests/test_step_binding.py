@@ -33,3 +33,26 @@ def test_a_product_as_the_first_call():
         except ValueError as e:
             print(e)
     """) == "tensors are on a GPU"
+
+
+def test_a_thread_that_comes_between():
+    """Every entry point asks whether _step is there: while it is being loaded, no
+    moment shows it without what goes with it."""
+    assert fresh("""
+        import sys
+        import torch
+        from mivi_hip import step
+        seen = set()
+
+        def trace(frame, event, arg):
+            if frame.f_code is not step._load.__code__:
+                return None
+            frame.f_trace_opcodes = True
+            seen.add((step._step is not None, step._raw_stream is not None and step._device is not None
+                      and step.torch is not None))
+            return trace
+        sys.settrace(trace)
+        step._load()
+        sys.settrace(None)
+        print((False, False) in seen, (True, False) in seen, step._step is not None)
+    """) == "True False True"

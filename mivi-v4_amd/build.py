@@ -1,5 +1,5 @@
-"""Builds libmivi_hip.so (HIP kernels + C ABI) for gfx950, in-tree, and the
-Python binding of its step calls (_step.so).
+"""Builds libmivi_hip.so (HIP kernels + C ABI) for gfx950, in-tree, and, where
+torch can be imported, the Python binding of its step calls (_step.so).
 
     python mivi-v4_amd/build.py            # incremental
     python mivi-v4_amd/build.py --force    # rebuild everything
@@ -88,14 +88,23 @@ def build(force: bool = False) -> str:
 
 
 def _binding(force: bool) -> None:
-    """mivi_hip/_step.so: tensors to calls for the installed torch and Python."""
+    """mivi_hip/_step.so: tensors to calls for the installed torch and Python,
+    which a note beside the objects names."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        sys.stderr.write("no torch: mivi_hip/_step.so (the step calls for Python) is not built\n")
+        return
 
     src, out = os.path.join(CSRC, "step_calls.cpp"), os.path.join(HERE, "mivi_hip", "_step.so")
-    if not force and os.path.exists(out) and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in _deps(src)):
-        return
+    note, made_for = os.path.join(BUILD, "step_calls.for"), f"torch {torch.__version__}, Python {sys.version}\n"
+    if not force and os.path.exists(out) and os.path.exists(note) \
+            and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in _deps(src)):
+        with open(note) as f:
+            if f.read() == made_for:
+                return
     t = os.path.dirname(torch.__file__)
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I" + sysconfig.get_paths()["include"], "-isystem", os.path.join(t, "include"), src, "-o", out + ".tmp",
@@ -106,6 +115,8 @@ def _binding(force: bool) -> None:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("compile failed: step_calls.cpp")
     shutil.move(out + ".tmp", out)
+    with open(note, "w") as f:
+        f.write(made_for)
 
 
 if __name__ == "__main__":

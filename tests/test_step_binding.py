@@ -56,3 +56,58 @@ def test_a_thread_that_comes_between():
         sys.settrace(None)
         print((False, False) in seen, (True, False) in seen, step._step is not None)
     """) == "True False True"
+
+
+@pytest.fixture
+def build(tmp_path, monkeypatch):
+    """build.py with the compiler replaced: the commands that it would run."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("mivi_build", os.path.join(PKG, "build.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    commands = []
+
+    def run(cmd, **_):
+        commands.append(cmd)
+        with open(cmd[cmd.index("-o") + 1], "w"):
+            return subprocess.CompletedProcess(cmd, 0, "", "")
+    monkeypatch.setattr(m.subprocess, "run", run)
+    (tmp_path / "mivi_hip").mkdir()
+    for name, at in (("HERE", tmp_path), ("BUILD", tmp_path / "_build"), ("OUT", tmp_path / "mivi_hip" / "libmivi_hip.so")):
+        monkeypatch.setattr(m, name, str(at))
+    monkeypatch.setattr(m, "_deps", lambda src: [src])
+    m.commands = commands
+    return m
+
+
+def bindings(m):
+    n = sum(any(str(a).endswith("step_calls.cpp") for a in c) for c in m.commands)
+    m.commands.clear()
+    return n
+
+
+def test_a_build_without_torch(build, monkeypatch):
+    """The library is for hosts in any language: it is built, its Python binding is not."""
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert build.build() == build.OUT and os.path.exists(build.OUT)
+    assert bindings(build) == 0
+    assert not os.path.exists(os.path.join(os.path.dirname(build.OUT), "_step.so"))
+
+
+def test_a_build_for_another_torch(build, monkeypatch):
+    """The binding is built again where torch or Python changed, its source or not."""
+    import torch
+    build.build()
+    assert bindings(build) == 1
+    build.build()
+    assert bindings(build) == 0
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + ".next")
+    build.build()
+    assert bindings(build) == 1
+    build.build()
+    assert bindings(build) == 0
+    monkeypatch.setattr(sys, "version", "3.99 " + sys.version)
+    build.build()
+    assert bindings(build) == 1
+    build.build(force=True)
+    assert bindings(build) == 1

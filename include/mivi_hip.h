@@ -293,7 +293,9 @@ int32_t mivi_hip_kv_q4_attention(int32_t type, void* out, size_t out_len, size_t
  * tokens. No counterparts as calls in the reference. Tensors, `type`, strides,
  * starts, lens, streams and captures as for the 4-bit cache; nothing is
  * allocated. A tensor may be written over the one it is made from (same address
- * and strides); written tensors must not overlap anything else.
+ * and strides); written tensors must not overlap anything else. Sizes past what
+ * one launch counts (2^32 threads: some 4 million rows of a norm over 8192) are
+ * refused with MIVI_ERR_ARITHMETIC_OVERFLOW.
  * ------------------------------------------------------------------- */
 
 /* s = x + residual (residual may be NULL), out = s w / sqrt(mean s^2 + eps) over

@@ -288,8 +288,8 @@ __device__ __forceinline__ void store_tiles(const W4Args& a, const float* red, i
 // normal numbers.)
 //
 // HBM and vector instructions bound it: one fp16 input over 65535 x 2048 in groups
-// of 64 with zeros 17.0 us, 4.3 TB/s, the vector pipe 57 % of the cycles; eight 8-bit
-// ones over 28672 x 8192 26.4 us, 4.6 TB/s, 41 %; one f32 input over 8192 x 2048 5.9, a
+// of 64 with zeros 16.2 us, 4.5 TB/s, the vector pipe 57 % of the cycles; eight 8-bit
+// ones over 28672 x 8192 26.5 us, 4.6 TB/s, 41 %; one f32 input over 8192 x 2048 5.9, a
 // chain of x's load, its conversion, four steps and the join.
 constexpr int kFewRing = 4;  // steps of a wave in flight
 
@@ -515,8 +515,8 @@ constexpr bool rows_of_8(int x, int units) { return x != X_I8 || units < 4; }
 // registers a phase ahead. 8 waves have two buffers and one barrier a phase; 16
 // have one buffer and two barriers, but four waves a SIMD, whose loads from LDS,
 // products and sums overlap better. 80 bf16 inputs over 14336 x 4096 in groups of 32
-// with zeros: 27.8 us, 338 TFLOP/s; the vector pipe (conversion, a scale for every
-// product's results) 57 % of the cycles, the matrix cores 14 %, LDS 27 %.
+// with zeros: 28.1 us, 334 TFLOP/s; the vector pipe (conversion, a scale for every
+// product's results) 58 % of the cycles, the matrix cores 15 %, LDS 27 %.
 template <int X, int U, int W, int NT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void w4_rows_kernel(W4Args a) {
     static_assert(WAVES == 8 ? NT < 8 || rows_of_8(X, U) : rows_of_16(X, U, NT), "a form that no plan takes");
@@ -834,10 +834,14 @@ W4Plan w4_plan(W4Args* a, int x, int units, size_t batch, size_t tiles, size_t s
     // Blocks of inputs, waves of a workgroup and of a tile by an estimate. A phase
     // of 8 waves takes 1.2 us and 0.06 a tile of columns where a CU has one workgroup
     // (staging, products and the barrier in turn), 0.35 and 0.2 where two share it;
-    // of 16 waves, which have twice the steps, 1.35 and 0.28. (80 bf16 inputs, 14336 x
-    // 4096, groups of 32: one block and 16 waves 29.8 us, 8 waves 34.5, two blocks of
-    // 8 waves 52; 4096 x 14336, groups of 128: two blocks and 16 waves 30.6, one 34.0,
-    // of 8 waves 38 and 85. 512 inputs: blocks of 128 and 8 waves 124, of 74 138.)
+    // of 16 waves, which have twice the steps, 1.35 and 0.28. Measured, the first of each
+    // the estimate's choice: 80 bf16 inputs, 14336 x 4096, groups of 32: one block and 16
+    // waves 29.7 us, 8 waves 34.8, two blocks 38 and 48; 4096 x 14336, groups of 128: two
+    // blocks and 16 waves 33.0, 8 waves 41, one block 66 and 85; 512 inputs, 14336 x 4096:
+    // blocks of 128 and 8 waves 116, of 64 and 16 waves 114, of 74 and 16 waves 126; 80 f32
+    // ones: two blocks and 16 waves 45, 8 waves 54, four blocks 54 and more. (8-bit inputs
+    // take less than a phase is thought to: 80 over 8192 x 2048 two blocks of 8 waves 17.5,
+    // of 16 11.4; 512 over 14336 x 4096 blocks of 128 135, of 64 and 16 waves 109.)
     double best = 0;
     for (const int nt : {1, 2, 3, 4, 5, 8}) {
         if (nt == 8 && !rows_of_8(x, units)) break;

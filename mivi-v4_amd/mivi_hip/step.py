@@ -4,7 +4,8 @@ own layers: `rms_norm`, `rms_norm_q8`, `rope` (with `rope_frequencies`),
 include/mivi_hip.h, the mivi_hip_* calls of the same names).
 
 Tensors are GPU tensors of one device; work is enqueued on `stream`, or on the
-device's current one.
+device's current one. A tensor used on another stream than its own (a W4Weights
+too) is the caller's to keep until that work is done.
 """
 from __future__ import annotations
 
